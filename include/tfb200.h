@@ -50,9 +50,10 @@ enum tfb200_status {
   TFB200_ENOSPC = -6        /* output buffer (text) too small */
 };
 
-enum tfb200_dtype { TFB200_BF16 = 0, TFB200_F32 = 1 };
+enum tfb200_dtype { TFB200_BF16 = 0, TFB200_F32 = 1, TFB200_I8 = 2 };
 
-enum tfb200_gelu { TFB200_GELU_ERF = 0, TFB200_GELU_TANH = 1 };
+/* TFB200_GELU_NONE is for the calls that say so. */
+enum tfb200_gelu { TFB200_GELU_ERF = 0, TFB200_GELU_TANH = 1, TFB200_GELU_NONE = 2 };
 
 /* A row-major matrix view: data[r * ld + c], r < rows, c < cols. */
 typedef struct tfb200_mat {
@@ -60,7 +61,7 @@ typedef struct tfb200_mat {
   int64_t rows;
   int64_t cols;
   int64_t ld;
-  int32_t dtype; /* enum tfb200_dtype; the kernels take TFB200_BF16 */
+  int32_t dtype; /* enum tfb200_dtype; TFB200_BF16 unless the call says otherwise */
 } tfb200_mat;
 
 /* ABI version (TFB200_ABI_VERSION of the built library). */
@@ -205,6 +206,66 @@ int tfb200_residual_add(const float* partial, int64_t ld_partial, const tfb200_m
 int tfb200_fused_mlp_noalloc(const tfb200_mat* x, const void* gamma, const tfb200_mat* w1, const void* b1,
                              const tfb200_mat* w2, const tfb200_mat* residual, float eps, int gelu_mode,
                              tfb200_mat* y, void* stream);
+
+/* ---- 8-bit integer weights and activations ------------------------------
+ * int8 matrices (TFB200_I8) stand for q * scale with one fp32 scale per row: a
+ * row is a token of an activation and an output channel of a weight, so weights
+ * are held as [out, in], both operands of a product running along the inner
+ * dimension. q is symmetric, -127 .. 127 (products accept -128 as well). Any
+ * leading dimension and alignment is accepted; products are fast when both int8
+ * operands start on 16-byte boundaries with leading dimensions % 16 == 0. Only
+ * the `cols` columns of a row are read or written. The scales are contiguous
+ * device arrays. The reference has no integer path; the fused calls are the
+ * 8-bit forms of golden.fused_rmsnorm_matmul and golden.fused_mlp
+ * (golden.py:97-122).
+ *
+ * A row that holds an infinity or a NaN gets scale NaN (and q = 0), so every
+ * value computed from it is NaN; the other rows are not touched by it. A row of
+ * zeros gets scale 0. RMSNorm's sum of squares is held in fp32: a row where it
+ * overflows (values above about 1e18) counts as not finite. */
+
+/* q[m,k] = rn(x[m,k] * 127 / amax), scale[m] = amax / 127, amax = max_k |x[m,k]|,
+ * rounding half to even. X [M,K] bf16, Q [M,K] int8, scale [M]. Also lays out
+ * weights: the rows of W^T are its output channels. */
+int tfb200_quantize_int8(const tfb200_mat* x, tfb200_mat* q, float* scale, void* stream);
+
+/* The same of t = rmsnorm(S, gamma, eps), S = X, or S = X + R when `residual` is
+ * given, in which case `sum` receives bf16(S) (it may be X or R; otherwise it is
+ * NULL). The norm and q are taken from the unrounded S. X, R, sum [M,K] bf16,
+ * gamma [K] bf16, Q [M,K] int8, scale [M]. */
+int tfb200_rmsnorm_int8(const tfb200_mat* x, const tfb200_mat* residual, const void* gamma, float eps,
+                        tfb200_mat* sum, tfb200_mat* q, float* scale, void* stream);
+
+/* C[m,n] = gelu(a_scale[m] * b_scale[n] * sum_k A[m,k] B[n,k] + bias[n]) + R[m,n].
+ * A [M,K] and B [N,K] int8, a_scale [M], b_scale [N], bias [N] bf16 or NULL,
+ * gelu_mode any of enum tfb200_gelu, residual [M,N] bf16 or NULL, C [M,N] bf16 or
+ * fp32. The sums are exact in int32, which bounds K to 131071
+ * (TFB200_EUNSUPPORTED above); scales, bias, GELU and residual are applied in
+ * fp32 and rounded once. K == 0 gives gelu(bias) + R. Equal calls give equal
+ * bits. workspace: tfb200_matmul_int8_workspace_size bytes, 256-byte aligned. */
+size_t tfb200_matmul_int8_workspace_size(int64_t m, int64_t k, int64_t n);
+int tfb200_matmul_int8(const tfb200_mat* a, const float* a_scale, const tfb200_mat* b, const float* b_scale,
+                       const void* bias, int gelu_mode, const tfb200_mat* residual, tfb200_mat* c, void* stream,
+                       void* workspace, size_t workspace_bytes);
+
+/* Y = rmsnorm_int8(X, gamma, eps) @ W^T with int8 W [N,K] and w_scale [N]:
+ * tfb200_rmsnorm_int8, then tfb200_matmul_int8, with the int8 rows in `workspace`
+ * (tfb200_fused_rmsnorm_matmul_int8_workspace_size bytes, 256-byte aligned). */
+size_t tfb200_fused_rmsnorm_matmul_int8_workspace_size(int64_t m, int64_t k, int64_t n);
+int tfb200_fused_rmsnorm_matmul_int8(const tfb200_mat* x, const void* gamma, const tfb200_mat* w,
+                                     const float* w_scale, float eps, tfb200_mat* y, void* stream, void* workspace,
+                                     size_t workspace_bytes);
+
+/* Y = quantize(gelu(rmsnorm_int8(X) @ W1^T + b1)) @ W2^T + R, the hidden block
+ * quantised per token. W1 [H,K], w1_scale [H], b1 [H] bf16 or NULL, W2 [N,H],
+ * w2_scale [N], R [M,N] (may be X when N == K), Y [M,N] bf16; K and H at most
+ * 131071. workspace: tfb200_fused_mlp_int8_workspace_size bytes, 256-byte
+ * aligned. */
+size_t tfb200_fused_mlp_int8_workspace_size(int64_t m, int64_t k, int64_t h, int64_t n);
+int tfb200_fused_mlp_int8(const tfb200_mat* x, const void* gamma, const tfb200_mat* w1, const float* w1_scale,
+                          const void* b1, const tfb200_mat* w2, const float* w2_scale, const tfb200_mat* residual,
+                          float eps, int gelu_mode, tfb200_mat* y, void* stream, void* workspace,
+                          size_t workspace_bytes);
 
 /* The tensixflow front end of this backend on IR text: parse the dialect
  * subset of the fused path, apply `args` in order (the tensixflow-opt flags

@@ -1,0 +1,87 @@
+// Host-side interfaces of the 8-bit integer path: row quantisation, RMSNorm
+// with an int8 result, and the int8 matrix product. Shared by int8_*.cu.
+#pragma once
+
+#include "internal.h"
+
+namespace tfb200 {
+
+// What a product's epilogue writes: bf16 or fp32 for the caller, or the fused
+// MLP's hidden block, fp16 of h * hidden_factor(row) (int8_math.cuh).
+enum Int8Out : int { kInt8OutBf16 = 0, kInt8OutF32 = 1, kInt8OutHidden = 2 };
+
+// Longest inner dimension: |sum_k a b| <= 128 * 128 * K must stay in int32.
+constexpr int64_t kInt8MaxK = 131071;
+
+// v = a_scale[m] * b_scale[n] * sum_k A[m,k] B[n,k], then + bias[n], GELU and
+// + residual[m,n] (each optional). A [M,K] and B [N,K] are int8, row-major.
+struct Int8Gemm {
+  int64_t M = 0, N = 0, K = 0;
+  const int8_t* A = nullptr;
+  int64_t lda = 0;
+  const int8_t* B = nullptr;
+  int64_t ldb = 0;
+  const float* a_scale = nullptr;
+  const float* b_scale = nullptr;
+  const bf16* bias = nullptr;
+  int gelu = kGeluNone;
+  const bf16* residual = nullptr;
+  int64_t ldr = 0;
+  void* C = nullptr;
+  int64_t ldc = 0;
+  int out = kInt8OutBf16;
+  const float* bound = nullptr;  // kInt8OutHidden: {max |b_scale|, max |bias|}
+  void* ws = nullptr;            // int8_gemm_ws(M, N, K).total bytes, 256-byte aligned, its counters cleared
+  // The kernel that precedes this product in the stream writes neither B nor
+  // b_scale (it is this library's own staging launch), so their first tiles may
+  // be requested before it has completed.
+  bool b_stable = false;
+};
+
+// Device workspace of one product: `clear_bytes` of counters, zero on entry,
+// then its partial-sum slots.
+struct Int8GemmWs {
+  size_t clear_bytes = 0, total = 0;
+};
+Int8GemmWs int8_gemm_ws(int64_t m, int64_t n, int64_t k);
+int run_int8_gemm(const Int8Gemm& g, cudaStream_t stream, std::string* err);
+
+// One row at a time: q = rn(t * 127 / amax_k |t|) with t = x (kInt8RowsQuant),
+// t = (x + residual) * gamma with scale = amax / (127 rms) (kInt8RowsNorm), or
+// t = the fused MLP's fp16 hidden block (kInt8RowsHidden).
+enum Int8RowsKind : int { kInt8RowsQuant = 0, kInt8RowsNorm = 1, kInt8RowsHidden = 2 };
+struct Int8Rows {
+  int kind = kInt8RowsQuant;
+  int64_t M = 0, K = 0;
+  const void* x = nullptr;
+  int64_t ldx = 0;
+  const bf16* residual = nullptr;  // kInt8RowsNorm, optional
+  int64_t ldr = 0;
+  const bf16* gamma = nullptr;
+  float eps = 0.0f;
+  bf16* sum = nullptr;  // bf16(x + residual), with a residual
+  int64_t lds = 0;
+  int8_t* q = nullptr;
+  int64_t ldq = 0;
+  float* scale = nullptr;
+  // kInt8RowsHidden: the inner dimension and row scales of the product that
+  // wrote the block, and its bound.
+  int64_t up_k = 0;
+  const float* up_scale = nullptr;
+  const float* bound = nullptr;
+  // Optional: the bound of a product that follows, {max |b_scale|, max |bias|}
+  // over bound_n columns, written to bound_out by one more CTA.
+  const float* b_scale = nullptr;
+  const bf16* bias = nullptr;
+  int64_t bound_n = 0;
+  float* bound_out = nullptr;
+  // Optional: counters of the products that follow, cleared by the same launch
+  // (16-byte aligned, a multiple of 16 bytes).
+  void* zero = nullptr;
+  size_t zero_bytes = 0;
+};
+// Clears `bytes` (16-byte aligned, a multiple of 16) ahead of a bare product.
+int run_int8_clear(void* p, size_t bytes, cudaStream_t stream, std::string* err);
+int run_int8_rows(const Int8Rows& r, cudaStream_t stream, std::string* err);
+
+}  // namespace tfb200

@@ -1,0 +1,419 @@
+// Rows to int8: symmetric quantisation with one scale per row, alone
+// (tfb200_quantize_int8), behind RMSNorm and the residual's addition
+// (tfb200_rmsnorm_int8), and of the fused MLP's hidden block.
+//
+//   t = x                    scale = amax / 127
+//   t = (x + r) * gamma      scale = amax / 127 * 1 / sqrt(mean_k (x + r)^2 + eps)
+//   q = rn(t * (127 / amax)),  amax = max_k |t|
+//
+// The row's 1 / rms multiplies every t alike, so it cancels in t / amax and q
+// does not depend on it: the rounding to int8 acts on t itself, and 1 / rms only
+// enters the scale. A row of zeros gives q = 0 and scale 0. A row that holds an
+// infinity or a NaN (or whose sum of squares leaves fp32) gives q = 0 and scale
+// NaN, so everything computed from it is NaN.
+//
+// HBM-bound: 2K bytes read and K written per row (4K and 3K with a residual).
+// A row's T threads hold it in registers, kPer values each, so that it is read
+// once and all its loads are in flight together; T is the smallest block that
+// holds the row. Rows up to 1024 values take one warp and four rows a block.
+#include <algorithm>
+
+#include "int8_math.cuh"
+
+namespace tfb200 {
+
+namespace {
+
+constexpr int kPer = 32;       // values per thread
+constexpr int kMaxRow = 1024 * kPer;
+
+struct RowsParams {
+  int M, K;
+  const void* x;
+  int64_t ldx;
+  const bf16* residual;
+  int64_t ldr;
+  const bf16* gamma;
+  float eps;
+  bf16* sum;
+  int64_t lds;
+  int8_t* q;
+  int64_t ldq;
+  float* scale;
+  int up_k;
+  const float* up_scale;
+  const float* bound;
+  const float* b_scale;
+  const bf16* bias;
+  int64_t bound_n;
+  float* bound_out;
+  int row_blocks;  // the block after them computes bound_out
+  uint4* zero;
+  int64_t zero_vecs;
+};
+
+// Counters of the products that follow, cleared by all threads of the grid.
+__device__ __forceinline__ void clear_words(uint4* zero, int64_t n) {
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * blockDim.x;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < n; i += stride)
+    zero[i] = make_uint4(0u, 0u, 0u, 0u);
+}
+
+__global__ void __launch_bounds__(256) k_int8_clear(uint4* zero, int64_t n) {
+  grid_dep_wait();
+  grid_dep_launch();
+  clear_words(zero, n);
+}
+
+template <int KIND>
+__device__ __forceinline__ float in_value(uint16_t bits) {
+  if (KIND == kInt8RowsHidden) return __half2float(__ushort_as_half(bits));
+  return __uint_as_float(static_cast<uint32_t>(bits) << 16);
+}
+
+// Largest |value| as its bits: unsigned order puts infinities and NaN on top.
+__device__ __forceinline__ uint32_t mag(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+
+struct RowStat {
+  float ss;
+  uint32_t amax;
+};
+
+__device__ __forceinline__ RowStat warp_stat(RowStat s, bool squares) {
+  if (squares) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s.ss += __shfl_xor_sync(0xffffffffu, s.ss, o);
+  }
+  s.amax = __reduce_max_sync(0xffffffffu, s.amax);
+  return s;
+}
+
+// The statistics over the block's threads (one row per block).
+__device__ __forceinline__ RowStat block_stat(RowStat s, bool squares) {
+  __shared__ float part_ss[32];
+  __shared__ uint32_t part_max[32];
+  s = warp_stat(s, squares);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  if (lane == 0) {
+    part_ss[warp] = s.ss;
+    part_max[warp] = s.amax;
+  }
+  __syncthreads();
+  s.ss = lane < warps ? part_ss[lane] : 0.0f;
+  s.amax = lane < warps ? part_max[lane] : 0u;
+  return warp_stat(s, squares);
+}
+
+struct RowScale {
+  float up, r, scale;  // q = rn(t * up * r)
+};
+
+template <int KIND>
+__device__ __forceinline__ RowScale row_scale(const RowsParams& p, int64_t row, RowStat s) {
+  RowScale o;
+  const float amax = __uint_as_float(s.amax);
+  // 127 / amax leaves fp32 for the smallest values: those rows are taken up by
+  // a power of two first (exact).
+  o.up = amax < 1e-30f ? 7.9228163e28f : 1.0f;
+  bool bad = s.amax >= 0x7F800000u;
+  if (KIND == kInt8RowsNorm) {
+    bad = bad || !(s.ss <= 3.402823466e38f);
+    o.scale = amax * (1.0f / sqrtf(s.ss / static_cast<float>(p.K) + p.eps) / 127.0f);
+  } else if (KIND == kInt8RowsHidden) {
+    o.scale = amax / 127.0f / hidden_factor(p.up_k, p.up_scale[row], p.bound);
+  } else {
+    o.scale = amax / 127.0f;
+  }
+  o.r = s.amax == 0u || bad ? 0.0f : 127.0f / (amax * o.up);
+  if (bad) {
+    o.up = 0.0f;
+    o.scale = __uint_as_float(0x7FC00000u);
+  }
+  return o;
+}
+
+// rn(v) for |v| <= 127 in the low byte: adding 1.5 * 2^23 leaves the integer,
+// rounded half to even, in the low bits (a conversion instruction runs at a
+// quarter of the add's rate).
+__device__ __forceinline__ uint32_t q_bits(float t, const RowScale& s) {
+  return __float_as_uint(__fadd_rn(__fmul_rn(__fmul_rn(t, s.up), s.r), 12582912.0f));
+}
+__device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+
+// The bound of the product that follows, by one block.
+__device__ void bound_block(const RowsParams& p) {
+  float s = 0.0f, b = 0.0f;
+  for (int64_t n = threadIdx.x; n < p.bound_n; n += blockDim.x) {
+    s = fmaxf(s, fabsf(p.b_scale[n]));
+    if (p.bias) b = fmaxf(b, fabsf(__bfloat162float(p.bias[n])));
+  }
+  const uint32_t smax = block_stat({0.0f, mag(s)}, false).amax;
+  __syncthreads();
+  const uint32_t bmax = block_stat({0.0f, mag(b)}, false).amax;
+  if (threadIdx.x == 0) {
+    p.bound_out[0] = __uint_as_float(smax);
+    p.bound_out[1] = __uint_as_float(bmax);
+  }
+}
+
+// VEC: rows start on 16-byte boundaries (8 for q); a thread takes 8 neighbouring
+// values at a time. Otherwise a thread takes single values, T apart.
+// WARP: a warp per row (T = 32), else a block per row (T = blockDim.x).
+// The row stays in registers as its 16-bit values, two a word, and is widened
+// again for the second pass: held as fp32 it spilled at 1024 threads.
+template <int KIND, bool RES, bool VEC, bool WARP>
+__global__ void __launch_bounds__(WARP ? 128 : 1024) k_int8_rows(const RowsParams p) {
+  // Launched with programmatic serialization: wait for the grid before (it may
+  // write x or still read q), then let the next grid start its prologue.
+  grid_dep_wait();
+  grid_dep_launch();
+  clear_words(p.zero, p.zero_vecs);
+  if (static_cast<int>(blockIdx.x) >= p.row_blocks) {
+    bound_block(p);
+    return;
+  }
+  const int T = WARP ? 32 : blockDim.x;
+  const int t = WARP ? threadIdx.x & 31 : threadIdx.x;
+  const int64_t row = WARP ? static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5) : blockIdx.x;
+  if (WARP && row >= p.M) return;
+  const uint16_t* x = static_cast<const uint16_t*>(p.x) + row * p.ldx;
+  const uint16_t* r = RES ? reinterpret_cast<const uint16_t*>(p.residual) + row * p.ldr : nullptr;
+  const uint16_t* g = reinterpret_cast<const uint16_t*>(p.gamma);
+  const int K = p.K;
+  // First of the 8 values of group i, and the distance between them.
+  constexpr int G = kPer / 8;
+  const int step = VEC ? 1 : T;
+  auto first = [&](int i) { return VEC ? (t + i * T) * 8 : t + i * 8 * T; };
+
+  // Plain loads: the sum may be written over x or the residual.
+  auto load8 = [&](const uint16_t* src, int k, uint32_t (&w)[4]) {
+    if (VEC && k + 8 <= K) {
+      const uint4 v = *reinterpret_cast<const uint4*>(src + k);
+      w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int k0 = k + 2 * j * step, k1 = k0 + step;
+        const uint32_t lo = k0 < K ? src[k0] : 0u, hi = k1 < K ? src[k1] : 0u;
+        w[j] = lo | hi << 16;
+      }
+    }
+  };
+  uint32_t xw[G][4], rw[RES ? G : 1][4];
+#pragma unroll
+  for (int i = 0; i < G; ++i) {
+    load8(x, first(i), xw[i]);
+    if (RES) load8(r, first(i), rw[i]);
+  }
+  auto half16 = [](const uint32_t (&w)[4], int j) { return static_cast<uint16_t>(w[j >> 1] >> (16 * (j & 1))); };
+  // The 8 values t of group i; with STAT also their statistics and the sum.
+  RowStat st{0.0f, 0u};
+  auto group = [&](int i, bool stat, float (&v)[8]) {
+    const int k = first(i);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      v[j] = in_value<KIND>(half16(xw[i], j));
+      if (RES) v[j] = __fadd_rn(v[j], in_value<kInt8RowsQuant>(half16(rw[RES ? i : 0], j)));
+    }
+    if (KIND == kInt8RowsNorm) {
+      if (stat) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) st.ss = fmaf(v[j], v[j], st.ss);
+        if (RES) {
+          bf16* sum = p.sum + row * p.lds;
+          if (VEC && k + 8 <= K) {
+            *reinterpret_cast<uint4*>(sum + k) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]),
+                                                            pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (k + j * step < K) sum[k + j * step] = __float2bfloat16_rn(v[j]);
+          }
+        }
+      }
+      if (VEC && k + 8 <= K) {
+        const uint4 gv = __ldg(reinterpret_cast<const uint4*>(g + k));
+        const uint32_t gw[4] = {gv.x, gv.y, gv.z, gv.w};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = __fmul_rn(v[j], in_value<kInt8RowsQuant>(half16(gw, j)));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (k + j * step < K) v[j] = __fmul_rn(v[j], in_value<kInt8RowsQuant>(__ldg(g + k + j * step)));
+      }
+    }
+    if (stat) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) st.amax = max(st.amax, mag(v[j]));
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < G; ++i) {
+    float v[8];
+    if (first(i) < K) group(i, true, v);
+  }
+  st = WARP ? warp_stat(st, KIND == kInt8RowsNorm) : block_stat(st, KIND == kInt8RowsNorm);
+  const RowScale sc = row_scale<KIND>(p, row, st);
+  if (t == 0) p.scale[row] = sc.scale;
+  int8_t* q = p.q + row * p.ldq;
+  const bool zero = sc.r == 0.0f;  // a row of zeros, or one that is not finite
+#pragma unroll
+  for (int i = 0; i < G; ++i) {
+    const int k = first(i);
+    if (k >= K) break;
+    float v[8];
+    group(i, false, v);
+    uint32_t b[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) b[j] = zero ? 0u : q_bits(v[j], sc);
+    if (VEC && k + 8 <= K) {
+      *reinterpret_cast<uint2*>(q + k) = make_uint2(pack4(b[0], b[1], b[2], b[3]), pack4(b[4], b[5], b[6], b[7]));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (k + j * step < K) q[k + j * step] = static_cast<int8_t>(b[j] & 0xFFu);
+    }
+  }
+}
+
+// Rows longer than the registers of a block: the row is read twice, the second
+// time mostly from L2.
+template <int KIND, bool RES>
+__global__ void __launch_bounds__(1024) k_int8_rows_long(const RowsParams p) {
+  grid_dep_wait();
+  grid_dep_launch();
+  clear_words(p.zero, p.zero_vecs);
+  if (static_cast<int>(blockIdx.x) >= p.row_blocks) {
+    bound_block(p);
+    return;
+  }
+  const int64_t row = blockIdx.x;
+  const uint16_t* x = static_cast<const uint16_t*>(p.x) + row * p.ldx;
+  const uint16_t* r = RES ? reinterpret_cast<const uint16_t*>(p.residual) + row * p.ldr : nullptr;
+  const uint16_t* g = reinterpret_cast<const uint16_t*>(p.gamma);
+  auto value = [&](int k) {
+    float s = in_value<KIND>(x[k]);
+    if (RES) s = __fadd_rn(s, in_value<kInt8RowsQuant>(r[k]));
+    return s;
+  };
+  RowStat st{0.0f, 0u};
+#pragma unroll 4
+  for (int k = threadIdx.x; k < p.K; k += blockDim.x) {
+    float s = value(k);
+    if (KIND == kInt8RowsNorm) {
+      st.ss = fmaf(s, s, st.ss);
+      s = __fmul_rn(s, in_value<kInt8RowsQuant>(g[k]));
+    }
+    st.amax = max(st.amax, mag(s));
+  }
+  st = block_stat(st, KIND == kInt8RowsNorm);
+  const RowScale sc = row_scale<KIND>(p, row, st);
+  if (threadIdx.x == 0) p.scale[row] = sc.scale;
+  const bool zero = sc.r == 0.0f;
+  // A thread reads a value of x again before it writes the sum, which may be x.
+#pragma unroll 4
+  for (int k = threadIdx.x; k < p.K; k += blockDim.x) {
+    float s = value(k);
+    if (RES) p.sum[row * p.lds + k] = __float2bfloat16_rn(s);
+    if (KIND == kInt8RowsNorm) s = __fmul_rn(s, in_value<kInt8RowsQuant>(g[k]));
+    p.q[row * p.ldq + k] = zero ? 0 : static_cast<int8_t>(q_bits(s, sc) & 0xFFu);
+  }
+}
+
+template <int KIND, bool RES>
+cudaError_t launch_rows(RowsParams& p, bool vec, cudaStream_t s) {
+  const bool warp = p.K <= 32 * kPer;
+  int T = 128;
+  while (!warp && T < 1024 && T * kPer < p.K) T *= 2;
+  if (p.K > kMaxRow) T = 1024;
+  p.row_blocks = warp ? (p.M + 3) / 4 : p.M;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(p.row_blocks) + (p.bound_out ? 1u : 0u), 1, 1);
+  cfg.blockDim = dim3(static_cast<unsigned>(T), 1, 1);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = p.K > kMaxRow ? cudaLaunchKernelEx(&cfg, k_int8_rows_long<KIND, RES>, p)
+                  : warp ? (vec ? cudaLaunchKernelEx(&cfg, k_int8_rows<KIND, RES, true, true>, p)
+                                : cudaLaunchKernelEx(&cfg, k_int8_rows<KIND, RES, false, true>, p))
+                         : (vec ? cudaLaunchKernelEx(&cfg, k_int8_rows<KIND, RES, true, false>, p)
+                                : cudaLaunchKernelEx(&cfg, k_int8_rows<KIND, RES, false, false>, p));
+  return e == cudaSuccess ? cudaGetLastError() : e;
+}
+
+bool al(const void* p, unsigned b) { return (reinterpret_cast<uintptr_t>(p) & (b - 1)) == 0; }
+
+}  // namespace
+
+int run_int8_clear(void* ptr, size_t bytes, cudaStream_t stream, std::string* err) {
+  const int64_t n = static_cast<int64_t>(bytes / 16);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>((n + 255) / 256, 148)), 1, 1);
+  cfg.blockDim = dim3(256, 1, 1);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, k_int8_clear, static_cast<uint4*>(ptr), n);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (e != cudaSuccess) {
+    *err = std::string("counter clear launch: ") + cudaGetErrorString(e);
+    return -3;
+  }
+  count_launch();
+  return 0;
+}
+
+int run_int8_rows(const Int8Rows& r, cudaStream_t stream, std::string* err) {
+  if (r.M > (int64_t(1) << 30) || r.K > (int64_t(1) << 30)) {
+    *err = "dimension too large";
+    return -2;
+  }
+  RowsParams p{};
+  p.M = static_cast<int>(r.M);
+  p.K = static_cast<int>(r.K);
+  p.x = r.x;
+  p.ldx = r.ldx;
+  p.residual = r.residual;
+  p.ldr = r.ldr;
+  p.gamma = r.gamma;
+  p.eps = r.eps;
+  p.sum = r.sum;
+  p.lds = r.lds;
+  p.q = r.q;
+  p.ldq = r.ldq;
+  p.scale = r.scale;
+  p.up_k = static_cast<int>(r.up_k);
+  p.up_scale = r.up_scale;
+  p.bound = r.bound;
+  p.b_scale = r.b_scale;
+  p.bias = r.bias;
+  p.bound_n = r.bound_n;
+  p.bound_out = r.bound_out;
+  p.zero = static_cast<uint4*>(r.zero);
+  p.zero_vecs = static_cast<int64_t>(r.zero_bytes / 16);
+  const bool norm = r.kind == kInt8RowsNorm, res = norm && r.residual;
+  // One row alone has no stride to keep aligned.
+  auto rows_ok = [&](const void* b, int64_t ld) { return al(b, 16) && (ld % 8 == 0 || r.M == 1); };
+  const bool vec = rows_ok(r.x, r.ldx) && al(r.q, 8) && (r.ldq % 8 == 0 || r.M == 1) && (!norm || al(r.gamma, 16)) &&
+                   (!res || (rows_ok(r.residual, r.ldr) && rows_ok(r.sum, r.lds)));
+  const cudaError_t e = r.kind == kInt8RowsHidden ? launch_rows<kInt8RowsHidden, false>(p, vec, stream)
+                        : !norm                   ? launch_rows<kInt8RowsQuant, false>(p, vec, stream)
+                        : res                     ? launch_rows<kInt8RowsNorm, true>(p, vec, stream)
+                                                  : launch_rows<kInt8RowsNorm, false>(p, vec, stream);
+  if (e != cudaSuccess) {
+    *err = std::string("int8 rows launch: ") + cudaGetErrorString(e);
+    return -3;
+  }
+  count_launch();
+  return 0;
+}
+
+}  // namespace tfb200

@@ -23,8 +23,10 @@ TFB200_EWORKSPACE = -5
 TFB200_ENOSPC = -6
 TFB200_BF16 = 0
 TFB200_F32 = 1
+TFB200_I8 = 2
 TFB200_GELU_ERF = 0
 TFB200_GELU_TANH = 1
+TFB200_GELU_NONE = 2
 TFB200_NOALLOC_SCRATCH_BYTES = 8 * 1024 * 1024
 
 # Every symbol include/tfb200.h declares (checked by tests/test_abi.py).
@@ -46,6 +48,14 @@ EXPORTS = (
     "tfb200_ipc_open",
     "tfb200_ipc_close",
     "tfb200_residual_add",
+    "tfb200_quantize_int8",
+    "tfb200_rmsnorm_int8",
+    "tfb200_matmul_int8_workspace_size",
+    "tfb200_matmul_int8",
+    "tfb200_fused_rmsnorm_matmul_int8_workspace_size",
+    "tfb200_fused_rmsnorm_matmul_int8",
+    "tfb200_fused_mlp_int8_workspace_size",
+    "tfb200_fused_mlp_int8",
     "tfb200_device_status",
     "tfb200_clear_device_status",
     "tfb200_opt",
@@ -114,6 +124,14 @@ def lib() -> ctypes.CDLL:
         "tfb200_ipc_get": ([vp, vp, ctypes.POINTER(ctypes.c_size_t)], i32),
         "tfb200_ipc_open": ([vp, ctypes.POINTER(ctypes.c_void_p)], i32),
         "tfb200_ipc_close": ([vp], i32),
+        "tfb200_quantize_int8": ([P, P, vp, vp], i32),
+        "tfb200_rmsnorm_int8": ([P, P, vp, f32, P, P, vp, vp], i32),
+        "tfb200_matmul_int8_workspace_size": ([ctypes.c_int64] * 3, sz),
+        "tfb200_matmul_int8": ([P, vp, P, vp, vp, i32, P, P, vp, vp, sz], i32),
+        "tfb200_fused_rmsnorm_matmul_int8_workspace_size": ([ctypes.c_int64] * 3, sz),
+        "tfb200_fused_rmsnorm_matmul_int8": ([P, vp, P, vp, f32, P, vp, vp, sz], i32),
+        "tfb200_fused_mlp_int8_workspace_size": ([ctypes.c_int64] * 4, sz),
+        "tfb200_fused_mlp_int8": ([P, vp, P, vp, vp, P, vp, P, f32, i32, P, vp, vp, sz], i32),
         "tfb200_device_status": ([], i32),
         "tfb200_clear_device_status": ([], i32),
         "tfb200_opt": ([ctypes.c_char_p, ctypes.c_char_p, vp, sz, ctypes.POINTER(ctypes.c_size_t)], i32),
