@@ -10,7 +10,7 @@ R = ctypes.byref
 
 
 def mat(rows, cols, dtype, ld=None, data=4096):
-    return L.Mat(data, rows, cols, cols if ld is None else ld, dtype)
+    return L.Mat(data, rows, cols, max(cols, 1) if ld is None else ld, dtype)
 
 
 @pytest.fixture(scope="module")

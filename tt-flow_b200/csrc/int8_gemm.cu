@@ -1,7 +1,22 @@
 // The int8 matrix product C = epi(A @ B^T): A [M,K] tokens, B [N,K] channels,
 // both running along K, int32 sums (exact up to K = 131071), one fp32 scale per
 // token and per channel applied to the finished sum.
+//
+// k_int8_pair: the tensor-core kernel, persistent over 256 x 256 output tiles,
+// one tile per pair of CTAs (tcgen05.mma.cta_group::2.kind::i8, 256 x 256 x 32).
+// Both operands run along k, so a stage is 128 rows of A and 128 rows of B per
+// CTA, 128 k values (128 bytes) each, in the 128-byte swizzle: 32 KiB a stage,
+// six stages. The int32 accumulator is double-buffered in TMEM, so that the
+// epilogue of one tile runs beside the next tile's products. The work schedule
+// (full waves, then a last wave split over idle pairs) is pair_sched.h; the
+// parts of a split tile are int32, so adding them is exact in any order.
+// k_int8_gemm_any: operands that TMA cannot describe.
+#include <atomic>
+#include <mutex>
+
 #include "int8_math.cuh"
+#include "kernel_config.h"
+#include "pair_sched.h"
 
 namespace tfb200 {
 
@@ -66,15 +81,568 @@ __global__ void __launch_bounds__(256) k_int8_gemm_any(const int8_t* A, int64_t 
   }
 }
 
+// ------------------------------------------------------------ CTA-pair kernel
+
+constexpr int kBM = 128;                   // rows of A, and rows of B, per CTA
+constexpr int kBN = 256;                   // columns of a pair's tile
+constexpr int kBK = 128;                   // k values per stage (128 bytes)
+constexpr int kStages = cfg::kPairStages;
+constexpr uint32_t kTileBytes = kBM * kBK;  // one operand's stage: 16 KiB
+constexpr int kEpiWarps = cfg::kPairEpiWarps;
+constexpr int kChunks = kBN / 32 / (kEpiWarps / 4);  // 32-column chunks per epilogue warp
+constexpr uint32_t kStageOut = 32 * 64;              // one staged block: 32 rows of 64 bytes
+constexpr int kGroup = cfg::kGroupM;                 // row tiles per raster group
+constexpr int kSmPairs = 74;                         // CTA pairs of a B200
+
+struct PairCtl {
+  uint64_t full[kStages];
+  uint64_t empty[kStages];
+  uint64_t tfull[2];
+  uint64_t tempty[2];
+  uint64_t drain;
+  uint32_t tmem_base;
+  int abort;
+};
+
+constexpr size_t kPairSmem =
+    1024 + 2 * kStages * kTileBytes + static_cast<size_t>(kEpiWarps) * 2 * kStageOut + sizeof(PairCtl);
+
+struct PairParams {
+  Int8Epi e;
+  int vec_ok;     // scales, bias and residual allow 16-byte loads
+  int tma_store;  // C is stored through shared memory with TMA
+  int b_prefetch;
+  sched::PairSched ps;
+  int32_t* slots;
+  int* flags;
+  int* status;
+  uint64_t timeout_ns;
+};
+
+__device__ __forceinline__ void tile_of(int t, int num_m, int num_n, int& tm, int& tn) {
+  const int per_group = kGroup * num_n;
+  const int g = t / per_group;
+  const int rows = min(num_m - g * kGroup, kGroup);
+  const int local = t - g * per_group;
+  tm = g * kGroup + local % rows;
+  tn = local / rows;
+}
+
+__device__ __forceinline__ void give_up(PairCtl* ctl, int* status) {
+  ctl->abort = 1;
+  atomicExch(status, kDevTimeout);
+}
+
+// 32 columns of one row, col0 .. col0 + 31, finished in fp32.
+__device__ __forceinline__ void finish32(const PairParams& p, const uint32_t (&v)[32], float sa, float factor,
+                                         int64_t row, int col0, float (&f)[32]) {
+  const Int8Epi& e = p.e;
+  if (p.vec_ok && col0 + 32 <= e.N) {
+    const float4* sp = reinterpret_cast<const float4*>(e.b_scale + col0);
+    if (e.bias) {
+      const uint4* bp = reinterpret_cast<const uint4*>(e.bias + col0);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float4 s0 = __ldg(sp + 2 * u), s1 = __ldg(sp + 2 * u + 1);
+        const uint4 b = __ldg(bp + u);
+        const float s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+        const uint32_t w[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          f[8 * u + j] = int8_scaled(static_cast<int32_t>(v[8 * u + j]), sa, s[j],
+                                     (j & 1) ? bf16_hi(w[j >> 1]) : bf16_lo(w[j >> 1]));
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float4 s4 = __ldg(sp + u);
+        const float s[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[4 * u + j] = int8_scaled(static_cast<int32_t>(v[4 * u + j]), sa, s[j]);
+      }
+    }
+    if (e.gelu == kGeluErf) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) f[j] = int8_gelu(f[j], kGeluErf);
+    } else if (e.gelu == kGeluTanh) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) f[j] = int8_gelu(f[j], kGeluTanh);
+    }
+    if (e.residual) {
+      const uint4* rp = reinterpret_cast<const uint4*>(e.residual + row * e.ldr + col0);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const uint4 b = rp[u];
+        const uint32_t w[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          f[8 * u + 2 * j] = __fadd_rn(f[8 * u + 2 * j], bf16_lo(w[j]));
+          f[8 * u + 2 * j + 1] = __fadd_rn(f[8 * u + 2 * j + 1], bf16_hi(w[j]));
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      f[j] = 0.0f;
+      const int n = col0 + j;
+      if (n < e.N) {
+        f[j] = int8_value(e, static_cast<int32_t>(v[j]), sa, n);
+        if (e.residual) f[j] = __fadd_rn(f[j], __bfloat162float(e.residual[row * e.ldr + n]));
+      }
+    }
+  }
+  if (e.out == kInt8OutHidden) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) f[j] *= factor;
+  }
+}
+
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// 16 bytes at 16-byte unit u of the lane's row in a staged block (64-byte
+// swizzle: conflict-free for eight rows).
+__device__ __forceinline__ void stage16(uint32_t buf, int lane, int u, uint32_t a, uint32_t b, uint32_t c,
+                                        uint32_t d) {
+  const uint32_t at = buf + static_cast<uint32_t>(lane * 64 + ((u ^ ((lane >> 1) & 3)) << 4));
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+__global__ void __launch_bounds__(cfg::kPairThreads, 1)
+    k_int8_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                const __grid_constant__ CUtensorMap tmC, const PairParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint8_t* sA = smem;
+  uint8_t* sB = sA + kStages * kTileBytes;
+  uint8_t* sC = sB + kStages * kTileBytes;
+  PairCtl* ctl = reinterpret_cast<PairCtl*>(sC + kEpiWarps * 2 * kStageOut);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(smem_u32(&ctl->full[s]), 1);
+      mbar_init(smem_u32(&ctl->empty[s]), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(smem_u32(&ctl->tfull[b]), 1);
+      mbar_init(smem_u32(&ctl->tempty[b]), 2 * kEpiWarps);  // the epilogue warps of both CTAs
+    }
+    mbar_init(smem_u32(&ctl->drain), 1);
+    ctl->abort = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+    if (p.tma_store) tma_prefetch_desc(&tmC);
+  }
+  if (warp == 2) {
+    tmem_alloc_pair(smem_u32(&ctl->tmem_base), 2 * kBN);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  cluster_sync();  // both CTAs' barriers exist before any remote arrival
+  tc_fence_after();
+  const uint32_t tmem_base = ctl->tmem_base;
+  grid_dep_launch();
+  if (warp != 0) grid_dep_wait();  // the producer waits below, after its weight prefetch
+
+  const int pair = blockIdx.x >> 1;
+  const sched::PairSched& ps = p.ps;
+  const int nwork = sched::work_count(ps, pair);
+  const int num_m = (p.e.M + 2 * kBM - 1) / (2 * kBM);
+  const int num_n = (p.e.N + kBN - 1) / kBN;
+
+  if (warp == 0) {
+    // ------------------------------------------------ TMA producer (both CTAs)
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      // The first stages of B, if the preceding kernel does not write it, are
+      // requested while that kernel finishes; A follows after the wait.
+      int npre = 0;
+      if (p.b_prefetch && nwork > 0) {
+        const sched::Work w = sched::work_item(ps, pair, 0);
+        int tm, tn;
+        tile_of(w.tile, num_m, num_n, tm, tn);
+        npre = min(kStages, w.k1 - w.k0);
+        for (int s = 0; s < npre; ++s) {
+          const uint32_t fb = mapa_shared(smem_u32(&ctl->full[s]), 0);
+          if (leader) mbar_arrive_expect_tx(smem_u32(&ctl->full[s]), 4 * kTileBytes);
+          tma_load_2d_pair(smem_u32(sB + s * kTileBytes), &tmB, fb, (w.k0 + s) * kBK,
+                           tn * kBN + static_cast<int>(rank) * kBM);
+        }
+      }
+      grid_dep_wait();
+      for (int i = 0; i < nwork && ok; ++i) {
+        const sched::Work w = sched::work_item(ps, pair, i);
+        int tm, tn;
+        tile_of(w.tile, num_m, num_n, tm, tn);
+        for (int kb = w.k0; kb < w.k1; ++kb) {
+          const bool pre = i == 0 && kb - w.k0 < npre;  // armed, B in flight
+          if (!pre && !mbar_wait(smem_u32(&ctl->empty[stage]), phase ^ 1u, &ctl->abort, p.timeout_ns)) {
+            give_up(ctl, p.status);
+            ok = false;
+            break;
+          }
+          const uint32_t fb = mapa_shared(smem_u32(&ctl->full[stage]), 0);
+          if (leader && !pre) mbar_arrive_expect_tx(smem_u32(&ctl->full[stage]), 4 * kTileBytes);
+          tma_load_2d_pair(smem_u32(sA + stage * kTileBytes), &tmA, fb, kb * kBK,
+                           tm * 2 * kBM + static_cast<int>(rank) * kBM);
+          if (!pre)
+            tma_load_2d_pair(smem_u32(sB + stage * kTileBytes), &tmB, fb, kb * kBK,
+                             tn * kBN + static_cast<int>(rank) * kBM);
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      if (!ok) {
+        // Copies already issued land within microseconds; give them time before
+        // the cluster tears down.
+        const uint64_t t0 = global_ns();
+        while (global_ns() - t0 < 1000000ull) {
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // --------------------------------------------------- MMA issuer (leader)
+    if (lane == 0 && leader) {
+      constexpr uint32_t idesc = idesc_i8(2 * kBM, kBN);
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int i = 0; i < nwork && ok; ++i) {
+        const sched::Work w = sched::work_item(ps, pair, i);
+        const int acc = i & 1;
+        const uint32_t use = static_cast<uint32_t>(i >> 1);
+        if (!mbar_wait(smem_u32(&ctl->tempty[acc]), (use & 1u) ^ 1u, &ctl->abort, p.timeout_ns)) {
+          give_up(ctl, p.status);
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d = tmem_base + static_cast<uint32_t>(acc * kBN);
+        for (int kb = w.k0; kb < w.k1; ++kb) {
+          if (!mbar_wait(smem_u32(&ctl->full[stage]), phase, &ctl->abort, p.timeout_ns)) {
+            give_up(ctl, p.status);
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t a0 = smem_u32(sA + stage * kTileBytes);
+          const uint32_t b0 = smem_u32(sB + stage * kTileBytes);
+#pragma unroll
+          for (int k = 0; k < kBK / 32; ++k)
+            mma_i8_pair(d, sdesc_sw128(a0 + k * 32, 16, 1024), sdesc_sw128(b0 + k * 32, 16, 1024), idesc,
+                        (kb != w.k0 || k != 0) ? 1u : 0u);
+          mma_commit_pair_both(smem_u32(&ctl->empty[stage]), 0x3);
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (ok) mma_commit_pair_both(smem_u32(&ctl->tfull[acc]), 0x3);
+      }
+      mma_commit_pair(smem_u32(&ctl->drain));
+      const uint64_t t0 = global_ns();
+      while (!mbar_test(smem_u32(&ctl->drain), 0) && global_ns() - t0 < p.timeout_ns) {
+      }
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------- epilogue (both CTAs)
+    // Warp w reads TMEM lane quadrant q = w % 4 (rows q*32 .. q*32+31 of this
+    // CTA's 128) and half of the tile's column chunks.
+    const int q = warp & 3;
+    const int ew = warp - 4;
+    const int c0 = (ew >> 2) * kChunks;
+    const int r = q * 32 + lane;
+    const uint32_t bufs = smem_u32(sC) + static_cast<uint32_t>(ew * 2) * kStageOut;
+    for (int i = 0; i < nwork; ++i) {
+      const sched::Work w = sched::work_item(ps, pair, i);
+      int tm, tn;
+      tile_of(w.tile, num_m, num_n, tm, tn);
+      const int acc = i & 1;
+      const uint32_t use = static_cast<uint32_t>(i >> 1);
+      bool ok = mbar_wait(smem_u32(&ctl->tfull[acc]), use & 1u, &ctl->abort, p.timeout_ns);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) {
+        if (lane == 0) give_up(ctl, p.status);
+        break;
+      }
+      tc_fence_after();
+      const int64_t row0 = static_cast<int64_t>(tm) * 2 * kBM + static_cast<int64_t>(rank) * kBM + q * 32;
+      const int64_t row = row0 + lane;
+      const uint32_t tacc = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * kBN);
+      const bool part = w.role == sched::kPart, fix = w.role == sched::kMain;
+      float sa = 0.0f, factor = 1.0f;
+      if (!part && row < p.e.M) {
+        sa = __ldg(p.e.a_scale + row);
+        if (p.e.out == kInt8OutHidden) factor = hidden_factor(p.e.K, sa, p.e.bound);
+      }
+      for (int c = c0; ok && c < c0 + kChunks; ++c) {
+        const int col0 = tn * kBN + c * 32;
+        if (col0 >= p.e.N || row0 >= p.e.M) break;  // warp-uniform: nothing of this block is in the matrix
+        uint32_t v[32];
+        tmem_ld_32cols(tacc + static_cast<uint32_t>(c * 32), v);
+        tmem_wait_ld();
+        if (part) {
+          // A helper's part: its 32 rows of the chunk go to the part's slot
+          // (layout [chunk][column / 4][row][4]); each lane then counts its row
+          // in on the chunk's flag (release).
+          int4* slot = reinterpret_cast<int4*>(p.slots + (static_cast<int64_t>(w.slot) * 2 + rank) * (kBM * kBN)) + r;
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            __stcg(slot + (c * 8 + j) * kBM,
+                   make_int4(static_cast<int>(v[4 * j]), static_cast<int>(v[4 * j + 1]),
+                             static_cast<int>(v[4 * j + 2]), static_cast<int>(v[4 * j + 3])));
+          red_add_release_gpu(p.flags + ((w.slot * 2 + static_cast<int>(rank)) * kEpiWarps + ew) * kChunks + (c - c0),
+                              1);
+          continue;
+        }
+        if (fix) {
+          // The parts of a split tile, each once all its rows are in (acquire).
+          for (int j = 0; j < ps.parts; ++j) {
+            const int* f = p.flags + (((w.slot + j) * 2 + static_cast<int>(rank)) * kEpiWarps + ew) * kChunks + (c - c0);
+            const uint64_t t0 = global_ns();
+            while (ok && ld_acquire_gpu(f) != 32)
+              if (ctl->abort || global_ns() - t0 > p.timeout_ns) ok = false;
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            const int4* slot =
+                reinterpret_cast<const int4*>(p.slots + (static_cast<int64_t>(w.slot + j) * 2 + rank) * (kBM * kBN)) +
+                r + c * 8 * kBM;
+#pragma unroll
+            for (int j4 = 0; j4 < 8; ++j4) {
+              const int4 a = __ldcg(slot + j4 * kBM);
+              v[4 * j4] += static_cast<uint32_t>(a.x);
+              v[4 * j4 + 1] += static_cast<uint32_t>(a.y);
+              v[4 * j4 + 2] += static_cast<uint32_t>(a.z);
+              v[4 * j4 + 3] += static_cast<uint32_t>(a.w);
+            }
+          }
+          if (!ok) {
+            if (lane == 0) give_up(ctl, p.status);
+            break;
+          }
+        }
+        float f[32];
+        if (row < p.e.M) {
+          finish32(p, v, sa, factor, row, col0, f);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) f[j] = 0.0f;
+        }
+        if (!p.tma_store) {
+          if (row < p.e.M) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              if (col0 + j >= p.e.N) break;
+              if (p.e.out == kInt8OutF32)
+                static_cast<float*>(p.e.C)[row * p.e.ldc + col0 + j] = f[j];
+              else  // the hidden block is always stored with TMA
+                static_cast<bf16*>(p.e.C)[row * p.e.ldc + col0 + j] = __float2bfloat16_rn(f[j]);
+            }
+          }
+          continue;
+        }
+        // Stage the warp's block and store it with TMA (rows and columns past
+        // the matrix are clipped): 32 x 32 16-bit values, or two blocks of
+        // 32 x 16 fp32 values.
+        if (p.e.out == kInt8OutF32) {
+          if (lane == 0) bulk_wait_read<0>();
+          __syncwarp();
+#pragma unroll
+          for (int u = 0; u < 8; ++u)
+            stage16(bufs + (u >> 2) * kStageOut, lane, u & 3, __float_as_uint(f[4 * u]), __float_as_uint(f[4 * u + 1]),
+                    __float_as_uint(f[4 * u + 2]), __float_as_uint(f[4 * u + 3]));
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&tmC, bufs, col0, static_cast<int32_t>(row0));
+            if (col0 + 16 < p.e.N) tma_store_2d(&tmC, bufs + kStageOut, col0 + 16, static_cast<int32_t>(row0));
+            bulk_commit();
+          }
+        } else {
+          const uint32_t buf = bufs + static_cast<uint32_t>(c & 1) * kStageOut;
+          if (lane == 0) bulk_wait_read<1>();  // the store that used this buffer has read it
+          __syncwarp();
+          if (p.e.out == kInt8OutHidden) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              stage16(buf, lane, u, pack_half(f[8 * u], f[8 * u + 1]), pack_half(f[8 * u + 2], f[8 * u + 3]),
+                      pack_half(f[8 * u + 4], f[8 * u + 5]), pack_half(f[8 * u + 6], f[8 * u + 7]));
+          } else {
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              stage16(buf, lane, u, pack_bf16(f[8 * u], f[8 * u + 1]), pack_bf16(f[8 * u + 2], f[8 * u + 3]),
+                      pack_bf16(f[8 * u + 4], f[8 * u + 5]), pack_bf16(f[8 * u + 6], f[8 * u + 7]));
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&tmC, buf, col0, static_cast<int32_t>(row0));
+            bulk_commit();
+          }
+        }
+      }
+      if (!ok) break;
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        const uint32_t te = smem_u32(&ctl->tempty[acc]);
+        if (leader)
+          mbar_arrive(te);
+        else
+          mbar_arrive_cluster(mapa_shared(te, 0));
+      }
+    }
+    if (lane == 0 && p.tma_store) bulk_wait_all();  // staged stores have left shared memory
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // no CTA leaves while its peer may still touch its barriers or shared memory
+  if (warp == 2) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, 2 * kBN);
+  }
+}
+
+bool al(const void* p, unsigned b) { return (reinterpret_cast<uintptr_t>(p) & (b - 1)) == 0; }
+
+int64_t pair_tiles(int64_t m, int64_t n) { return (m + 2 * kBM - 1) / (2 * kBM) * ((n + kBN - 1) / kBN); }
+
+// The schedule over all the pairs of a B200; a short last wave is split when
+// that shortens the busiest pair by 2 % or more.
+sched::PairSched pair_plan(int64_t m, int64_t n, int64_t k) {
+  return sched::plan(static_cast<int>(pair_tiles(m, n)), static_cast<int>((k + kBK - 1) / kBK), kSmPairs,
+                     sched::kMaxSlots);
+}
+
+// Per-device set-up of the first call; calls may come from several host
+// threads. *pairs: how many pairs are resident at once.
+cudaError_t pair_ready(int* pairs) {
+  static std::mutex mu;
+  static std::atomic<int> resident[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  *pairs = resident[dev].load(std::memory_order_acquire);
+  if (*pairs > 0) return cudaSuccess;
+  std::lock_guard<std::mutex> lock(mu);
+  e = cudaFuncSetAttribute(k_int8_pair, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kPairSmem));
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t q{};
+  q.gridDim = dim3(static_cast<unsigned>(sm_count()), 1, 1);
+  q.blockDim = dim3(cfg::kPairThreads, 1, 1);
+  q.dynamicSmemBytes = kPairSmem;
+  cudaLaunchAttribute a[1];
+  a[0].id = cudaLaunchAttributeClusterDimension;
+  a[0].val.clusterDim = {2, 1, 1};
+  q.attrs = a;
+  q.numAttrs = 1;
+  int n = 0;
+  e = cudaOccupancyMaxActiveClusters(&n, k_int8_pair, &q);
+  if (e == cudaSuccess && n <= 0) e = cudaErrorLaunchOutOfResources;
+  if (e != cudaSuccess) return e;
+  resident[dev].store(n, std::memory_order_release);
+  *pairs = n;
+  return cudaSuccess;
+}
+
+bool map8(CUtensorMap* m, const int8_t* base, int64_t rows, int64_t cols, int64_t ld, uint32_t box_rows,
+          std::string* err) {
+  return make_map_box(m, base, rows, cols, rows > 1 ? ld : (cols + 15) / 16 * 16, kBK, box_rows,
+                      CU_TENSOR_MAP_SWIZZLE_128B, err, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1);
+}
+
+int launch_pair(const Int8Gemm& g, cudaStream_t s, std::string* err) {
+  int resident = 0;
+  cudaError_t e = pair_ready(&resident);
+  if (e != cudaSuccess) {
+    *err = std::string("int8 pair gemm set-up: ") + cudaGetErrorString(e);
+    return -3;
+  }
+  PairParams p{};
+  p.e = int8_epi(g);
+  p.status = device_status_ptr(err);
+  if (!p.status) return -3;
+  p.timeout_ns = wait_limit_ns();
+  p.vec_ok = al(g.b_scale, 16) && (!g.bias || al(g.bias, 16)) &&
+             (!g.residual || (al(g.residual, 16) && g.ldr % 8 == 0));
+  const int esz = g.out == kInt8OutF32 ? 4 : 2;
+  p.tma_store = al(g.C, 16) && g.ldc * esz % 16 == 0;
+  p.b_prefetch = g.b_stable;
+  CUtensorMap ta{}, tb{}, tc{};
+  if (!map8(&ta, g.A, g.M, g.K, g.lda, kBM, err) || !map8(&tb, g.B, g.N, g.K, g.ldb, kBM, err)) return -3;
+  if (p.tma_store && !make_map_box(&tc, g.C, g.M, g.N, g.ldc, static_cast<uint32_t>(64 / esz), 32,
+                                   CU_TENSOR_MAP_SWIZZLE_64B, err,
+                                   g.out == kInt8OutF32      ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : g.out == kInt8OutHidden ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                             : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                                   esz))
+    return -3;
+  p.ps = pair_plan(g.M, g.N, g.K);
+  if (p.ps.rem > 0 && resident >= kSmPairs) {
+    p.flags = static_cast<int*>(g.ws);
+    p.slots = reinterpret_cast<int32_t*>(static_cast<char*>(g.ws) + int8_gemm_ws(g.M, g.N, g.K).clear_bytes);
+  } else {
+    p.ps = sched::plan(p.ps.tiles, p.ps.kblocks, p.ps.tiles < resident ? p.ps.tiles : resident, 0);
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(2 * p.ps.pairs), 1, 1);
+  cfg.blockDim = dim3(cfg::kPairThreads, 1, 1);
+  cfg.dynamicSmemBytes = kPairSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute a[2];
+  a[0].id = cudaLaunchAttributeClusterDimension;
+  a[0].val.clusterDim = {2, 1, 1};
+  a[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  a[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = a;
+  cfg.numAttrs = 2;
+  e = cudaLaunchKernelEx(&cfg, k_int8_pair, ta, tb, tc, p);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (e != cudaSuccess) {
+    *err = std::string("int8 pair gemm launch: ") + cudaGetErrorString(e);
+    return -3;
+  }
+  count_launch();
+  return 0;
+}
+
 }  // namespace
 
-Int8GemmWs int8_gemm_ws(int64_t, int64_t, int64_t) { return {}; }
+Int8GemmWs int8_gemm_ws(int64_t m, int64_t n, int64_t k) {
+  Int8GemmWs w;
+  if (k <= 0 || pair_tiles(m, n) > (1 << 30)) return w;
+  const sched::PairSched ps = pair_plan(m, n, k);
+  if (ps.rem > 0) {
+    w.clear_bytes = (static_cast<size_t>(ps.rem) * ps.parts * sched::kFlagsPerSlot * sizeof(int) + 255) / 256 * 256;
+    w.total = w.clear_bytes + static_cast<size_t>(ps.rem) * ps.parts * sched::kSlotBytes;
+  }
+  return w;
+}
 
 int run_int8_gemm(const Int8Gemm& g, cudaStream_t stream, std::string* err) {
   if (g.M > (int64_t(1) << 30) || g.N > (int64_t(1) << 30) || g.K > kInt8MaxK) {
     *err = "dimension too large";
     return -2;
   }
+  // TMA describes operands that start on 16-byte boundaries with row strides
+  // that are multiples of 16 bytes (one row has no stride).
+  if (g.K > 0 && al(g.A, 16) && al(g.B, 16) && (g.lda % 16 == 0 || g.M == 1) && (g.ldb % 16 == 0 || g.N == 1) &&
+      pair_tiles(g.M, g.N) <= (1 << 30))
+    return launch_pair(g, stream, err);
   const int64_t by = (g.N + kAnyTile - 1) / kAnyTile;
   const dim3 grid(static_cast<unsigned>((g.M + kAnyTile - 1) / kAnyTile), static_cast<unsigned>(by < 65535 ? by : 65535));
   k_int8_gemm_any<<<grid, 256, 0, stream>>>(g.A, g.lda, g.B, g.ldb, int8_epi(g));

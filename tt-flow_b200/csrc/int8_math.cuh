@@ -69,17 +69,25 @@ __device__ __forceinline__ float hidden_factor(int K, float a_scale, const float
   return __uint_as_float(__float_as_uint(r) & 0x7F800000u);
 }
 
+// acc * sa * sb, and + bias: the same roundings in every kernel and layout.
+__device__ __forceinline__ float int8_scaled(int32_t acc, float sa, float sb) {
+  return __fmul_rn(__fmul_rn(__int2float_rn(acc), sa), sb);
+}
+__device__ __forceinline__ float int8_scaled(int32_t acc, float sa, float sb, float bias) {
+  return __fmaf_rn(__fmul_rn(__int2float_rn(acc), sa), sb, bias);
+}
+
 // One output value from its integer sum, without the residual.
 __device__ __forceinline__ float int8_value(const Int8Epi& e, int32_t acc, float sa, int n) {
-  float v = static_cast<float>(acc) * sa * e.b_scale[n];
-  if (e.bias) v += __bfloat162float(e.bias[n]);
+  const float v =
+      e.bias ? int8_scaled(acc, sa, e.b_scale[n], __bfloat162float(e.bias[n])) : int8_scaled(acc, sa, e.b_scale[n]);
   return int8_gelu(v, e.gelu);
 }
 
 // One output value, finished and stored; `factor` is the row's hidden factor.
 __device__ __forceinline__ void int8_store(const Int8Epi& e, int32_t acc, float sa, float factor, int64_t m, int n) {
   float v = int8_value(e, acc, sa, n);
-  if (e.residual) v += __bfloat162float(e.residual[m * e.ldr + n]);
+  if (e.residual) v = __fadd_rn(v, __bfloat162float(e.residual[m * e.ldr + n]));
   if (e.out == kInt8OutF32)
     static_cast<float*>(e.C)[m * e.ldc + n] = v;
   else if (e.out == kInt8OutBf16)

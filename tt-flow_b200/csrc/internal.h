@@ -136,10 +136,12 @@ int launch_residual_add(const float* part, int64_t ldp, const bf16* res, int64_t
 
 // Tensor map of a row-major bf16 matrix [rows, cols] (leading dimension ld),
 // box of 64 columns x box_rows rows, 128-byte swizzle, zero fill outside.
+// make_map_box also describes other element types.
 bool make_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64_t ld, uint32_t box_rows,
               std::string* err);
 bool make_map_box(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64_t ld, uint32_t box_cols,
-                  uint32_t box_rows, CUtensorMapSwizzle swizzle, std::string* err);
+                  uint32_t box_rows, CUtensorMapSwizzle swizzle, std::string* err,
+                  CUtensorMapDataType type = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, int elem_bytes = 2);
 
 // RMSNorm staging pass (rmsnorm_prep.cu): writes bf16(x * gamma) with leading
 // dimension staged_ld(K) and inv[m] = 1/sqrt(mean_k(x^2) + eps) into `ws`
