@@ -27,10 +27,11 @@ MAX_ROWS, MAX_K, MAX_OUT = 8192, 16384, 28672
 
 
 def _ops():
-    root = str(Path(__file__).resolve().parents[1] / "tt-flow_b200")
-    if root not in sys.path:
-        sys.path.insert(0, root)
-    from tfb200 import ops
+    try:
+        from tfb200 import ops
+    except ImportError:
+        sys.path.insert(0, str(Path(__file__).resolve().parents[1] / "tt-flow_b200"))
+        from tfb200 import ops
 
     return ops
 
