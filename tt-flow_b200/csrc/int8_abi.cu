@@ -57,11 +57,11 @@ bool same_shape(const tfb200_mat* a, const tfb200_mat* b) { return a->rows == b-
 
 const bf16* as_bf16(const void* p) { return static_cast<const bf16*>(p); }
 
-// Workspace of the fused calls: int8 rows and their scales, (MLP: fp16 hidden
-// block, its int8 form and scales, the bound), then each product's region, whose
+// Workspace of the fused calls: int8 rows and their scales, (MLP: the hidden
+// block, its int8 form and scales), then each product's region, whose
 // counters the rows launch ahead of it clears.
 struct Layout {
-  size_t q = 0, scale = 0, hidden = 0, hq = 0, hscale = 0, bound = 0, up = 0, down = 0, up_clear = 0, down_clear = 0,
+  size_t q = 0, scale = 0, hidden = 0, hq = 0, hscale = 0, up = 0, down = 0, up_clear = 0, down_clear = 0,
          total = 0;
 };
 
@@ -77,10 +77,9 @@ Layout layout(int64_t m, int64_t k, int64_t h, int64_t n) {
   l.q = take(rows * ld16(k));
   l.scale = take(rows * 4);
   if (h > 0) {
-    l.hidden = take(rows * ld16(h) * 2);
+    l.hidden = take(int8_hidden(m, h).bytes);
     l.hq = take(rows * ld16(h));
     l.hscale = take(rows * 4);
-    l.bound = take(8);
   }
   const Int8GemmWs up = int8_gemm_ws(m, h > 0 ? h : n, k);
   l.up = take(up.total);
@@ -326,9 +325,10 @@ int tfb200_fused_mlp_int8(const tfb200_mat* x, const void* gamma, const tfb200_m
     if (const int rc = ws_check(fn, workspace, workspace_bytes, l.total)) return rc;
     char* ws = static_cast<char*>(workspace);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    float* bound = reinterpret_cast<float*>(ws + l.bound);
-    // Norm and quantisation of the tokens; the same launch reads W1's scales and
-    // bias for the hidden block's bound and clears the up projection's counters.
+    const Int8Hidden hl = int8_hidden(M, H);
+    float* hmax = reinterpret_cast<float*>(ws + l.hidden + hl.max_at);
+    // Norm and quantisation of the tokens; the same launch clears the up
+    // projection's counters.
     Int8Rows r;
     r.kind = kInt8RowsNorm;
     r.M = M;
@@ -340,10 +340,6 @@ int tfb200_fused_mlp_int8(const tfb200_mat* x, const void* gamma, const tfb200_m
     r.q = reinterpret_cast<int8_t*>(ws + l.q);
     r.ldq = ld16(K);
     r.scale = reinterpret_cast<float*>(ws + l.scale);
-    r.b_scale = w1_scale;
-    r.bias = as_bf16(b1);
-    r.bound_n = H;
-    r.bound_out = bound;
     r.zero = ws + l.up;
     r.zero_bytes = l.up_clear;
     int rc = run_int8_rows(r, s, &err);
@@ -361,9 +357,10 @@ int tfb200_fused_mlp_int8(const tfb200_mat* x, const void* gamma, const tfb200_m
     up.bias = as_bf16(b1);
     up.gelu = gelu_of(gelu_mode);
     up.C = ws + l.hidden;
-    up.ldc = ld16(H);
+    up.ldc = hl.ld;
     up.out = kInt8OutHidden;
-    up.bound = bound;
+    up.hidden_max = hmax;
+    up.ldm = hl.ldm;
     up.ws = ws + l.up;
     up.b_stable = true;
     rc = run_int8_gemm(up, s, &err);
@@ -375,9 +372,8 @@ int tfb200_fused_mlp_int8(const tfb200_mat* x, const void* gamma, const tfb200_m
     hr.K = H;
     hr.x = up.C;
     hr.ldx = up.ldc;
-    hr.up_k = K;
-    hr.up_scale = r.scale;
-    hr.bound = bound;
+    hr.hidden_max = hmax;
+    hr.ldm = hl.ldm;
     hr.q = reinterpret_cast<int8_t*>(ws + l.hq);
     hr.ldq = ld16(H);
     hr.scale = reinterpret_cast<float*>(ws + l.hscale);

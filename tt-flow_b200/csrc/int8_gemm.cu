@@ -71,11 +71,37 @@ __global__ void __launch_bounds__(256) k_int8_gemm_any(const int8_t* A, int64_t 
       const int64_t m = m0 + ty + 16 * i;
       if (m >= e.M) break;
       const float s = e.a_scale[m];
-      const float factor = e.out == kInt8OutHidden ? hidden_factor(e.K, s, e.bound) : 1.0f;
+      if (e.out != kInt8OutHidden) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int64_t n = n0 + tx + 16 * j;
-        if (n < e.N) int8_store(e, acc[i][j], s, factor, m, static_cast<int>(n));
+        for (int j = 0; j < 4; ++j) {
+          const int64_t n = n0 + tx + 16 * j;
+          if (n < e.N) int8_store(e, acc[i][j], s, m, static_cast<int>(n));
+        }
+        continue;
+      }
+      // Two blocks of 32 columns, each held by 16 neighbouring lanes.
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float v[2];
+        uint32_t amax = 0;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int64_t n = n0 + tx + 16 * (2 * h + j);
+          v[j] = n < e.N ? int8_value(e, acc[i][2 * h + j], s, static_cast<int>(n)) : 0.0f;
+          amax = max(amax, mag(v[j]));
+        }
+        // The 16 lanes hold one row: all of them are here.
+        const unsigned lanes = 0xFFFFu << (threadIdx.x & 16);
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(lanes, amax, o));
+        const UpScale us = up_scale(amax, 32767.0f);
+        const int64_t block = n0 / kHiddenBlock + h;
+        if (tx == 0 && block < e.ldm) e.hidden_max[m * e.ldm + block] = hidden_max(amax);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int64_t n = n0 + tx + 16 * (2 * h + j);
+          if (n < e.N) static_cast<int16_t*>(e.C)[m * e.ldc + n] = static_cast<int16_t>(hidden_bits(v[j], us) & 0xFFFFu);
+        }
       }
     }
   }
@@ -133,9 +159,9 @@ __device__ __forceinline__ void give_up(PairCtl* ctl, int* status) {
   atomicExch(status, kDevTimeout);
 }
 
-// 32 columns of one row, col0 .. col0 + 31, finished in fp32.
-__device__ __forceinline__ void finish32(const PairParams& p, const uint32_t (&v)[32], float sa, float factor,
-                                         int64_t row, int col0, float (&f)[32]) {
+// 32 columns of one row, col0 .. col0 + 31, finished in fp32 (0 past the matrix).
+__device__ __forceinline__ void finish32(const PairParams& p, const uint32_t (&v)[32], float sa, int64_t row,
+                                         int col0, float (&f)[32]) {
   const Int8Epi& e = p.e;
   if (p.vec_ok && col0 + 32 <= e.N) {
     const float4* sp = reinterpret_cast<const float4*>(e.b_scale + col0);
@@ -192,15 +218,6 @@ __device__ __forceinline__ void finish32(const PairParams& p, const uint32_t (&v
       }
     }
   }
-  if (e.out == kInt8OutHidden) {
-#pragma unroll
-    for (int j = 0; j < 32; ++j) f[j] *= factor;
-  }
-}
-
-__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
 }
 
 // 16 bytes at 16-byte unit u of the lane's row in a staged block (64-byte
@@ -383,11 +400,8 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
       const int64_t row = row0 + lane;
       const uint32_t tacc = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * kBN);
       const bool part = w.role == sched::kPart, fix = w.role == sched::kMain;
-      float sa = 0.0f, factor = 1.0f;
-      if (!part && row < p.e.M) {
-        sa = __ldg(p.e.a_scale + row);
-        if (p.e.out == kInt8OutHidden) factor = hidden_factor(p.e.K, sa, p.e.bound);
-      }
+      const float sa = !part && row < p.e.M ? __ldg(p.e.a_scale + row) : 0.0f;
+      float hmax[kChunks] = {};
       for (int c = c0; ok && c < c0 + kChunks; ++c) {
         const int col0 = tn * kBN + c * 32;
         if (col0 >= p.e.N || row0 >= p.e.M) break;  // warp-uniform: nothing of this block is in the matrix
@@ -436,7 +450,7 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
         }
         float f[32];
         if (row < p.e.M) {
-          finish32(p, v, sa, factor, row, col0, f);
+          finish32(p, v, sa, row, col0, f);
         } else {
 #pragma unroll
           for (int j = 0; j < 32; ++j) f[j] = 0.0f;
@@ -476,10 +490,19 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
           if (lane == 0) bulk_wait_read<1>();  // the store that used this buffer has read it
           __syncwarp();
           if (p.e.out == kInt8OutHidden) {
+            uint32_t amax = 0;
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-              stage16(buf, lane, u, pack_half(f[8 * u], f[8 * u + 1]), pack_half(f[8 * u + 2], f[8 * u + 3]),
-                      pack_half(f[8 * u + 4], f[8 * u + 5]), pack_half(f[8 * u + 6], f[8 * u + 7]));
+            for (int j = 0; j < 32; ++j) amax = max(amax, mag(f[j]));
+            const UpScale us = up_scale(amax, 32767.0f);
+#pragma unroll
+            for (int k = 0; k < kChunks; ++k)
+              if (k == c - c0) hmax[k] = hidden_max(amax);
+            uint32_t w[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              w[j] = __byte_perm(hidden_bits(f[2 * j], us), hidden_bits(f[2 * j + 1], us), 0x5410);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) stage16(buf, lane, u, w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
           } else {
 #pragma unroll
             for (int u = 0; u < 4; ++u)
@@ -495,6 +518,10 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
         }
       }
       if (!ok) break;
+      // The maxima of this warp's 128 columns.
+      if (p.e.out == kInt8OutHidden && !part && row < p.e.M && tn * kBN + c0 * 32 < p.e.N)
+        *reinterpret_cast<float4*>(p.e.hidden_max + row * p.e.ldm + tn * (kBN / kHiddenBlock) + c0) =
+            make_float4(hmax[0], hmax[1], hmax[2], hmax[3]);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
@@ -587,7 +614,7 @@ int launch_pair(const Int8Gemm& g, cudaStream_t s, std::string* err) {
   if (p.tma_store && !make_map_box(&tc, g.C, g.M, g.N, g.ldc, static_cast<uint32_t>(64 / esz), 32,
                                    CU_TENSOR_MAP_SWIZZLE_64B, err,
                                    g.out == kInt8OutF32      ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
-                                   : g.out == kInt8OutHidden ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                   : g.out == kInt8OutHidden ? CU_TENSOR_MAP_DATA_TYPE_UINT16
                                                              : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
                                    esz))
     return -3;

@@ -1,8 +1,6 @@
 // Device arithmetic shared by the kernels of the 8-bit integer path.
 #pragma once
 
-#include <cuda_fp16.h>
-
 #include "int8.h"
 #include "sm100_ptx.cuh"
 
@@ -20,7 +18,8 @@ struct Int8Epi {
   void* C;
   int64_t ldc;
   int out;
-  const float* bound;
+  float* hidden_max;
+  int64_t ldm;
 };
 
 inline Int8Epi int8_epi(const Int8Gemm& g) {
@@ -37,7 +36,8 @@ inline Int8Epi int8_epi(const Int8Gemm& g) {
   e.C = g.C;
   e.ldc = g.ldc;
   e.out = g.out;
-  e.bound = g.bound;
+  e.hidden_max = g.hidden_max;
+  e.ldm = g.ldm;
   return e;
 }
 
@@ -56,17 +56,35 @@ __device__ __forceinline__ float int8_gelu(float x, int mode) {
   return x;
 }
 
-// Power of two that brings row m's hidden values into fp16 whatever they are:
-// |h| <= |u| <= 127 * 127 * K * a_scale * max |b_scale| + max |bias|, and the
-// factor takes that bound to at most 32768. The products a model forms lie two
-// to three orders of magnitude under the bound, where fp16 still holds 11 bits,
-// eight times finer than bf16: with bf16 the second quantisation moved about
-// 2 % of the hidden values by a step.
-__device__ __forceinline__ float hidden_factor(int K, float a_scale, const float* bound) {
-  const float u = 16129.0f * static_cast<float>(K) * fabsf(a_scale) * bound[0] + bound[1];
-  if (!(u > 0.0f)) return 1.0f;  // an empty bound, or a NaN row
-  const float r = fminf(fmaxf(32768.0f / u, 1.17549435e-38f), 1.2676506e30f);
-  return __uint_as_float(__float_as_uint(r) & 0x7F800000u);
+// Largest |value| as its bits: unsigned order puts infinities and NaN on top.
+__device__ __forceinline__ uint32_t mag(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+
+// rn(v) for |v| < 2^22, half to even, in the low 16 bits: adding 1.5 * 2^23
+// leaves the integer in the low bits (a conversion instruction runs at a quarter
+// of the add's rate).
+__device__ __forceinline__ uint32_t round_bits(float v) { return __float_as_uint(__fadd_rn(v, 12582912.0f)); }
+
+// limit / amax as two factors: the reciprocal leaves fp32 for the smallest amax,
+// which are taken up by a power of two first (exact). {0, 0} for a maximum of
+// zero and for one that is not finite.
+struct UpScale {
+  float up, r;
+};
+__device__ __forceinline__ UpScale up_scale(uint32_t amax_bits, float limit) {
+  const float amax = __uint_as_float(amax_bits);
+  UpScale s;
+  s.up = amax < 1e-30f ? 7.9228163e28f : 1.0f;
+  s.r = amax_bits == 0u || amax_bits >= 0x7F800000u ? 0.0f : __fmul_rn(__frcp_rn(amax * s.up), limit);
+  return s;
+}
+
+// The maximum kept for a block of the hidden values (Int8Hidden).
+__device__ __forceinline__ float hidden_max(uint32_t amax_bits) {
+  return __uint_as_float(amax_bits >= 0x7F800000u ? 0x7FC00000u : amax_bits);
+}
+// One hidden value in the low 16 bits; s = up_scale(its block's maximum, 32767).
+__device__ __forceinline__ uint32_t hidden_bits(float h, UpScale s) {
+  return s.r == 0.0f ? 0u : round_bits(h * s.up * s.r);
 }
 
 // acc * sa * sb, and + bias: the same roundings in every kernel and layout.
@@ -84,16 +102,14 @@ __device__ __forceinline__ float int8_value(const Int8Epi& e, int32_t acc, float
   return int8_gelu(v, e.gelu);
 }
 
-// One output value, finished and stored; `factor` is the row's hidden factor.
-__device__ __forceinline__ void int8_store(const Int8Epi& e, int32_t acc, float sa, float factor, int64_t m, int n) {
+// One output value but for a hidden one, finished and stored.
+__device__ __forceinline__ void int8_store(const Int8Epi& e, int32_t acc, float sa, int64_t m, int n) {
   float v = int8_value(e, acc, sa, n);
   if (e.residual) v = __fadd_rn(v, __bfloat162float(e.residual[m * e.ldr + n]));
   if (e.out == kInt8OutF32)
     static_cast<float*>(e.C)[m * e.ldc + n] = v;
-  else if (e.out == kInt8OutBf16)
-    static_cast<bf16*>(e.C)[m * e.ldc + n] = __float2bfloat16_rn(v);
   else
-    static_cast<__half*>(e.C)[m * e.ldc + n] = __float2half_rn(v * factor);
+    static_cast<bf16*>(e.C)[m * e.ldc + n] = __float2bfloat16_rn(v);
 }
 
 }  // namespace tfb200

@@ -40,14 +40,8 @@ struct RowsParams {
   int8_t* q;
   int64_t ldq;
   float* scale;
-  int up_k;
-  const float* up_scale;
-  const float* bound;
-  const float* b_scale;
-  const bf16* bias;
-  int64_t bound_n;
-  float* bound_out;
-  int row_blocks;  // the block after them computes bound_out
+  const float* hidden_max;
+  int64_t ldm;
   uint4* zero;
   int64_t zero_vecs;
 };
@@ -67,12 +61,9 @@ __global__ void __launch_bounds__(256) k_int8_clear(uint4* zero, int64_t n) {
 
 template <int KIND>
 __device__ __forceinline__ float in_value(uint16_t bits) {
-  if (KIND == kInt8RowsHidden) return __half2float(__ushort_as_half(bits));
+  if (KIND == kInt8RowsHidden) return static_cast<float>(static_cast<int16_t>(bits));
   return __uint_as_float(static_cast<uint32_t>(bits) << 16);
 }
-
-// Largest |value| as its bits: unsigned order puts infinities and NaN on top.
-__device__ __forceinline__ uint32_t mag(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 
 struct RowStat {
   float ss;
@@ -105,57 +96,27 @@ __device__ __forceinline__ RowStat block_stat(RowStat s, bool squares) {
 }
 
 struct RowScale {
-  float up, r, scale;  // q = rn(t * up * r)
+  UpScale u;  // q = rn(t * u.up * u.r)
+  float scale;
 };
 
 template <int KIND>
-__device__ __forceinline__ RowScale row_scale(const RowsParams& p, int64_t row, RowStat s) {
+__device__ __forceinline__ RowScale row_scale(const RowsParams& p, RowStat s) {
   RowScale o;
+  if (KIND == kInt8RowsNorm && !(s.ss <= 3.402823466e38f)) s.amax = 0x7FC00000u;
+  o.u = up_scale(s.amax, 127.0f);
   const float amax = __uint_as_float(s.amax);
-  // 127 / amax leaves fp32 for the smallest values: those rows are taken up by
-  // a power of two first (exact).
-  o.up = amax < 1e-30f ? 7.9228163e28f : 1.0f;
-  bool bad = s.amax >= 0x7F800000u;
-  if (KIND == kInt8RowsNorm) {
-    bad = bad || !(s.ss <= 3.402823466e38f);
-    o.scale = amax * (1.0f / sqrtf(s.ss / static_cast<float>(p.K) + p.eps) / 127.0f);
-  } else if (KIND == kInt8RowsHidden) {
-    o.scale = amax / 127.0f / hidden_factor(p.up_k, p.up_scale[row], p.bound);
-  } else {
-    o.scale = amax / 127.0f;
-  }
-  o.r = s.amax == 0u || bad ? 0.0f : 127.0f / (amax * o.up);
-  if (bad) {
-    o.up = 0.0f;
-    o.scale = __uint_as_float(0x7FC00000u);
-  }
+  o.scale = KIND == kInt8RowsNorm ? amax * (1.0f / sqrtf(s.ss / static_cast<float>(p.K) + p.eps) / 127.0f)
+                                  : amax / 127.0f;
+  if (s.amax >= 0x7F800000u) o.scale = __uint_as_float(0x7FC00000u);
   return o;
 }
 
-// rn(v) for |v| <= 127 in the low byte: adding 1.5 * 2^23 leaves the integer,
-// rounded half to even, in the low bits (a conversion instruction runs at a
-// quarter of the add's rate).
 __device__ __forceinline__ uint32_t q_bits(float t, const RowScale& s) {
-  return __float_as_uint(__fadd_rn(__fmul_rn(__fmul_rn(t, s.up), s.r), 12582912.0f));
+  return round_bits(__fmul_rn(__fmul_rn(t, s.u.up), s.u.r));
 }
 __device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
-}
-
-// The bound of the product that follows, by one block.
-__device__ void bound_block(const RowsParams& p) {
-  float s = 0.0f, b = 0.0f;
-  for (int64_t n = threadIdx.x; n < p.bound_n; n += blockDim.x) {
-    s = fmaxf(s, fabsf(p.b_scale[n]));
-    if (p.bias) b = fmaxf(b, fabsf(__bfloat162float(p.bias[n])));
-  }
-  const uint32_t smax = block_stat({0.0f, mag(s)}, false).amax;
-  __syncthreads();
-  const uint32_t bmax = block_stat({0.0f, mag(b)}, false).amax;
-  if (threadIdx.x == 0) {
-    p.bound_out[0] = __uint_as_float(smax);
-    p.bound_out[1] = __uint_as_float(bmax);
-  }
 }
 
 // VEC: rows start on 16-byte boundaries (8 for q); a thread takes 8 neighbouring
@@ -170,10 +131,6 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) k_int8_rows(const RowsParam
   grid_dep_wait();
   grid_dep_launch();
   clear_words(p.zero, p.zero_vecs);
-  if (static_cast<int>(blockIdx.x) >= p.row_blocks) {
-    bound_block(p);
-    return;
-  }
   const int T = WARP ? 32 : blockDim.x;
   const int t = WARP ? threadIdx.x & 31 : threadIdx.x;
   const int64_t row = WARP ? static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5) : blockIdx.x;
@@ -207,14 +164,23 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) k_int8_rows(const RowsParam
     load8(x, first(i), xw[i]);
     if (RES) load8(r, first(i), rw[i]);
   }
+  float hm[KIND == kInt8RowsHidden ? G : 1];
+  if (KIND == kInt8RowsHidden) {
+#pragma unroll
+    for (int i = 0; i < G; ++i)
+      hm[i] = first(i) < K ? p.hidden_max[row * p.ldm + first(i) / kHiddenBlock] : 0.0f;
+  }
   auto half16 = [](const uint32_t (&w)[4], int j) { return static_cast<uint16_t>(w[j >> 1] >> (16 * (j & 1))); };
   // The 8 values t of group i; with STAT also their statistics and the sum.
   RowStat st{0.0f, 0u};
   auto group = [&](int i, bool stat, float (&v)[8]) {
     const int k = first(i);
+    // Eight hidden values lie in one block of 32.
+    const float block = KIND == kInt8RowsHidden ? hm[i] * (1.0f / 32767.0f) : 1.0f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       v[j] = in_value<KIND>(half16(xw[i], j));
+      if (KIND == kInt8RowsHidden) v[j] *= block;
       if (RES) v[j] = __fadd_rn(v[j], in_value<kInt8RowsQuant>(half16(rw[RES ? i : 0], j)));
     }
     if (KIND == kInt8RowsNorm) {
@@ -255,10 +221,10 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) k_int8_rows(const RowsParam
     if (first(i) < K) group(i, true, v);
   }
   st = WARP ? warp_stat(st, KIND == kInt8RowsNorm) : block_stat(st, KIND == kInt8RowsNorm);
-  const RowScale sc = row_scale<KIND>(p, row, st);
+  const RowScale sc = row_scale<KIND>(p, st);
   if (t == 0) p.scale[row] = sc.scale;
   int8_t* q = p.q + row * p.ldq;
-  const bool zero = sc.r == 0.0f;  // a row of zeros, or one that is not finite
+  const bool zero = sc.u.r == 0.0f;  // a row of zeros, or one that is not finite
 #pragma unroll
   for (int i = 0; i < G; ++i) {
     const int k = first(i);
@@ -285,16 +251,13 @@ __global__ void __launch_bounds__(1024) k_int8_rows_long(const RowsParams p) {
   grid_dep_wait();
   grid_dep_launch();
   clear_words(p.zero, p.zero_vecs);
-  if (static_cast<int>(blockIdx.x) >= p.row_blocks) {
-    bound_block(p);
-    return;
-  }
   const int64_t row = blockIdx.x;
   const uint16_t* x = static_cast<const uint16_t*>(p.x) + row * p.ldx;
   const uint16_t* r = RES ? reinterpret_cast<const uint16_t*>(p.residual) + row * p.ldr : nullptr;
   const uint16_t* g = reinterpret_cast<const uint16_t*>(p.gamma);
   auto value = [&](int k) {
     float s = in_value<KIND>(x[k]);
+    if (KIND == kInt8RowsHidden) s *= p.hidden_max[row * p.ldm + k / kHiddenBlock] * (1.0f / 32767.0f);
     if (RES) s = __fadd_rn(s, in_value<kInt8RowsQuant>(r[k]));
     return s;
   };
@@ -309,9 +272,9 @@ __global__ void __launch_bounds__(1024) k_int8_rows_long(const RowsParams p) {
     st.amax = max(st.amax, mag(s));
   }
   st = block_stat(st, KIND == kInt8RowsNorm);
-  const RowScale sc = row_scale<KIND>(p, row, st);
+  const RowScale sc = row_scale<KIND>(p, st);
   if (threadIdx.x == 0) p.scale[row] = sc.scale;
-  const bool zero = sc.r == 0.0f;
+  const bool zero = sc.u.r == 0.0f;
   // A thread reads a value of x again before it writes the sum, which may be x.
 #pragma unroll 4
   for (int k = threadIdx.x; k < p.K; k += blockDim.x) {
@@ -323,14 +286,13 @@ __global__ void __launch_bounds__(1024) k_int8_rows_long(const RowsParams p) {
 }
 
 template <int KIND, bool RES>
-cudaError_t launch_rows(RowsParams& p, bool vec, cudaStream_t s) {
+cudaError_t launch_rows(const RowsParams& p, bool vec, cudaStream_t s) {
   const bool warp = p.K <= 32 * kPer;
   int T = 128;
   while (!warp && T < 1024 && T * kPer < p.K) T *= 2;
   if (p.K > kMaxRow) T = 1024;
-  p.row_blocks = warp ? (p.M + 3) / 4 : p.M;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(p.row_blocks) + (p.bound_out ? 1u : 0u), 1, 1);
+  cfg.gridDim = dim3(static_cast<unsigned>(warp ? (p.M + 3) / 4 : p.M), 1, 1);
   cfg.blockDim = dim3(static_cast<unsigned>(T), 1, 1);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
@@ -338,11 +300,12 @@ cudaError_t launch_rows(RowsParams& p, bool vec, cudaStream_t s) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  constexpr bool kAny = KIND != kInt8RowsHidden;  // the hidden block is always aligned
   cudaError_t e = p.K > kMaxRow ? cudaLaunchKernelEx(&cfg, k_int8_rows_long<KIND, RES>, p)
                   : warp ? (vec ? cudaLaunchKernelEx(&cfg, k_int8_rows<KIND, RES, true, true>, p)
-                                : cudaLaunchKernelEx(&cfg, k_int8_rows<KIND, RES, false, true>, p))
+                                : cudaLaunchKernelEx(&cfg, k_int8_rows<KIND, RES, !kAny, true>, p))
                          : (vec ? cudaLaunchKernelEx(&cfg, k_int8_rows<KIND, RES, true, false>, p)
-                                : cudaLaunchKernelEx(&cfg, k_int8_rows<KIND, RES, false, false>, p));
+                                : cudaLaunchKernelEx(&cfg, k_int8_rows<KIND, RES, !kAny, false>, p));
   return e == cudaSuccess ? cudaGetLastError() : e;
 }
 
@@ -390,13 +353,8 @@ int run_int8_rows(const Int8Rows& r, cudaStream_t stream, std::string* err) {
   p.q = r.q;
   p.ldq = r.ldq;
   p.scale = r.scale;
-  p.up_k = static_cast<int>(r.up_k);
-  p.up_scale = r.up_scale;
-  p.bound = r.bound;
-  p.b_scale = r.b_scale;
-  p.bias = r.bias;
-  p.bound_n = r.bound_n;
-  p.bound_out = r.bound_out;
+  p.hidden_max = r.hidden_max;
+  p.ldm = r.ldm;
   p.zero = static_cast<uint4*>(r.zero);
   p.zero_vecs = static_cast<int64_t>(r.zero_bytes / 16);
   const bool norm = r.kind == kInt8RowsNorm, res = norm && r.residual;
