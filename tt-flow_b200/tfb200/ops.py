@@ -260,86 +260,116 @@ def residual_add(partial: torch.Tensor, residual: torch.Tensor, out: torch.Tenso
 
 # ------------------------------------------------- 8-bit integer operators
 
-_DTYPES = {torch.bfloat16: L.TFB200_BF16, torch.float32: L.TFB200_F32, torch.int8: L.TFB200_I8}
 _GELU_INT8 = {**_GELU, "none": L.TFB200_GELU_NONE, None: L.TFB200_GELU_NONE}
+_DTYPES = {torch.bfloat16: L.TFB200_BF16, torch.float32: L.TFB200_F32, torch.int8: L.TFB200_I8}
+
+# A decode step makes these calls while the GPU waits for them, so each looks at a tensor once: ``_rows`` and ``_out``
+# return the operand's C descriptor beside its shape, and the device and stream are read without building the objects
+# torch.cuda's accessors return (25 us a product with them, 13 us without).
 
 
-def _rows(t: torch.Tensor, name: str, dtype: torch.dtype, cols: int | None = None) -> torch.Tensor:
-    """The operand as rows (leading dimensions flattened) with unit column stride and rows that do not overlap; a
-    view that is not is copied."""
+def _bad(t, name: str, dtype: torch.dtype, dev: torch.device | None):
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        raise TypeError(f"{name} must be a CUDA tensor")
+        return TypeError(f"{name} must be a CUDA tensor")
     if t.dtype != dtype:
-        raise TypeError(f"{name} must be {dtype} (got {t.dtype})")
-    if t.dim() < 2:
-        raise ValueError(f"{name} must have at least 2 dimensions")
-    if cols is not None and t.shape[-1] != cols:
-        raise ValueError(f"{name} has {t.shape[-1]} columns, expected {cols}")
-    if t.dim() > 2:
+        return TypeError(f"{name} must be {dtype} (got {t.dtype})")
+    return ValueError(f"{name} is on {t.device}; the other operands are on {dev}")
+
+
+def _rows(t: torch.Tensor, name: str, dtype: torch.dtype, dev: torch.device | None = None, two_d: bool = False):
+    """(rows, columns, tfb200_mat, tensor) of an operand: leading dimensions flattened, unit column stride, rows that
+    do not overlap. A view that is not so is copied; the tensor keeps the memory alive."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != dtype or (dev is not None and t.device != dev):
+        raise _bad(t, name, dtype, dev)
+    n = t.dim()
+    if n != 2:
+        if n < 2 or two_d:
+            raise ValueError(f"{name} must have {'' if two_d else 'at least '}2 dimensions (got {n})")
         t = t.reshape(math.prod(t.shape[:-1]), t.shape[-1])
-    if (t.stride(1) != 1 and t.shape[1] > 1) or (t.stride(0) < t.shape[1] and t.shape[0] > 1):
+    rows, cols = t.shape
+    ld, unit = t.stride()
+    if (unit != 1 and cols > 1) or (ld < cols and rows > 1):
         t = t.contiguous()
-    return t
+        ld = cols
+    return rows, cols, L.Mat(t.data_ptr(), rows, cols, ld if rows > 1 and ld > 0 else max(cols, 1), _DTYPES[dtype]), t
 
 
-def _out(t: torch.Tensor, name: str, dtype: torch.dtype, shape) -> torch.Tensor:
-    """A caller's output, as rows that are written in place."""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        raise TypeError(f"{name} must be a CUDA tensor")
-    if t.dtype != dtype:
-        raise TypeError(f"{name} must be {dtype} (got {t.dtype})")
+def _out(t: torch.Tensor, name: str, dtype: torch.dtype, shape, dev: torch.device):
+    """``_rows`` of a caller's output, which is written in place: nothing is copied."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != dtype or t.device != dev:
+        raise _bad(t, name, dtype, dev)
     if tuple(t.shape) != tuple(shape):
         raise ValueError(f"{name} must be {list(shape)} (got {list(t.shape)})")
-    if t.dim() == 1:
-        if not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous")
-        return t
-    try:
-        r = t.view(-1, t.shape[-1]) if t.dim() > 2 and t.numel() else t.reshape(math.prod(shape[:-1]), shape[-1])
-    except RuntimeError:
-        raise ValueError(f"{name}: the leading dimensions must flatten into rows without a copy") from None
-    if (r.shape[1] > 1 and r.stride(1) != 1) or (r.shape[0] > 1 and r.stride(0) < r.shape[1]):
+    if t.dim() > 2:
+        try:
+            t = t.view(math.prod(shape[:-1]), shape[-1])
+        except RuntimeError:
+            raise ValueError(f"{name}: the leading dimensions must flatten into rows without a copy") from None
+    r = _rows(t, name, dtype)
+    if r[3].data_ptr() != t.data_ptr():
         raise ValueError(f"{name} must have unit column stride and rows that do not overlap")
     return r
 
 
-def _scales(t: torch.Tensor, n: int, name: str) -> torch.Tensor:
-    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.float32:
-        raise TypeError(f"{name} must be a CUDA float32 tensor")
-    if t.numel() != n:
-        raise ValueError(f"{name} has {t.numel()} elements, expected {n}")
-    return t.reshape(-1).contiguous()
+def _out_scale(t: torch.Tensor, n: int, dev: torch.device) -> int:
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.float32 or t.device != dev:
+        raise _bad(t, "scale", torch.float32, dev)
+    if t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"scale must be contiguous and have {n} elements (got {list(t.shape)})")
+    return t.data_ptr()
 
 
-def _mat(t: torch.Tensor | None):
-    """tfb200_mat (by reference) of rows from ``_rows`` / ``_out``; NULL for None."""
+def _vec1(t, n: int, name: str, dtype: torch.dtype, dev: torch.device):
+    """A contiguous vector of n elements (any shape), or None."""
     if t is None:
         return None
-    rows, cols = t.shape
-    return ctypes.byref(L.Mat(t.data_ptr(), rows, cols, t.stride(0) if rows > 1 else max(cols, 1), _DTYPES[t.dtype]))
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != dtype or t.device != dev:
+        raise _bad(t, name, dtype, dev)
+    if t.numel() != n:
+        raise ValueError(f"{name} has {t.numel()} elements, expected {n}")
+    return t if t.is_contiguous() else t.reshape(-1).contiguous()
+
+
+def _space(need: int, ws: torch.Tensor | None, dev: torch.device):
+    """(tensor, address, bytes) of the workspace of a call that needs `need` bytes."""
+    if ws is None and need == 0:
+        return None, None, 0
+    ws = _workspace(need, ws, dev)
+    return ws, ws.data_ptr(), ws.numel() * ws.element_size()
+
+
+def _call(dev: torch.device, fn, *args) -> None:
+    """One C call with ``dev`` current; a ``_call`` among ``args`` stands for dev's current stream."""
+    i = dev.index
+    s = torch._C._cuda_getCurrentRawStream(i)
+    args = [s if a is _call else a for a in args]
+    if torch._C._cuda_getDevice() == i:
+        rc = fn(*args)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args)
+    if rc:
+        L.check(rc)
+
+
+def _ref(r):
+    return None if r is None else ctypes.byref(r[2])
 
 
 def _ptr(t: torch.Tensor | None):
     return None if t is None else t.data_ptr()
 
 
-def _call(dev: torch.device, fn: str, *args) -> None:
-    """One C call with ``dev`` current; the string "stream" among ``args`` stands for dev's current stream."""
-    s = torch.cuda.current_stream(dev).cuda_stream
-    f, a = getattr(L.lib(), fn), [s if isinstance(x, str) else x for x in args]
-    if torch.cuda.current_device() == dev.index:
-        L.check(f(*a))
-    else:
-        with torch.cuda.device(dev):
-            L.check(f(*a))
-
-
-def _int8_empty(shape, rows: int, device) -> tuple[torch.Tensor, torch.Tensor]:
-    """A new int8 tensor of ``shape``, and as rows, that start a multiple of 16 bytes apart: what the products read
-    best."""
+def _new_int8(shape, rows: int, dev):
+    """A new int8 tensor of ``shape``, and as ``_rows``: its rows start a multiple of 16 bytes apart, as the products
+    read best."""
     k = shape[-1]
-    q2 = torch.empty(rows, (k + 15) // 16 * 16, dtype=torch.int8, device=device)[:, :k]
-    return (q2 if len(shape) == 2 else q2.unflatten(0, shape[:-1])), q2
+    ld = (k + 15) // 16 * 16
+    q = torch.empty(rows, ld, dtype=torch.int8, device=dev)
+    mat = L.Mat(q.data_ptr(), rows, k, max(ld, 1), L.TFB200_I8)
+    if ld != k:
+        q = q[:, :k]
+    return (q if len(shape) == 2 else q.unflatten(0, shape[:-1])), (rows, k, mat, q)
 
 
 def quantize_int8(x: torch.Tensor, out: tuple | None = None) -> tuple[torch.Tensor, torch.Tensor]:
@@ -350,17 +380,16 @@ def quantize_int8(x: torch.Tensor, out: tuple | None = None) -> tuple[torch.Tens
     a returned ``q`` start 16 bytes apart or a multiple of it (its row stride may exceed its width); the products
     accept other strides but run slower on them. ``out = (q, scale)`` takes the results in place.
     """
-    x2 = _rows(x, "x", torch.bfloat16)
-    rows = x2.shape[0]
+    xr = _rows(x, "x", torch.bfloat16)
+    rows, dev = xr[0], x.device
     if out is None:
-        q, q2 = _int8_empty(x.shape, rows, x.device)
-        scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+        q, qr = _new_int8(x.shape, rows, dev)
+        scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
+        sp = scale.data_ptr()
     else:
         q, scale = out
-        q2 = _out(q, "q", torch.int8, x.shape)
-        _out(scale.reshape(-1) if scale.is_contiguous() else scale, "scale", torch.float32, (rows,))
-    dev = _device_of(("x", x), ("q", q), ("scale", scale))
-    _call(dev, "tfb200_quantize_int8", _mat(x2), _mat(q2), _ptr(scale), "stream")
+        qr, sp = _out(q, "q", torch.int8, x.shape, dev), _out_scale(scale, rows, dev)
+    _call(dev, L.lib().tfb200_quantize_int8, _ref(xr), _ref(qr), sp, _call)
     return q, scale
 
 
@@ -370,37 +399,44 @@ def rmsnorm_int8(x: torch.Tensor, gamma: torch.Tensor, eps: float = 1e-6, residu
     ``(q, scale, sum)`` of ``rmsnorm(x + residual, gamma, eps)`` and ``sum = bf16(x + residual)``. The norm and ``q``
     are taken from the unrounded sum. ``out`` takes the results in place; its ``sum`` may be ``x`` or ``residual``.
     """
-    x2 = _rows(x, "x", torch.bfloat16)
-    rows, K = x2.shape
-    g = _vec(gamma, K, "gamma")
-    r2 = None
+    xr = _rows(x, "x", torch.bfloat16)
+    rows, K, dev = xr[0], xr[1], x.device
+    g = _vec1(gamma, K, "gamma", torch.bfloat16, dev)
+    rr = tr = total = None
     if residual is not None:
+        rr = _rows(residual, "residual", torch.bfloat16, dev)
         if residual.shape != x.shape:
             raise ValueError(f"residual must have the shape of x (got {list(residual.shape)})")
-        r2 = _rows(residual, "residual", torch.bfloat16)
-    total = t2 = None
     if out is None:
-        q, q2 = _int8_empty(x.shape, rows, x.device)
-        scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-        if r2 is not None:
-            total = torch.empty(x.shape, dtype=torch.bfloat16, device=x.device)
-            t2 = total.view(rows, K)
+        q, qr = _new_int8(x.shape, rows, dev)
+        scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
+        sp = scale.data_ptr()
+        if rr is not None:
+            total = torch.empty(x.shape, dtype=torch.bfloat16, device=dev)
+            tr = (rows, K, L.Mat(total.data_ptr(), rows, K, max(K, 1), L.TFB200_BF16), total)
     else:
         if len(out) != (2 if residual is None else 3):
             raise ValueError("out must be (q, scale), and (q, scale, sum) with a residual")
         q, scale = out[:2]
-        q2 = _out(q, "q", torch.int8, x.shape)
-        _out(scale.reshape(-1) if scale.is_contiguous() else scale, "scale", torch.float32, (rows,))
-        if r2 is not None:
+        qr, sp = _out(q, "q", torch.int8, x.shape, dev), _out_scale(scale, rows, dev)
+        if rr is not None:
             total = out[2]
-            t2 = _out(total, "sum", torch.bfloat16, x.shape)
-    dev = _device_of(("x", x), ("gamma", gamma), ("residual", residual), ("q", q), ("scale", scale), ("sum", total))
-    _call(dev, "tfb200_rmsnorm_int8", _mat(x2), _mat(r2), _ptr(g), eps, _mat(t2), _mat(q2), _ptr(scale), "stream")
+            tr = _out(total, "sum", torch.bfloat16, x.shape, dev)
+    _call(dev, L.lib().tfb200_rmsnorm_int8, _ref(xr), _ref(rr), _ptr(g), eps, _ref(tr), _ref(qr), sp, _call)
     return (q, scale) if residual is None else (q, scale, total)
 
 
+def _result(x: torch.Tensor, rows: int, n: int, dtype: torch.dtype, out: torch.Tensor | None):
+    """A product's output, [..., N] for an input [..., K] (a caller's may also be given as [rows, N])."""
+    if out is None:
+        y = torch.empty(rows, n, dtype=dtype, device=x.device)
+        r = (rows, n, L.Mat(y.data_ptr(), rows, n, max(n, 1), _DTYPES[dtype]), y)
+        return (y if x.dim() == 2 else y.view(*x.shape[:-1], n)), r
+    return out, _out(out, "out", dtype, (rows, n) if out.dim() == 2 else (*x.shape[:-1], n), x.device)
+
+
 def matmul_int8_workspace_bytes(m: int, k: int, n: int) -> int:
-    return int(L.lib().tfb200_matmul_int8_workspace_size(m, k, n))
+    return L.lib().tfb200_matmul_int8_workspace_size(m, k, n)
 
 
 def matmul_int8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor,
@@ -411,41 +447,34 @@ def matmul_int8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale
     per row of each; exact integer sums, the rest in fp32, rounded once to ``out_dtype`` (bf16 or fp32). ``bias`` is
     bf16 ``[N]``, ``gelu`` "erf", "tanh" or None, ``residual`` bf16 ``[..., N]``. K is at most 131071.
     """
-    a2 = _rows(a, "a", torch.int8)
-    if isinstance(b, torch.Tensor) and b.dim() != 2:
-        raise ValueError("b must be [N, K]")
-    b2 = _rows(b, "b", torch.int8)
-    M, K = a2.shape
-    N = b2.shape[0]
-    if b2.shape[1] != K:
-        raise ValueError(f"matmul_int8: a has K={K} but b has {b2.shape[1]} columns")
-    if out_dtype not in (torch.bfloat16, torch.float32):
+    ar = _rows(a, "a", torch.int8)
+    M, K, dev = ar[0], ar[1], a.device
+    br = _rows(b, "b", torch.int8, dev, True)
+    N = br[0]
+    if br[1] != K:
+        raise ValueError(f"matmul_int8: a has K={K} but b has {br[1]} columns")
+    if out_dtype is not torch.bfloat16 and out_dtype is not torch.float32:
         raise TypeError(f"out_dtype must be bfloat16 or float32 (got {out_dtype})")
     if gelu not in _GELU_INT8:
         raise ValueError(f"gelu must be 'erf', 'tanh' or None (got {gelu!r})")
-    sa, sb = _scales(a_scale, M, "a_scale"), _scales(b_scale, N, "b_scale")
-    bv = _vec(bias, N, "bias")
-    r2 = None
+    sa = _vec1(a_scale, M, "a_scale", torch.float32, dev)
+    sb = _vec1(b_scale, N, "b_scale", torch.float32, dev)
+    bv = _vec1(bias, N, "bias", torch.bfloat16, dev)
+    rr = None
     if residual is not None:
-        r2 = _rows(residual, "residual", torch.bfloat16, N)
-        if r2.shape[0] != M:
+        rr = _rows(residual, "residual", torch.bfloat16, dev)
+        if rr[0] != M or rr[1] != N:
             raise ValueError(f"residual must be [{M},{N}] (got {list(residual.shape)})")
-    shape = (*a.shape[:-1], N)
-    if out is None:
-        y = torch.empty(M, N, dtype=out_dtype, device=a.device)
-        y2 = y
-    else:
-        y, y2 = out, _out(out, "out", out_dtype, shape if out.dim() != 2 else (M, N))
-    dev = _device_of(("a", a), ("a_scale", a_scale), ("b", b), ("b_scale", b_scale), ("bias", bias),
-                     ("residual", residual), ("out", out))
-    ws = _workspace(matmul_int8_workspace_bytes(M, K, N), workspace, dev)
-    _call(dev, "tfb200_matmul_int8", _mat(a2), _ptr(sa), _mat(b2), _ptr(sb), _ptr(bv), _GELU_INT8[gelu], _mat(r2),
-          _mat(y2), "stream", _ptr(ws), ws.numel() * ws.element_size())
-    return y if out is not None or a.dim() == 2 else y.view(shape)
+    y, yr = _result(a, M, N, out_dtype, out)
+    lib = L.lib()
+    ws, wp, wn = _space(lib.tfb200_matmul_int8_workspace_size(M, K, N), workspace, dev)
+    _call(dev, lib.tfb200_matmul_int8, _ref(ar), _ptr(sa), _ref(br), _ptr(sb), _ptr(bv), _GELU_INT8[gelu], _ref(rr),
+          _ref(yr), _call, wp, wn)
+    return y
 
 
 def rmsnorm_matmul_int8_workspace_bytes(m: int, k: int, n: int) -> int:
-    return int(L.lib().tfb200_fused_rmsnorm_matmul_int8_workspace_size(m, k, n))
+    return L.lib().tfb200_fused_rmsnorm_matmul_int8_workspace_size(m, k, n)
 
 
 def fused_rmsnorm_matmul_int8(x: torch.Tensor, gamma: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
@@ -453,27 +482,24 @@ def fused_rmsnorm_matmul_int8(x: torch.Tensor, gamma: torch.Tensor, w: torch.Ten
                               workspace: torch.Tensor | None = None) -> torch.Tensor:
     """``rmsnorm(x, gamma, eps) @ w`` on int8 ``w [N, K]`` with ``w_scale [N]``: ``fused_rmsnorm_matmul`` with the
     normalised rows quantised per token (``rmsnorm_int8``, then ``matmul_int8``)."""
-    x2 = _rows(x, "x", torch.bfloat16)
-    if isinstance(w, torch.Tensor) and w.dim() != 2:
-        raise ValueError("w must be [N, K]")
-    w2 = _rows(w, "w", torch.int8)
-    M, K = x2.shape
-    N = w2.shape[0]
-    if w2.shape[1] != K:
-        raise ValueError(f"fused_rmsnorm_matmul_int8: x has K={K} but w has {w2.shape[1]} columns")
-    g, ws1 = _vec(gamma, K, "gamma"), _scales(w_scale, N, "w_scale")
-    shape = (*x.shape[:-1], N)
-    y = torch.empty(M, N, dtype=torch.bfloat16, device=x.device) if out is None else out
-    y2 = y if out is None else _out(out, "out", torch.bfloat16, shape if out.dim() != 2 else (M, N))
-    dev = _device_of(("x", x), ("gamma", gamma), ("w", w), ("w_scale", w_scale), ("out", out))
-    ws = _workspace(rmsnorm_matmul_int8_workspace_bytes(M, K, N), workspace, dev)
-    _call(dev, "tfb200_fused_rmsnorm_matmul_int8", _mat(x2), _ptr(g), _mat(w2), _ptr(ws1), eps, _mat(y2), "stream",
-          _ptr(ws), ws.numel() * ws.element_size())
-    return y if out is not None or x.dim() == 2 else y.view(shape)
+    xr = _rows(x, "x", torch.bfloat16)
+    M, K, dev = xr[0], xr[1], x.device
+    wr = _rows(w, "w", torch.int8, dev, True)
+    N = wr[0]
+    if wr[1] != K:
+        raise ValueError(f"fused_rmsnorm_matmul_int8: x has K={K} but w has {wr[1]} columns")
+    g = _vec1(gamma, K, "gamma", torch.bfloat16, dev)
+    sw = _vec1(w_scale, N, "w_scale", torch.float32, dev)
+    y, yr = _result(x, M, N, torch.bfloat16, out)
+    lib = L.lib()
+    ws, wp, wn = _space(lib.tfb200_fused_rmsnorm_matmul_int8_workspace_size(M, K, N), workspace, dev)
+    _call(dev, lib.tfb200_fused_rmsnorm_matmul_int8, _ref(xr), _ptr(g), _ref(wr), _ptr(sw), eps, _ref(yr), _call, wp,
+          wn)
+    return y
 
 
 def mlp_int8_workspace_bytes(m: int, k: int, h: int, n: int) -> int:
-    return int(L.lib().tfb200_fused_mlp_int8_workspace_size(m, k, h, n))
+    return L.lib().tfb200_fused_mlp_int8_workspace_size(m, k, h, n)
 
 
 def fused_mlp_int8(x: torch.Tensor, gamma: torch.Tensor, w1: torch.Tensor, w1_scale: torch.Tensor,
@@ -482,27 +508,24 @@ def fused_mlp_int8(x: torch.Tensor, gamma: torch.Tensor, w1: torch.Tensor, w1_sc
                    workspace: torch.Tensor | None = None) -> torch.Tensor:
     """``fused_mlp`` on int8 ``w1 [H, K]`` and ``w2 [N, H]`` with a scale per row: the normalised rows and the hidden
     block are quantised per token. ``b1`` is a bf16 ``[H]`` bias or None."""
-    x2 = _rows(x, "x", torch.bfloat16)
-    if any(isinstance(w, torch.Tensor) and w.dim() != 2 for w in (w1, w2)):
-        raise ValueError("w1 must be [H, K] and w2 [N, H]")
-    W1, W2 = _rows(w1, "w1", torch.int8), _rows(w2, "w2", torch.int8)
-    M, K = x2.shape
-    H, N = W1.shape[0], W2.shape[0]
-    if W1.shape[1] != K or W2.shape[1] != H:
+    xr = _rows(x, "x", torch.bfloat16)
+    M, K, dev = xr[0], xr[1], x.device
+    w1r, w2r = _rows(w1, "w1", torch.int8, dev, True), _rows(w2, "w2", torch.int8, dev, True)
+    H, N = w1r[0], w2r[0]
+    if w1r[1] != K or w2r[1] != H:
         raise ValueError("fused_mlp_int8: shapes do not chain (x[M,K], w1[H,K], w2[N,H])")
-    r2 = _rows(residual, "residual", torch.bfloat16, N)
-    if r2.shape[0] != M:
+    rr = _rows(residual, "residual", torch.bfloat16, dev)
+    if rr[0] != M or rr[1] != N:
         raise ValueError(f"fused_mlp_int8: residual must be [{M},{N}] (got {list(residual.shape)})")
     if gelu not in _GELU:
         raise ValueError(f"gelu must be 'erf' or 'tanh' (got {gelu!r})")
-    g, b = _vec(gamma, K, "gamma"), _vec(b1, H, "b1")
-    s1, s2 = _scales(w1_scale, H, "w1_scale"), _scales(w2_scale, N, "w2_scale")
-    shape = (*x.shape[:-1], N)
-    y = torch.empty(M, N, dtype=torch.bfloat16, device=x.device) if out is None else out
-    y2 = y if out is None else _out(out, "out", torch.bfloat16, shape if out.dim() != 2 else (M, N))
-    dev = _device_of(("x", x), ("gamma", gamma), ("w1", w1), ("w1_scale", w1_scale), ("b1", b1), ("w2", w2),
-                     ("w2_scale", w2_scale), ("residual", residual), ("out", out))
-    ws = _workspace(mlp_int8_workspace_bytes(M, K, H, N), workspace, dev)
-    _call(dev, "tfb200_fused_mlp_int8", _mat(x2), _ptr(g), _mat(W1), _ptr(s1), _ptr(b), _mat(W2), _ptr(s2), _mat(r2),
-          eps, _GELU[gelu], _mat(y2), "stream", _ptr(ws), ws.numel() * ws.element_size())
-    return y if out is not None or x.dim() == 2 else y.view(shape)
+    g = _vec1(gamma, K, "gamma", torch.bfloat16, dev)
+    b = _vec1(b1, H, "b1", torch.bfloat16, dev)
+    s1 = _vec1(w1_scale, H, "w1_scale", torch.float32, dev)
+    s2 = _vec1(w2_scale, N, "w2_scale", torch.float32, dev)
+    y, yr = _result(x, M, N, torch.bfloat16, out)
+    lib = L.lib()
+    ws, wp, wn = _space(lib.tfb200_fused_mlp_int8_workspace_size(M, K, H, N), workspace, dev)
+    _call(dev, lib.tfb200_fused_mlp_int8, _ref(xr), _ptr(g), _ref(w1r), _ptr(s1), _ptr(b), _ref(w2r), _ptr(s2),
+          _ref(rr), eps, _GELU[gelu], _ref(yr), _call, wp, wn)
+    return y
