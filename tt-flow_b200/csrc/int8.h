@@ -58,6 +58,10 @@ struct Int8Gemm {
   // b_scale (it is this library's own staging launch), so their first tiles may
   // be requested before it has completed.
   bool b_stable = false;
+  // Few rows only: the weights [next_n, next_k] of the product that follows on
+  // the stream, the first of which are brought into L2 while this one drains.
+  const int8_t* next_b = nullptr;
+  int64_t next_n = 0, next_k = 0, next_ld = 0;
 };
 
 // Device workspace of one product: `clear_bytes` of counters, zero on entry,
@@ -67,6 +71,14 @@ struct Int8GemmWs {
 };
 Int8GemmWs int8_gemm_ws(int64_t m, int64_t n, int64_t k);
 int run_int8_gemm(const Int8Gemm& g, cudaStream_t stream, std::string* err);
+
+// Few rows (int8_stream.cu); operands as run_int8_gemm checks them for TMA.
+constexpr int64_t kInt8StreamRows = 128;
+Int8GemmWs int8_stream_ws(int64_t m, int64_t n);
+int run_int8_stream(const Int8Gemm& g, cudaStream_t stream, std::string* err);
+// Tensor map of an int8 matrix in boxes of 128 columns (int8_gemm.cu).
+bool int8_map(CUtensorMap* m, const int8_t* base, int64_t rows, int64_t cols, int64_t ld, uint32_t box_rows,
+              std::string* err);
 
 // One row at a time: q = rn(t * 127 / amax_k |t|) with t = x (kInt8RowsQuant),
 // t = (x + residual) * gamma with scale = amax / (127 rms) (kInt8RowsNorm), or

@@ -363,6 +363,10 @@ int tfb200_fused_mlp_int8(const tfb200_mat* x, const void* gamma, const tfb200_m
     up.ldm = hl.ldm;
     up.ws = ws + l.up;
     up.b_stable = true;
+    up.next_b = static_cast<const int8_t*>(w2->data);
+    up.next_n = N;
+    up.next_k = H;
+    up.next_ld = w2->ld;
     rc = run_int8_gemm(up, s, &err);
     if (rc) return fail(rc, fn, "up projection: " + err);
     // The hidden block, per token.

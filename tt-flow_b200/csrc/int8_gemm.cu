@@ -35,7 +35,7 @@ __device__ __forceinline__ uint32_t load4(const int8_t* p, int k, int K) {
 
 __global__ void __launch_bounds__(256) k_int8_gemm_any(const int8_t* A, int64_t lda, const int8_t* B, int64_t ldb,
                                                        const Int8Epi e) {
-  __shared__ uint32_t sa[kAnyTile][kAnyK / 4 + 1], sb[kAnyTile][kAnyK / 4 + 1];
+  __shared__ uint32_t sa[kAnyTile][kAnyK / 4 + 1], sb[kAnyTile][kAnyK / 4 + 1], sums[kAnyTile * kAnyTile];
   const int64_t m0 = static_cast<int64_t>(blockIdx.x) * kAnyTile;
   const int row = threadIdx.x >> 2, seg = (threadIdx.x & 3) * 4;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
@@ -66,44 +66,32 @@ __global__ void __launch_bounds__(256) k_int8_gemm_any(const int8_t* A, int64_t 
       }
       __syncthreads();
     }
+    // The sums go through shared memory to eight neighbouring columns of a row
+    // per thread.
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int64_t m = m0 + ty + 16 * i;
-      if (m >= e.M) break;
-      const float s = e.a_scale[m];
-      if (e.out != kInt8OutHidden) {
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int64_t n = n0 + tx + 16 * j;
-          if (n < e.N) int8_store(e, acc[i][j], s, m, static_cast<int>(n));
-        }
-        continue;
-      }
-      // Two blocks of 32 columns, each held by 16 neighbouring lanes.
+      for (int j = 0; j < 4; ++j) sums[(ty + 16 * i) * kAnyTile + tx + 16 * j] = static_cast<uint32_t>(acc[i][j]);
+    __syncthreads();
+#pragma unroll 1
+    for (int it = threadIdx.x; it < kAnyTile * kAnyTile / 8; it += 256) {
+      const int64_t m = m0 + it / (kAnyTile / 8);
+      const int c = it % (kAnyTile / 8) * 8;
+      const int n = static_cast<int>(n0) + c;
+      const bool in = m < e.M && n < e.N;
+      uint32_t v[8];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float v[2];
-        uint32_t amax = 0;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int64_t n = n0 + tx + 16 * (2 * h + j);
-          v[j] = n < e.N ? int8_value(e, acc[i][2 * h + j], s, static_cast<int>(n)) : 0.0f;
-          amax = max(amax, mag(v[j]));
-        }
-        // The 16 lanes hold one row: all of them are here.
-        const unsigned lanes = 0xFFFFu << (threadIdx.x & 16);
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(lanes, amax, o));
-        const UpScale us = up_scale(amax, 32767.0f);
-        const int64_t block = n0 / kHiddenBlock + h;
-        if (tx == 0 && block < e.ldm) e.hidden_max[m * e.ldm + block] = hidden_max(amax);
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int64_t n = n0 + tx + 16 * (2 * h + j);
-          if (n < e.N) static_cast<int16_t*>(e.C)[m * e.ldc + n] = static_cast<int16_t>(hidden_bits(v[j], us) & 0xFFFFu);
-        }
+      for (int j = 0; j < 8; ++j) v[j] = sums[it / (kAnyTile / 8) * kAnyTile + c + j];
+      float f[8] = {};
+      if (in) int8_values(e, v, e.a_scale[m], int8_cols(e, n, e.vec_cols), f);
+      if (e.out == kInt8OutHidden) {
+        int8_store_hidden(e, m, n, in, f);
+      } else if (in) {
+        if (e.residual) int8_residual(e, m, n, e.vec_res, f);
+        int8_store(e, m, n, e.vec_out, f);
       }
     }
+    __syncthreads();
   }
 }
 
@@ -128,15 +116,20 @@ struct PairCtl {
   uint64_t drain;
   uint32_t tmem_base;
   int abort;
+  // Scales and bias of the tile's columns, for the epilogue. Read from global
+  // memory chunk by chunk they cost an L2 round trip each behind the operands'
+  // traffic, longer than the products of a 4096-deep tile.
+  alignas(16) float sb[kBN];
+  alignas(16) uint16_t bias[kBN];
 };
 
 constexpr size_t kPairSmem =
     1024 + 2 * kStages * kTileBytes + static_cast<size_t>(kEpiWarps) * 2 * kStageOut + sizeof(PairCtl);
+static_assert(kPairSmem <= 227 * 1024, "shared memory of one CTA");
 
 struct PairParams {
   Int8Epi e;
-  int vec_ok;     // scales, bias and residual allow 16-byte loads
-  int tma_store;  // C is stored through shared memory with TMA
+  int fast;  // the residual and C are laid out in 16-byte steps; C is stored with TMA
   int b_prefetch;
   sched::PairSched ps;
   int32_t* slots;
@@ -154,70 +147,27 @@ __device__ __forceinline__ void tile_of(int t, int num_m, int num_n, int& tm, in
   tn = local / rows;
 }
 
+// Work item i of a pair: the full waves' tiles, then one piece of the split last
+// wave. The last `rem` pairs keep k-blocks [0, kc) of its tiles and finish them;
+// of the pairs before them, pair g takes part g (tile g / parts).
+struct Work {
+  int tile, k0, k1, role, slot;
+};
+__device__ __forceinline__ int item_count(const sched::PairSched& s, int p) {
+  if (s.rem == 0) return p < s.tiles ? (s.tiles - 1 - p) / s.pairs + 1 : 0;
+  return s.waves + (p >= s.pairs - s.rem || p < s.rem * s.parts ? 1 : 0);
+}
+__device__ __forceinline__ Work item_at(const sched::PairSched& s, int p, int i) {
+  if (s.rem == 0 || i < s.waves) return {p + i * s.pairs, 0, s.kblocks, sched::kFull, 0};
+  const int base = s.waves * s.pairs, r = p - (s.pairs - s.rem);
+  if (r >= 0) return {base + r, 0, s.kc, sched::kMain, r * s.parts};
+  const int j = p % s.parts, tail = s.kblocks - s.kc;
+  return {base + p / s.parts, s.kc + tail * j / s.parts, s.kc + tail * (j + 1) / s.parts, sched::kPart, p};
+}
+
 __device__ __forceinline__ void give_up(PairCtl* ctl, int* status) {
   ctl->abort = 1;
   atomicExch(status, kDevTimeout);
-}
-
-// 32 columns of one row, col0 .. col0 + 31, finished in fp32 (0 past the matrix).
-__device__ __forceinline__ void finish32(const PairParams& p, const uint32_t (&v)[32], float sa, int64_t row,
-                                         int col0, float (&f)[32]) {
-  const Int8Epi& e = p.e;
-  if (p.vec_ok && col0 + 32 <= e.N) {
-    const float4* sp = reinterpret_cast<const float4*>(e.b_scale + col0);
-    if (e.bias) {
-      const uint4* bp = reinterpret_cast<const uint4*>(e.bias + col0);
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const float4 s0 = __ldg(sp + 2 * u), s1 = __ldg(sp + 2 * u + 1);
-        const uint4 b = __ldg(bp + u);
-        const float s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
-        const uint32_t w[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          f[8 * u + j] = int8_scaled(static_cast<int32_t>(v[8 * u + j]), sa, s[j],
-                                     (j & 1) ? bf16_hi(w[j >> 1]) : bf16_lo(w[j >> 1]));
-      }
-    } else {
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const float4 s4 = __ldg(sp + u);
-        const float s[4] = {s4.x, s4.y, s4.z, s4.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) f[4 * u + j] = int8_scaled(static_cast<int32_t>(v[4 * u + j]), sa, s[j]);
-      }
-    }
-    if (e.gelu == kGeluErf) {
-#pragma unroll
-      for (int j = 0; j < 32; ++j) f[j] = int8_gelu(f[j], kGeluErf);
-    } else if (e.gelu == kGeluTanh) {
-#pragma unroll
-      for (int j = 0; j < 32; ++j) f[j] = int8_gelu(f[j], kGeluTanh);
-    }
-    if (e.residual) {
-      const uint4* rp = reinterpret_cast<const uint4*>(e.residual + row * e.ldr + col0);
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const uint4 b = rp[u];
-        const uint32_t w[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          f[8 * u + 2 * j] = __fadd_rn(f[8 * u + 2 * j], bf16_lo(w[j]));
-          f[8 * u + 2 * j + 1] = __fadd_rn(f[8 * u + 2 * j + 1], bf16_hi(w[j]));
-        }
-      }
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      f[j] = 0.0f;
-      const int n = col0 + j;
-      if (n < e.N) {
-        f[j] = int8_value(e, static_cast<int32_t>(v[j]), sa, n);
-        if (e.residual) f[j] = __fadd_rn(f[j], __bfloat162float(e.residual[row * e.ldr + n]));
-      }
-    }
-  }
 }
 
 // 16 bytes at 16-byte unit u of the lane's row in a staged block (64-byte
@@ -228,6 +178,11 @@ __device__ __forceinline__ void stage16(uint32_t buf, int lane, int u, uint32_t 
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
+// Barrier of the four epilogue warps that share a half of the tile's columns.
+__device__ __forceinline__ void half_bar(int half) { asm volatile("bar.sync %0, 128;" ::"r"(half + 1) : "memory"); }
+
+// HIDDEN: C is the hidden block of an MLP (Int8Hidden), else bf16 or fp32.
+template <bool HIDDEN>
 __global__ void __launch_bounds__(cfg::kPairThreads, 1)
     k_int8_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                 const __grid_constant__ CUtensorMap tmC, const PairParams p) {
@@ -257,7 +212,7 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
     fence_mbar_init();
     tma_prefetch_desc(&tmA);
     tma_prefetch_desc(&tmB);
-    if (p.tma_store) tma_prefetch_desc(&tmC);
+    if (p.fast) tma_prefetch_desc(&tmC);
   }
   if (warp == 2) {
     tmem_alloc_pair(smem_u32(&ctl->tmem_base), 2 * kBN);
@@ -272,7 +227,7 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
 
   const int pair = blockIdx.x >> 1;
   const sched::PairSched& ps = p.ps;
-  const int nwork = sched::work_count(ps, pair);
+  const int nwork = item_count(ps, pair);
   const int num_m = (p.e.M + 2 * kBM - 1) / (2 * kBM);
   const int num_n = (p.e.N + kBN - 1) / kBN;
 
@@ -286,7 +241,7 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
       // requested while that kernel finishes; A follows after the wait.
       int npre = 0;
       if (p.b_prefetch && nwork > 0) {
-        const sched::Work w = sched::work_item(ps, pair, 0);
+        const Work w = item_at(ps, pair, 0);
         int tm, tn;
         tile_of(w.tile, num_m, num_n, tm, tn);
         npre = min(kStages, w.k1 - w.k0);
@@ -299,7 +254,7 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
       }
       grid_dep_wait();
       for (int i = 0; i < nwork && ok; ++i) {
-        const sched::Work w = sched::work_item(ps, pair, i);
+        const Work w = item_at(ps, pair, i);
         int tm, tn;
         tile_of(w.tile, num_m, num_n, tm, tn);
         for (int kb = w.k0; kb < w.k1; ++kb) {
@@ -338,7 +293,7 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
       uint32_t phase = 0;
       bool ok = true;
       for (int i = 0; i < nwork && ok; ++i) {
-        const sched::Work w = sched::work_item(ps, pair, i);
+        const Work w = item_at(ps, pair, i);
         const int acc = i & 1;
         const uint32_t use = static_cast<uint32_t>(i >> 1);
         if (!mbar_wait(smem_u32(&ctl->tempty[acc]), (use & 1u) ^ 1u, &ctl->abort, p.timeout_ns)) {
@@ -384,142 +339,218 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
     const int r = q * 32 + lane;
     const uint32_t bufs = smem_u32(sC) + static_cast<uint32_t>(ew * 2) * kStageOut;
     for (int i = 0; i < nwork; ++i) {
-      const sched::Work w = sched::work_item(ps, pair, i);
+      const Work w = item_at(ps, pair, i);
       int tm, tn;
       tile_of(w.tile, num_m, num_n, tm, tn);
       const int acc = i & 1;
       const uint32_t use = static_cast<uint32_t>(i >> 1);
-      bool ok = mbar_wait(smem_u32(&ctl->tfull[acc]), use & 1u, &ctl->abort, p.timeout_ns);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) {
-        if (lane == 0) give_up(ctl, p.status);
-        break;
-      }
-      tc_fence_after();
       const int64_t row0 = static_cast<int64_t>(tm) * 2 * kBM + static_cast<int64_t>(rank) * kBM + q * 32;
       const int64_t row = row0 + lane;
-      const uint32_t tacc = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * kBN);
+      const bool row_in = row < p.e.M;
       const bool part = w.role == sched::kPart, fix = w.role == sched::kMain;
-      const float sa = !part && row < p.e.M ? __ldg(p.e.a_scale + row) : 0.0f;
+      // While the tile's products run: the row's scale, a column's scale and bias
+      // per thread (four warps share a half's 128 columns), the residual into L2.
+      float sa = 0.0f;
+      if (!part) {
+        const int n = tn * kBN + c0 * 32 + r;
+        const float sb = n < p.e.N ? p.e.b_scale[n] : 0.0f;
+        const uint16_t bias = p.e.bias && n < p.e.N ? reinterpret_cast<const uint16_t*>(p.e.bias)[n] : uint16_t(0);
+        if (row_in) {
+          sa = p.e.a_scale[row];
+          if (!HIDDEN && p.e.residual)
+            for (int c = c0; c < c0 + kChunks && tn * kBN + c * 32 < p.e.N; c += 2)
+              prefetch_l2(p.e.residual + row * p.e.ldr + tn * kBN + c * 32);
+        }
+        half_bar(ew >> 2);  // the half's warps are done with the last tile's columns
+        ctl->sb[c0 * 32 + r] = sb;
+        ctl->bias[c0 * 32 + r] = bias;
+        half_bar(ew >> 2);
+      }
+      bool ok = mbar_wait(smem_u32(&ctl->tfull[acc]), use & 1u, &ctl->abort, p.timeout_ns);
+      ok = __all_sync(0xffffffffu, ok);
+      // A warp whose wait ran out goes on through the items, so that the other
+      // warps of its half meet it at their barriers; their waits end at once.
+      if (!ok) {
+        if (lane == 0) give_up(ctl, p.status);
+        continue;
+      }
+      tc_fence_after();
+      const uint32_t tacc = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * kBN);
+      int* const flags = p.flags + ((w.slot * 2 + static_cast<int>(rank)) * kEpiWarps + ew) * kChunks;
+      if (fix && row0 < p.e.M) {
+        // The parts of a split tile: lane (part, chunk) waits until all 32 rows of
+        // its chunk are in (acquire); the warp's barrier passes that on.
+        const int part_of = lane / kChunks, chunk = lane % kChunks;
+        if (part_of < ps.parts && tn * kBN + (c0 + chunk) * 32 < p.e.N) {
+          const int* f = flags + part_of * 2 * kEpiWarps * kChunks + chunk;
+          const uint64_t t0 = global_ns();
+          while (ok && ld_acquire_gpu(f) != 32)
+            if (ctl->abort || global_ns() - t0 > p.timeout_ns) ok = false;
+        }
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) {
+          if (lane == 0) give_up(ctl, p.status);
+          continue;
+        }
+      }
       float hmax[kChunks] = {};
-      for (int c = c0; ok && c < c0 + kChunks; ++c) {
+      for (int c = c0; c < c0 + kChunks; ++c) {
         const int col0 = tn * kBN + c * 32;
         if (col0 >= p.e.N || row0 >= p.e.M) break;  // warp-uniform: nothing of this block is in the matrix
+        // Slots: [chunk][column / 4][row][4], so that a warp's 16-byte accesses
+        // cover 512 contiguous bytes.
+        int4* slot = reinterpret_cast<int4*>(p.slots + (static_cast<int64_t>(w.slot) * 2 + rank) * (kBM * kBN)) +
+                     c * 8 * kBM + r;
+        uint4 res[4];
+        const bool whole = col0 + 32 <= p.e.N;
+        if (!HIDDEN && p.fast && p.e.residual && whole && row_in && !part) {
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            res[u] = *reinterpret_cast<const uint4*>(p.e.residual + row * p.e.ldr + col0 + u * 8);
+        }
         uint32_t v[32];
         tmem_ld_32cols(tacc + static_cast<uint32_t>(c * 32), v);
         tmem_wait_ld();
         if (part) {
-          // A helper's part: its 32 rows of the chunk go to the part's slot
-          // (layout [chunk][column / 4][row][4]); each lane then counts its row
-          // in on the chunk's flag (release).
-          int4* slot = reinterpret_cast<int4*>(p.slots + (static_cast<int64_t>(w.slot) * 2 + rank) * (kBM * kBN)) + r;
+          // A helper's rows of the chunk go to its slot; each lane then counts its
+          // row in on the chunk's flag (release).
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            __stcg(slot + (c * 8 + j) * kBM,
-                   make_int4(static_cast<int>(v[4 * j]), static_cast<int>(v[4 * j + 1]),
-                             static_cast<int>(v[4 * j + 2]), static_cast<int>(v[4 * j + 3])));
-          red_add_release_gpu(p.flags + ((w.slot * 2 + static_cast<int>(rank)) * kEpiWarps + ew) * kChunks + (c - c0),
-                              1);
+          for (int k = 0; k < 8; ++k)
+            __stcg(slot + k * kBM, make_int4(static_cast<int>(v[4 * k]), static_cast<int>(v[4 * k + 1]),
+                                             static_cast<int>(v[4 * k + 2]), static_cast<int>(v[4 * k + 3])));
+          red_add_release_gpu(flags + (c - c0), 1);
           continue;
         }
         if (fix) {
-          // The parts of a split tile, each once all its rows are in (acquire).
+#pragma unroll 2
           for (int j = 0; j < ps.parts; ++j) {
-            const int* f = p.flags + (((w.slot + j) * 2 + static_cast<int>(rank)) * kEpiWarps + ew) * kChunks + (c - c0);
-            const uint64_t t0 = global_ns();
-            while (ok && ld_acquire_gpu(f) != 32)
-              if (ctl->abort || global_ns() - t0 > p.timeout_ns) ok = false;
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            const int4* slot =
-                reinterpret_cast<const int4*>(p.slots + (static_cast<int64_t>(w.slot + j) * 2 + rank) * (kBM * kBN)) +
-                r + c * 8 * kBM;
 #pragma unroll
-            for (int j4 = 0; j4 < 8; ++j4) {
-              const int4 a = __ldcg(slot + j4 * kBM);
-              v[4 * j4] += static_cast<uint32_t>(a.x);
-              v[4 * j4 + 1] += static_cast<uint32_t>(a.y);
-              v[4 * j4 + 2] += static_cast<uint32_t>(a.z);
-              v[4 * j4 + 3] += static_cast<uint32_t>(a.w);
+            for (int k = 0; k < 8; ++k) {
+              const int4 add = __ldcg(slot + j * (kBM * kBN / 2) + k * kBM);
+              v[4 * k] += static_cast<uint32_t>(add.x);
+              v[4 * k + 1] += static_cast<uint32_t>(add.y);
+              v[4 * k + 2] += static_cast<uint32_t>(add.z);
+              v[4 * k + 3] += static_cast<uint32_t>(add.w);
             }
           }
-          if (!ok) {
-            if (lane == 0) give_up(ctl, p.status);
-            break;
-          }
         }
+        const uint32_t buf = bufs + (p.e.out == kInt8OutF32 ? 0u : static_cast<uint32_t>(c & 1) * kStageOut);
         float f[32];
-        if (row < p.e.M) {
-          finish32(p, v, sa, row, col0, f);
-        } else {
+        {
+          const float4* sb = reinterpret_cast<const float4*>(ctl->sb + c * 32);
+          const uint4* bias = reinterpret_cast<const uint4*>(ctl->bias + c * 32);
 #pragma unroll
-          for (int j = 0; j < 32; ++j) f[j] = 0.0f;
-        }
-        if (!p.tma_store) {
-          if (row < p.e.M) {
+          for (int u = 0; u < 4; ++u) {
+            const float4 s0 = sb[2 * u], s1 = sb[2 * u + 1];
+            const uint4 b = bias[u];
+            const float s8[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+            const uint32_t b8[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              if (col0 + j >= p.e.N) break;
-              if (p.e.out == kInt8OutF32)
-                static_cast<float*>(p.e.C)[row * p.e.ldc + col0 + j] = f[j];
-              else  // the hidden block is always stored with TMA
-                static_cast<bf16*>(p.e.C)[row * p.e.ldc + col0 + j] = __float2bfloat16_rn(f[j]);
-            }
+            for (int j = 0; j < 8; ++j)
+              f[u * 8 + j] = int8_scaled(static_cast<int32_t>(v[u * 8 + j]), sa, s8[j],
+                                         (j & 1) ? bf16_hi(b8[j >> 1]) : bf16_lo(b8[j >> 1]));
           }
+        }
+        if (p.e.gelu == kGeluErf) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) f[j] = int8_gelu(f[j], kGeluErf);
+        } else if (p.e.gelu == kGeluTanh) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) f[j] = int8_gelu(f[j], kGeluTanh);
+        }
+        if (!HIDDEN && !p.fast) {
+          // The residual or C is not laid out in 16-byte steps: the block goes
+          // through shared memory (as fp32 in both buffers, unit j ^ row of a row)
+          // and is finished row by row, a lane per column.
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            asm volatile("st.shared.b32 [%0], %1;" ::"r"(bufs + static_cast<uint32_t>((lane * 32 + (j ^ lane)) * 4)),
+                         "f"(f[j])
+                         : "memory");
+          __syncwarp();
+          const int n = col0 + lane;
+          const int rows = static_cast<int>(min(static_cast<int64_t>(32), p.e.M - row0));
+#pragma unroll 8
+          for (int k = 0; k < 32; ++k) {
+            if (k >= rows || n >= p.e.N) continue;
+            float x;
+            asm volatile("ld.shared.b32 %0, [%1];"
+                         : "=f"(x)
+                         : "r"(bufs + static_cast<uint32_t>((k * 32 + (lane ^ k)) * 4))
+                         : "memory");
+            if (p.e.residual) x = __fadd_rn(x, __bfloat162float(p.e.residual[(row0 + k) * p.e.ldr + n]));
+            if (p.e.out == kInt8OutF32)
+              static_cast<float*>(p.e.C)[(row0 + k) * p.e.ldc + n] = x;
+            else
+              static_cast<bf16*>(p.e.C)[(row0 + k) * p.e.ldc + n] = __float2bfloat16_rn(x);
+          }
+          __syncwarp();
           continue;
         }
-        // Stage the warp's block and store it with TMA (rows and columns past
-        // the matrix are clipped): 32 x 32 16-bit values, or two blocks of
-        // 32 x 16 fp32 values.
-        if (p.e.out == kInt8OutF32) {
-          if (lane == 0) bulk_wait_read<0>();
-          __syncwarp();
+        if (!HIDDEN && p.e.residual && row_in) {
+          if (whole) {
 #pragma unroll
-          for (int u = 0; u < 8; ++u)
-            stage16(bufs + (u >> 2) * kStageOut, lane, u & 3, __float_as_uint(f[4 * u]), __float_as_uint(f[4 * u + 1]),
-                    __float_as_uint(f[4 * u + 2]), __float_as_uint(f[4 * u + 3]));
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            tma_store_2d(&tmC, bufs, col0, static_cast<int32_t>(row0));
-            if (col0 + 16 < p.e.N) tma_store_2d(&tmC, bufs + kStageOut, col0 + 16, static_cast<int32_t>(row0));
-            bulk_commit();
-          }
-        } else {
-          const uint32_t buf = bufs + static_cast<uint32_t>(c & 1) * kStageOut;
-          if (lane == 0) bulk_wait_read<1>();  // the store that used this buffer has read it
-          __syncwarp();
-          if (p.e.out == kInt8OutHidden) {
-            uint32_t amax = 0;
+            for (int u = 0; u < 4; ++u) {
+              const uint32_t r8[4] = {res[u].x, res[u].y, res[u].z, res[u].w};
 #pragma unroll
-            for (int j = 0; j < 32; ++j) amax = max(amax, mag(f[j]));
-            const UpScale us = up_scale(amax, 32767.0f);
-#pragma unroll
-            for (int k = 0; k < kChunks; ++k)
-              if (k == c - c0) hmax[k] = hidden_max(amax);
-            uint32_t w[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-              w[j] = __byte_perm(hidden_bits(f[2 * j], us), hidden_bits(f[2 * j + 1], us), 0x5410);
-#pragma unroll
-            for (int u = 0; u < 4; ++u) stage16(buf, lane, u, w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
+              for (int j = 0; j < 8; ++j)
+                f[u * 8 + j] = __fadd_rn(f[u * 8 + j], (j & 1) ? bf16_hi(r8[j >> 1]) : bf16_lo(r8[j >> 1]));
+            }
           } else {
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-              stage16(buf, lane, u, pack_bf16(f[8 * u], f[8 * u + 1]), pack_bf16(f[8 * u + 2], f[8 * u + 3]),
-                      pack_bf16(f[8 * u + 4], f[8 * u + 5]), pack_bf16(f[8 * u + 6], f[8 * u + 7]));
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            tma_store_2d(&tmC, buf, col0, static_cast<int32_t>(row0));
-            bulk_commit();
+            for (int j = 0; j < 32; ++j)
+              if (col0 + j < p.e.N)
+                f[j] = __fadd_rn(f[j], __bfloat162float(p.e.residual[row * p.e.ldr + col0 + j]));
           }
         }
+        // The stores that used this buffer (fp32: both buffers) have read it.
+        if (lane == 0) {
+          if (p.e.out == kInt8OutF32)
+            bulk_wait_read<0>();
+          else
+            bulk_wait_read<1>();
+        }
+        __syncwarp();
+        if (HIDDEN) {
+          uint32_t amax = 0;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) amax = max(amax, mag(f[j]));
+          const UpScale us = up_scale(amax, 32767.0f);
+#pragma unroll
+          for (int k = 0; k < kChunks; ++k)
+            if (k == c - c0) hmax[k] = hidden_max(amax);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            uint32_t w2[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              w2[j] = __byte_perm(hidden_bits(f[u * 8 + 2 * j], us), hidden_bits(f[u * 8 + 2 * j + 1], us), 0x5410);
+            stage16(buf, lane, u, w2[0], w2[1], w2[2], w2[3]);
+          }
+        } else if (p.e.out == kInt8OutF32) {
+          // Two blocks of 32 x 16 fp32 values.
+#pragma unroll
+          for (int u = 0; u < 8; ++u)
+            stage16(buf + static_cast<uint32_t>(u >> 2) * kStageOut, lane, u & 3, __float_as_uint(f[4 * u]),
+                    __float_as_uint(f[4 * u + 1]), __float_as_uint(f[4 * u + 2]), __float_as_uint(f[4 * u + 3]));
+        } else {
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            stage16(buf, lane, u, pack_bf16(f[u * 8], f[u * 8 + 1]), pack_bf16(f[u * 8 + 2], f[u * 8 + 3]),
+                    pack_bf16(f[u * 8 + 4], f[u * 8 + 5]), pack_bf16(f[u * 8 + 6], f[u * 8 + 7]));
+        }
+        // Rows and columns past the matrix are clipped.
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_2d(&tmC, buf, col0, static_cast<int32_t>(row0));
+          if (p.e.out == kInt8OutF32 && col0 + 16 < p.e.N)
+            tma_store_2d(&tmC, buf + kStageOut, col0 + 16, static_cast<int32_t>(row0));
+          bulk_commit();
+        }
       }
-      if (!ok) break;
       // The maxima of this warp's 128 columns.
-      if (p.e.out == kInt8OutHidden && !part && row < p.e.M && tn * kBN + c0 * 32 < p.e.N)
+      if (HIDDEN && !part && row_in && tn * kBN + c0 * 32 < p.e.N)
         *reinterpret_cast<float4*>(p.e.hidden_max + row * p.e.ldm + tn * (kBN / kHiddenBlock) + c0) =
             make_float4(hmax[0], hmax[1], hmax[2], hmax[3]);
       tc_fence_before();
@@ -532,7 +563,7 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
           mbar_arrive_cluster(mapa_shared(te, 0));
       }
     }
-    if (lane == 0 && p.tma_store) bulk_wait_all();  // staged stores have left shared memory
+    if (lane == 0 && p.fast) bulk_wait_all();  // staged stores have left shared memory
   }
   tc_fence_before();
   __syncthreads();
@@ -566,7 +597,9 @@ cudaError_t pair_ready(int* pairs) {
   *pairs = resident[dev].load(std::memory_order_acquire);
   if (*pairs > 0) return cudaSuccess;
   std::lock_guard<std::mutex> lock(mu);
-  e = cudaFuncSetAttribute(k_int8_pair, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kPairSmem));
+  e = cudaFuncSetAttribute(k_int8_pair<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kPairSmem));
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(k_int8_pair<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kPairSmem));
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t q{};
   q.gridDim = dim3(static_cast<unsigned>(sm_count()), 1, 1);
@@ -578,18 +611,12 @@ cudaError_t pair_ready(int* pairs) {
   q.attrs = a;
   q.numAttrs = 1;
   int n = 0;
-  e = cudaOccupancyMaxActiveClusters(&n, k_int8_pair, &q);
+  e = cudaOccupancyMaxActiveClusters(&n, k_int8_pair<false>, &q);
   if (e == cudaSuccess && n <= 0) e = cudaErrorLaunchOutOfResources;
   if (e != cudaSuccess) return e;
   resident[dev].store(n, std::memory_order_release);
   *pairs = n;
   return cudaSuccess;
-}
-
-bool map8(CUtensorMap* m, const int8_t* base, int64_t rows, int64_t cols, int64_t ld, uint32_t box_rows,
-          std::string* err) {
-  return make_map_box(m, base, rows, cols, rows > 1 ? ld : (cols + 15) / 16 * 16, kBK, box_rows,
-                      CU_TENSOR_MAP_SWIZZLE_128B, err, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1);
 }
 
 int launch_pair(const Int8Gemm& g, cudaStream_t s, std::string* err) {
@@ -604,14 +631,12 @@ int launch_pair(const Int8Gemm& g, cudaStream_t s, std::string* err) {
   p.status = device_status_ptr(err);
   if (!p.status) return -3;
   p.timeout_ns = wait_limit_ns();
-  p.vec_ok = al(g.b_scale, 16) && (!g.bias || al(g.bias, 16)) &&
-             (!g.residual || (al(g.residual, 16) && g.ldr % 8 == 0));
   const int esz = g.out == kInt8OutF32 ? 4 : 2;
-  p.tma_store = al(g.C, 16) && g.ldc * esz % 16 == 0;
+  p.fast = al(g.C, 16) && g.ldc * esz % 16 == 0 && (!g.residual || p.e.vec_res);
   p.b_prefetch = g.b_stable;
   CUtensorMap ta{}, tb{}, tc{};
-  if (!map8(&ta, g.A, g.M, g.K, g.lda, kBM, err) || !map8(&tb, g.B, g.N, g.K, g.ldb, kBM, err)) return -3;
-  if (p.tma_store && !make_map_box(&tc, g.C, g.M, g.N, g.ldc, static_cast<uint32_t>(64 / esz), 32,
+  if (!int8_map(&ta, g.A, g.M, g.K, g.lda, kBM, err) || !int8_map(&tb, g.B, g.N, g.K, g.ldb, kBM, err)) return -3;
+  if (p.fast && !make_map_box(&tc, g.C, g.M, g.N, g.ldc, static_cast<uint32_t>(64 / esz), 32,
                                    CU_TENSOR_MAP_SWIZZLE_64B, err,
                                    g.out == kInt8OutF32      ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                    : g.out == kInt8OutHidden ? CU_TENSOR_MAP_DATA_TYPE_UINT16
@@ -637,7 +662,7 @@ int launch_pair(const Int8Gemm& g, cudaStream_t s, std::string* err) {
   a[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = a;
   cfg.numAttrs = 2;
-  e = cudaLaunchKernelEx(&cfg, k_int8_pair, ta, tb, tc, p);
+  e = cudaLaunchKernelEx(&cfg, g.out == kInt8OutHidden ? k_int8_pair<true> : k_int8_pair<false>, ta, tb, tc, p);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) {
     *err = std::string("int8 pair gemm launch: ") + cudaGetErrorString(e);
@@ -649,8 +674,15 @@ int launch_pair(const Int8Gemm& g, cudaStream_t s, std::string* err) {
 
 }  // namespace
 
+bool int8_map(CUtensorMap* m, const int8_t* base, int64_t rows, int64_t cols, int64_t ld, uint32_t box_rows,
+              std::string* err) {
+  return make_map_box(m, base, rows, cols, rows > 1 ? ld : (cols + 15) / 16 * 16, kBK, box_rows,
+                      CU_TENSOR_MAP_SWIZZLE_128B, err, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1);
+}
+
 Int8GemmWs int8_gemm_ws(int64_t m, int64_t n, int64_t k) {
   Int8GemmWs w;
+  if (k > 0 && m <= kInt8StreamRows) return int8_stream_ws(m, n);
   if (k <= 0 || pair_tiles(m, n) > (1 << 30)) return w;
   const sched::PairSched ps = pair_plan(m, n, k);
   if (ps.rem > 0) {
@@ -669,7 +701,7 @@ int run_int8_gemm(const Int8Gemm& g, cudaStream_t stream, std::string* err) {
   // that are multiples of 16 bytes (one row has no stride).
   if (g.K > 0 && al(g.A, 16) && al(g.B, 16) && (g.lda % 16 == 0 || g.M == 1) && (g.ldb % 16 == 0 || g.N == 1) &&
       pair_tiles(g.M, g.N) <= (1 << 30))
-    return launch_pair(g, stream, err);
+    return g.M <= kInt8StreamRows ? run_int8_stream(g, stream, err) : launch_pair(g, stream, err);
   const int64_t by = (g.N + kAnyTile - 1) / kAnyTile;
   const dim3 grid(static_cast<unsigned>((g.M + kAnyTile - 1) / kAnyTile), static_cast<unsigned>(by < 65535 ? by : 65535));
   k_int8_gemm_any<<<grid, 256, 0, stream>>>(g.A, g.lda, g.B, g.ldb, int8_epi(g));

@@ -20,6 +20,8 @@ struct Int8Epi {
   int out;
   float* hidden_max;
   int64_t ldm;
+  // 16-byte accesses: scales and bias; the residual's rows; C's rows.
+  bool vec_cols, vec_res, vec_out;
 };
 
 inline Int8Epi int8_epi(const Int8Gemm& g) {
@@ -38,6 +40,10 @@ inline Int8Epi int8_epi(const Int8Gemm& g) {
   e.out = g.out;
   e.hidden_max = g.hidden_max;
   e.ldm = g.ldm;
+  auto al16 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
+  e.vec_cols = al16(g.b_scale) && (!g.bias || al16(g.bias));
+  e.vec_res = al16(g.residual) && (g.ldr % 8 == 0 || g.M == 1);
+  e.vec_out = al16(g.C) && (g.ldc * (g.out == kInt8OutF32 ? 4 : 2) % 16 == 0 || g.M == 1);
   return e;
 }
 
@@ -87,29 +93,126 @@ __device__ __forceinline__ uint32_t hidden_bits(float h, UpScale s) {
   return s.r == 0.0f ? 0u : round_bits(h * s.up * s.r);
 }
 
-// acc * sa * sb, and + bias: the same roundings in every kernel and layout.
-__device__ __forceinline__ float int8_scaled(int32_t acc, float sa, float sb) {
-  return __fmul_rn(__fmul_rn(__int2float_rn(acc), sa), sb);
-}
+// acc * sa * sb + bias: the same roundings in every kernel and layout (without a
+// bias it is 0).
 __device__ __forceinline__ float int8_scaled(int32_t acc, float sa, float sb, float bias) {
   return __fmaf_rn(__fmul_rn(__int2float_rn(acc), sa), sb, bias);
 }
 
-// One output value from its integer sum, without the residual.
-__device__ __forceinline__ float int8_value(const Int8Epi& e, int32_t acc, float sa, int n) {
-  const float v =
-      e.bias ? int8_scaled(acc, sa, e.b_scale[n], __bfloat162float(e.bias[n])) : int8_scaled(acc, sa, e.b_scale[n]);
-  return int8_gelu(v, e.gelu);
+// Eight neighbouring columns n .. n + 7 of the epilogue's operands. `vec` says
+// that scales and bias start on 16-byte boundaries (n is a multiple of 8).
+struct Cols8 {
+  float sb[8], bias[8];
+};
+__device__ __forceinline__ Cols8 int8_cols(const Int8Epi& e, int n, bool vec) {
+  Cols8 c;
+  if (vec && n + 8 <= e.N) {
+    const float4 s0 = *reinterpret_cast<const float4*>(e.b_scale + n);
+    const float4 s1 = *reinterpret_cast<const float4*>(e.b_scale + n + 4);
+    const uint4 b = e.bias ? *reinterpret_cast<const uint4*>(e.bias + n) : make_uint4(0u, 0u, 0u, 0u);
+    const float s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+    const uint32_t w[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      c.sb[j] = s[j];
+      c.bias[j] = (j & 1) ? bf16_hi(w[j >> 1]) : bf16_lo(w[j >> 1]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      c.sb[j] = n + j < e.N ? e.b_scale[n + j] : 0.0f;
+      c.bias[j] = e.bias && n + j < e.N ? __bfloat162float(e.bias[n + j]) : 0.0f;
+    }
+  }
+  return c;
 }
 
-// One output value but for a hidden one, finished and stored.
-__device__ __forceinline__ void int8_store(const Int8Epi& e, int32_t acc, float sa, int64_t m, int n) {
-  float v = int8_value(e, acc, sa, n);
-  if (e.residual) v = __fadd_rn(v, __bfloat162float(e.residual[m * e.ldr + n]));
-  if (e.out == kInt8OutF32)
-    static_cast<float*>(e.C)[m * e.ldc + n] = v;
-  else
-    static_cast<bf16*>(e.C)[m * e.ldc + n] = __float2bfloat16_rn(v);
+// Scale, bias, GELU on eight columns of one row. The epilogues walk over groups
+// of eight in rolled loops: with 32 columns unrolled their code did not fit the
+// instruction caches, and fetching it took most of a small product's time (64 x
+// 4096 x 4096: 40 us, of which the weights' stream is 3).
+__device__ __forceinline__ void int8_values(const Int8Epi& e, const uint32_t (&acc)[8], float sa, const Cols8& c,
+                                            float (&f)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = int8_scaled(static_cast<int32_t>(acc[j]), sa, c.sb[j], c.bias[j]);
+  if (e.gelu == kGeluErf) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = int8_gelu(f[j], kGeluErf);
+  } else if (e.gelu == kGeluTanh) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = int8_gelu(f[j], kGeluTanh);
+  }
+}
+
+__device__ __forceinline__ void add8_bf16(const uint4& b, float (&f)[8]) {
+  const uint32_t w[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = __fadd_rn(f[j], (j & 1) ? bf16_hi(w[j >> 1]) : bf16_lo(w[j >> 1]));
+}
+
+// + residual on columns n .. n + 7 of row m; `vec`: its rows start on 16-byte
+// boundaries.
+__device__ __forceinline__ void int8_residual(const Int8Epi& e, int64_t m, int n, bool vec, float (&f)[8]) {
+  const bf16* r = e.residual + m * e.ldr + n;
+  if (vec && n + 8 <= e.N) {
+    add8_bf16(*reinterpret_cast<const uint4*>(r), f);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (n + j < e.N) f[j] = __fadd_rn(f[j], __bfloat162float(r[j]));
+  }
+}
+
+// Eight hidden values of row m, columns n .. n + 7 (zeros past the matrix), whose
+// block of 32 lies in four neighbouring lanes; `in`: row and first column are in
+// the matrix. The warp calls it together.
+__device__ __forceinline__ void int8_store_hidden(const Int8Epi& e, int64_t m, int n, bool in, float (&f)[8]) {
+  uint32_t amax = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if (n + j >= e.N) f[j] = 0.0f;
+    amax = max(amax, mag(f[j]));
+  }
+  amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+  amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+  if (!in) return;
+  const UpScale us = up_scale(amax, 32767.0f);
+  uint32_t w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) w[j] = __byte_perm(hidden_bits(f[2 * j], us), hidden_bits(f[2 * j + 1], us), 0x5410);
+  // The block's row stride is a multiple of 16 values, so eight at a multiple of
+  // eight stay in the row.
+  *reinterpret_cast<uint4*>(static_cast<int16_t*>(e.C) + m * e.ldc + n) = make_uint4(w[0], w[1], w[2], w[3]);
+  if ((n & (kHiddenBlock - 1)) == 0) e.hidden_max[m * e.ldm + n / kHiddenBlock] = hidden_max(amax);
+}
+
+__device__ __forceinline__ uint4 pack8_bf16(const float (&f)[8]) {
+  return make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
+}
+
+// Columns n .. n + 7 of row m of C (bf16 or fp32); `vec`: its rows start on
+// 16-byte boundaries.
+__device__ __forceinline__ void int8_store(const Int8Epi& e, int64_t m, int n, bool vec, const float (&f)[8]) {
+  if (e.out == kInt8OutF32) {
+    float* c = static_cast<float*>(e.C) + m * e.ldc + n;
+    if (vec && n + 8 <= e.N) {
+      *reinterpret_cast<float4*>(c) = make_float4(f[0], f[1], f[2], f[3]);
+      *reinterpret_cast<float4*>(c + 4) = make_float4(f[4], f[5], f[6], f[7]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (n + j < e.N) c[j] = f[j];
+    }
+  } else {
+    bf16* c = static_cast<bf16*>(e.C) + m * e.ldc + n;
+    if (vec && n + 8 <= e.N) {
+      *reinterpret_cast<uint4*>(c) = pack8_bf16(f);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (n + j < e.N) c[j] = __float2bfloat16_rn(f[j]);
+    }
+  }
 }
 
 }  // namespace tfb200
