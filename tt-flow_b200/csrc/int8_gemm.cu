@@ -376,15 +376,13 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
       }
       tc_fence_after();
       const uint32_t tacc = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * kBN);
-      int* const flags = p.flags + ((w.slot * 2 + static_cast<int>(rank)) * kEpiWarps + ew) * kChunks;
+      // A split tile's flags: one per part and epilogue warp.
+      int* const flag = p.flags + (w.slot * 2 + static_cast<int>(rank)) * kEpiWarps + ew;
       if (fix && row0 < p.e.M) {
-        // The parts of a split tile: lane (part, chunk) waits until all 32 rows of
-        // its chunk are in (acquire); the warp's barrier passes that on.
-        const int part_of = lane / kChunks, chunk = lane % kChunks;
-        if (part_of < ps.parts && tn * kBN + (c0 + chunk) * 32 < p.e.N) {
-          const int* f = flags + part_of * 2 * kEpiWarps * kChunks + chunk;
+        // Lane j waits for part j (acquire); the warp's barrier passes that on.
+        if (lane < ps.parts) {
           const uint64_t t0 = global_ns();
-          while (ok && ld_acquire_gpu(f) != 32)
+          while (ok && ld_acquire_gpu(flag + lane * 2 * kEpiWarps) == 0)
             if (ctl->abort || global_ns() - t0 > p.timeout_ns) ok = false;
         }
         ok = __all_sync(0xffffffffu, ok);
@@ -412,13 +410,11 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
         tmem_ld_32cols(tacc + static_cast<uint32_t>(c * 32), v);
         tmem_wait_ld();
         if (part) {
-          // A helper's rows of the chunk go to its slot; each lane then counts its
-          // row in on the chunk's flag (release).
+          // A helper's rows of the chunk go to its slot.
 #pragma unroll
           for (int k = 0; k < 8; ++k)
             __stcg(slot + k * kBM, make_int4(static_cast<int>(v[4 * k]), static_cast<int>(v[4 * k + 1]),
                                              static_cast<int>(v[4 * k + 2]), static_cast<int>(v[4 * k + 3])));
-          red_add_release_gpu(flags + (c - c0), 1);
           continue;
         }
         if (fix) {
@@ -469,20 +465,28 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
                          : "memory");
           __syncwarp();
           const int n = col0 + lane;
-          const int rows = static_cast<int>(min(static_cast<int64_t>(32), p.e.M - row0));
-#pragma unroll 8
-          for (int k = 0; k < 32; ++k) {
-            if (k >= rows || n >= p.e.N) continue;
-            float x;
-            asm volatile("ld.shared.b32 %0, [%1];"
-                         : "=f"(x)
-                         : "r"(bufs + static_cast<uint32_t>((k * 32 + (lane ^ k)) * 4))
-                         : "memory");
-            if (p.e.residual) x = __fadd_rn(x, __bfloat162float(p.e.residual[(row0 + k) * p.e.ldr + n]));
-            if (p.e.out == kInt8OutF32)
-              static_cast<float*>(p.e.C)[(row0 + k) * p.e.ldc + n] = x;
-            else
-              static_cast<bf16*>(p.e.C)[(row0 + k) * p.e.ldc + n] = __float2bfloat16_rn(x);
+          const int rows = n < p.e.N ? static_cast<int>(min(static_cast<int64_t>(32), p.e.M - row0)) : 0;
+#pragma unroll 1
+          for (int k0 = 0; k0 < rows; k0 += 8) {
+            float x[8], y[8] = {};
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              asm volatile("ld.shared.b32 %0, [%1];"
+                           : "=f"(x[k])
+                           : "r"(bufs + static_cast<uint32_t>(((k0 + k) * 32 + (lane ^ (k0 + k))) * 4))
+                           : "memory");
+              if (p.e.residual && k0 + k < rows) y[k] = __bfloat162float(p.e.residual[(row0 + k0 + k) * p.e.ldr + n]);
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              if (k0 + k >= rows) break;
+              const int64_t at = (row0 + k0 + k) * p.e.ldc + n;
+              const float z = __fadd_rn(x[k], y[k]);
+              if (p.e.out == kInt8OutF32)
+                static_cast<float*>(p.e.C)[at] = z;
+              else
+                static_cast<bf16*>(p.e.C)[at] = __float2bfloat16_rn(z);
+            }
           }
           __syncwarp();
           continue;
@@ -549,6 +553,11 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
           bulk_commit();
         }
       }
+      if (part) {
+        // One release for the warp's rows (one per chunk cost 1.3 us each).
+        __syncwarp();
+        if (lane == 0) st_release_gpu(flag, 1);
+      }
       // The maxima of this warp's 128 columns.
       if (HIDDEN && !part && row_in && tn * kBN + c0 * 32 < p.e.N)
         *reinterpret_cast<float4*>(p.e.hidden_max + row * p.e.ldm + tn * (kBN / kHiddenBlock) + c0) =
@@ -578,11 +587,33 @@ bool al(const void* p, unsigned b) { return (reinterpret_cast<uintptr_t>(p) & (b
 
 int64_t pair_tiles(int64_t m, int64_t n) { return (m + 2 * kBM - 1) / (2 * kBM) * ((n + kBN - 1) / kBN); }
 
-// The schedule over all the pairs of a B200; a short last wave is split when
-// that shortens the busiest pair by 2 % or more.
+// The schedule over all the pairs of a B200. A last wave of R < 74 tiles is split
+// when that shortens it: each of its tiles keeps k-blocks [0, kc) on one pair, and
+// S parts of the rest go to idle pairs, one each. Times in k-blocks (0.3 us): a
+// part costs kPartCost for writing its sums and the hand-over, and the finishing
+// pair kReadCost per part.
+constexpr int kPartCost = 8, kReadCost = 3;
 sched::PairSched pair_plan(int64_t m, int64_t n, int64_t k) {
-  return sched::plan(static_cast<int>(pair_tiles(m, n)), static_cast<int>((k + kBK - 1) / kBK), kSmPairs,
-                     sched::kMaxSlots);
+  sched::PairSched s;
+  s.tiles = static_cast<int>(pair_tiles(m, n));
+  s.kblocks = static_cast<int>((k + kBK - 1) / kBK);
+  s.pairs = kSmPairs;
+  const int rem = s.tiles % kSmPairs, idle = kSmPairs - rem;
+  int best = s.kblocks;
+  for (int parts = 1; rem > 0 && parts <= sched::kMaxParts && rem * parts <= idle; ++parts) {
+    // Equal pieces: kc = ceil(KB / (parts + 1)), the parts share the rest.
+    const int kc = (s.kblocks + parts) / (parts + 1);
+    if (s.kblocks - kc < parts) break;
+    const int cost = kc + kPartCost + kReadCost * parts;
+    if (cost < best) {
+      best = cost;
+      s.waves = s.tiles / kSmPairs;
+      s.rem = rem;
+      s.parts = parts;
+      s.kc = kc;
+    }
+  }
+  return s;
 }
 
 // Per-device set-up of the first call; calls may come from several host
@@ -686,7 +717,7 @@ Int8GemmWs int8_gemm_ws(int64_t m, int64_t n, int64_t k) {
   if (k <= 0 || pair_tiles(m, n) > (1 << 30)) return w;
   const sched::PairSched ps = pair_plan(m, n, k);
   if (ps.rem > 0) {
-    w.clear_bytes = (static_cast<size_t>(ps.rem) * ps.parts * sched::kFlagsPerSlot * sizeof(int) + 255) / 256 * 256;
+    w.clear_bytes = (static_cast<size_t>(ps.rem) * ps.parts * 2 * kEpiWarps * sizeof(int) + 255) / 256 * 256;
     w.total = w.clear_bytes + static_cast<size_t>(ps.rem) * ps.parts * sched::kSlotBytes;
   }
   return w;

@@ -12,10 +12,13 @@
 // infinity or a NaN (or whose sum of squares leaves fp32) gives q = 0 and scale
 // NaN, so everything computed from it is NaN.
 //
-// HBM-bound: 2K bytes read and K written per row (4K and 3K with a residual).
-// A row's T threads hold it in registers, kPer values each, so that it is read
-// once and all its loads are in flight together; T is the smallest block that
-// holds the row. Rows up to 1024 values take one warp and four rows a block.
+// HBM-bound: 2K bytes read and K written per row (4K and 3K with a residual). A
+// row's T threads hold it in registers, so that it is read once and all its
+// loads are in flight together. The arithmetic has to be kept short beside that:
+// values are held as packed fp32 pairs (one f32x2 instruction for two), plain
+// quantisation takes its maximum on the 16-bit words, and the hidden block's
+// comes with it (the first form, which widened every value twice, took 105 us
+// for an 8192 x 16384 hidden block and 86 us for as many bf16 values).
 #include <algorithm>
 
 #include "int8_math.cuh"
@@ -24,8 +27,8 @@ namespace tfb200 {
 
 namespace {
 
-constexpr int kPer = 32;       // values per thread
-constexpr int kMaxRow = 1024 * kPer;
+constexpr int kMaxT = 512;          // threads per row
+constexpr int kMaxRow = 64 * kMaxT;  // values of a row held in registers
 
 struct RowsParams {
   int M, K;
@@ -60,9 +63,27 @@ __global__ void __launch_bounds__(256) k_int8_clear(uint4* zero, int64_t n) {
 }
 
 template <int KIND>
-__device__ __forceinline__ float in_value(uint16_t bits) {
+__device__ __forceinline__ float in_value(uint32_t bits) {
   if (KIND == kInt8RowsHidden) return static_cast<float>(static_cast<int16_t>(bits));
-  return __uint_as_float(static_cast<uint32_t>(bits) << 16);
+  return __uint_as_float(bits << 16);
+}
+// The two values of a 32-bit word.
+template <int KIND>
+__device__ __forceinline__ uint64_t in_pair(uint32_t w) {
+  if (KIND == kInt8RowsHidden) return f2(in_value<KIND>(w & 0xFFFFu), in_value<KIND>(w >> 16));
+  return f2_from_bf16x2(w);
+}
+
+// max(a, |b|), NaN if one is.
+__device__ __forceinline__ float max_abs(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
+  return r;
+}
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
 }
 
 struct RowStat {
@@ -112,20 +133,23 @@ __device__ __forceinline__ RowScale row_scale(const RowsParams& p, RowStat s) {
   return o;
 }
 
-__device__ __forceinline__ uint32_t q_bits(float t, const RowScale& s) {
-  return round_bits(__fmul_rn(__fmul_rn(t, s.u.up), s.u.r));
+// rn of two values in the low bytes of a pair's halves.
+__device__ __forceinline__ uint64_t q_pair(uint64_t v, uint64_t r) {
+  return f2_add(f2_mul(v, r), f2(12582912.0f, 12582912.0f));
 }
-__device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+__device__ __forceinline__ uint32_t pack4(uint64_t a, uint64_t b) {
+  const uint32_t lo = __byte_perm(static_cast<uint32_t>(a), static_cast<uint32_t>(a >> 32), 0x0040);
+  const uint32_t hi = __byte_perm(static_cast<uint32_t>(b), static_cast<uint32_t>(b >> 32), 0x0040);
+  return __byte_perm(lo, hi, 0x5410);
 }
 
 // VEC: rows start on 16-byte boundaries (8 for q); a thread takes 8 neighbouring
 // values at a time. Otherwise a thread takes single values, T apart.
 // WARP: a warp per row (T = 32), else a block per row (T = blockDim.x).
-// The row stays in registers as its 16-bit values, two a word, and is widened
-// again for the second pass: held as fp32 it spilled at 1024 threads.
-template <int KIND, bool RES, bool VEC, bool WARP>
-__global__ void __launch_bounds__(WARP ? 128 : 1024) k_int8_rows(const RowsParams p) {
+// PER: values per thread.
+template <int KIND, bool RES, bool VEC, bool WARP, int PER>
+__global__ void __launch_bounds__(WARP ? 128 : kMaxT, !WARP && PER == 32 && KIND == kInt8RowsHidden ? 3 : 1)
+    k_int8_rows(const RowsParams p) {
   // Launched with programmatic serialization: wait for the grid before (it may
   // write x or still read q), then let the next grid start its prologue.
   grid_dep_wait();
@@ -139,8 +163,8 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) k_int8_rows(const RowsParam
   const uint16_t* r = RES ? reinterpret_cast<const uint16_t*>(p.residual) + row * p.ldr : nullptr;
   const uint16_t* g = reinterpret_cast<const uint16_t*>(p.gamma);
   const int K = p.K;
-  // First of the 8 values of group i, and the distance between them.
-  constexpr int G = kPer / 8;
+  // Groups of 8 values: the first of group i, and the distance between them.
+  constexpr int G = PER / 8;
   const int step = VEC ? 1 : T;
   auto first = [&](int i) { return VEC ? (t + i * T) * 8 : t + i * 8 * T; };
 
@@ -158,93 +182,105 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) k_int8_rows(const RowsParam
       }
     }
   };
-  uint32_t xw[G][4], rw[RES ? G : 1][4];
+  uint32_t xw[G][4], rw[RES ? G : 1][4], gw[KIND == kInt8RowsNorm && VEC ? G : 1][4];
+  float hm[KIND == kInt8RowsHidden ? G : 1];
 #pragma unroll
   for (int i = 0; i < G; ++i) {
     load8(x, first(i), xw[i]);
     if (RES) load8(r, first(i), rw[i]);
+    if (KIND == kInt8RowsNorm && VEC) load8(g, first(i), gw[VEC ? i : 0]);
+    // Eight hidden values lie in one block of 32.
+    if (KIND == kInt8RowsHidden) hm[i] = first(i) < K ? p.hidden_max[row * p.ldm + first(i) / kHiddenBlock] : 0.0f;
   }
-  float hm[KIND == kInt8RowsHidden ? G : 1];
+  RowStat st{0.0f, 0u};
+  uint64_t v[KIND == kInt8RowsNorm ? G : 1][4];  // kInt8RowsNorm: t
   if (KIND == kInt8RowsHidden) {
 #pragma unroll
+    for (int i = 0; i < G; ++i) st.amax = max(st.amax, mag(hm[i]));
+  } else if (KIND == kInt8RowsQuant) {
+    uint32_t m = 0;
+#pragma unroll
     for (int i = 0; i < G; ++i)
-      hm[i] = first(i) < K ? p.hidden_max[row * p.ldm + first(i) / kHiddenBlock] : 0.0f;
-  }
-  auto half16 = [](const uint32_t (&w)[4], int j) { return static_cast<uint16_t>(w[j >> 1] >> (16 * (j & 1))); };
-  // The 8 values t of group i; with STAT also their statistics and the sum.
-  RowStat st{0.0f, 0u};
-  auto group = [&](int i, bool stat, float (&v)[8]) {
-    const int k = first(i);
-    // Eight hidden values lie in one block of 32.
-    const float block = KIND == kInt8RowsHidden ? hm[i] * (1.0f / 32767.0f) : 1.0f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      v[j] = in_value<KIND>(half16(xw[i], j));
-      if (KIND == kInt8RowsHidden) v[j] *= block;
-      if (RES) v[j] = __fadd_rn(v[j], in_value<kInt8RowsQuant>(half16(rw[RES ? i : 0], j)));
-    }
-    if (KIND == kInt8RowsNorm) {
-      if (stat) {
+      for (int j = 0; j < 4; ++j) m = max_u16x2(m, xw[i][j] & 0x7FFF7FFFu);
+    st.amax = max(m << 16, m & 0xFFFF0000u);
+  } else {
+    uint64_t ss = 0;
+    float amax = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) st.ss = fmaf(v[j], v[j], st.ss);
+    for (int i = 0; i < G; ++i) {
+      const int k = first(i);
+      if (k < K) {
+        uint64_t s[4];
+        if (!VEC) load8(g, k, gw[0]);  // single loads: all of them at once would not fit the registers
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          s[j] = in_pair<KIND>(xw[i][j]);
+          if (RES) s[j] = f2_add(s[j], in_pair<KIND>(rw[RES ? i : 0][j]));
+          ss = f2_fma(s[j], s[j], ss);
+          v[i][j] = f2_mul(s[j], in_pair<KIND>(gw[VEC ? i : 0][j]));
+          float lo, hi;
+          f2_split(v[i][j], lo, hi);
+          amax = max_abs(max_abs(amax, lo), hi);
+        }
         if (RES) {
           bf16* sum = p.sum + row * p.lds;
+          uint32_t o[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float lo, hi;
+            f2_split(s[j], lo, hi);
+            o[j] = pack_bf16(lo, hi);
+          }
           if (VEC && k + 8 <= K) {
-            *reinterpret_cast<uint4*>(sum + k) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]),
-                                                            pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+            *reinterpret_cast<uint4*>(sum + k) = make_uint4(o[0], o[1], o[2], o[3]);
           } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-              if (k + j * step < K) sum[k + j * step] = __float2bfloat16_rn(v[j]);
+              if (k + j * step < K)
+                reinterpret_cast<uint16_t*>(sum)[k + j * step] = static_cast<uint16_t>(o[j >> 1] >> (16 * (j & 1)));
           }
         }
       }
-      if (VEC && k + 8 <= K) {
-        const uint4 gv = __ldg(reinterpret_cast<const uint4*>(g + k));
-        const uint32_t gw[4] = {gv.x, gv.y, gv.z, gv.w};
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = __fmul_rn(v[j], in_value<kInt8RowsQuant>(half16(gw, j)));
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (k + j * step < K) v[j] = __fmul_rn(v[j], in_value<kInt8RowsQuant>(__ldg(g + k + j * step)));
-      }
     }
-    if (stat) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) st.amax = max(st.amax, mag(v[j]));
-    }
-  };
-#pragma unroll
-  for (int i = 0; i < G; ++i) {
-    float v[8];
-    if (first(i) < K) group(i, true, v);
+    float lo, hi;
+    f2_split(ss, lo, hi);
+    st.ss = lo + hi;
+    st.amax = mag(amax);
   }
   st = WARP ? warp_stat(st, KIND == kInt8RowsNorm) : block_stat(st, KIND == kInt8RowsNorm);
   const RowScale sc = row_scale<KIND>(p, st);
   if (t == 0) p.scale[row] = sc.scale;
   int8_t* q = p.q + row * p.ldq;
-  const bool zero = sc.u.r == 0.0f;  // a row of zeros, or one that is not finite
+  // A row of zeros, or one that is not finite, is stored as zeros.
+  const uint32_t keep = sc.u.r == 0.0f ? 0u : 0xFFFFFFFFu;
+  const uint64_t rr = f2(sc.u.r, sc.u.r), up = f2(sc.u.up, sc.u.up);
 #pragma unroll
   for (int i = 0; i < G; ++i) {
     const int k = first(i);
     if (k >= K) break;
-    float v[8];
-    group(i, false, v);
-    uint32_t b[8];
+    uint64_t b[4];
+    // A hidden value and its factor: h = value * block, q = rn(value * block * r).
+    const float hr = KIND == kInt8RowsHidden ? hm[i] * sc.u.up * sc.u.r * (1.0f / 32767.0f) : 0.0f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) b[j] = zero ? 0u : q_bits(v[j], sc);
+    for (int j = 0; j < 4; ++j) {
+      uint64_t s = KIND == kInt8RowsNorm ? v[KIND == kInt8RowsNorm ? i : 0][j] : in_pair<KIND>(xw[i][j]);
+      if (KIND != kInt8RowsHidden && sc.u.up != 1.0f) s = f2_mul(s, up);
+      b[j] = q_pair(s, KIND == kInt8RowsHidden ? f2(hr, hr) : rr);
+    }
+    const uint2 o = make_uint2(pack4(b[0], b[1]) & keep, pack4(b[2], b[3]) & keep);
     if (VEC && k + 8 <= K) {
-      *reinterpret_cast<uint2*>(q + k) = make_uint2(pack4(b[0], b[1], b[2], b[3]), pack4(b[4], b[5], b[6], b[7]));
+      *reinterpret_cast<uint2*>(q + k) = o;
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (k + j * step < K) q[k + j * step] = static_cast<int8_t>(b[j] & 0xFFu);
+        if (k + j * step < K) q[k + j * step] = static_cast<int8_t>(((j < 4 ? o.x : o.y) >> (8 * (j & 3))) & 0xFFu);
     }
   }
 }
 
-// Rows longer than the registers of a block: the row is read twice, the second
+// Rows longer than the registers of a block (unaligned ones over 16384 values):
+// the row is read twice, the second
 // time mostly from L2.
 template <int KIND, bool RES>
 __global__ void __launch_bounds__(1024) k_int8_rows_long(const RowsParams p) {
@@ -257,40 +293,53 @@ __global__ void __launch_bounds__(1024) k_int8_rows_long(const RowsParams p) {
   const uint16_t* g = reinterpret_cast<const uint16_t*>(p.gamma);
   auto value = [&](int k) {
     float s = in_value<KIND>(x[k]);
-    if (KIND == kInt8RowsHidden) s *= p.hidden_max[row * p.ldm + k / kHiddenBlock] * (1.0f / 32767.0f);
-    if (RES) s = __fadd_rn(s, in_value<kInt8RowsQuant>(r[k]));
+    if (RES) s = __fadd_rn(s, in_value<KIND>(r[k]));
     return s;
   };
   RowStat st{0.0f, 0u};
+  if (KIND == kInt8RowsHidden) {
+    for (int k = threadIdx.x * kHiddenBlock; k < p.K; k += blockDim.x * kHiddenBlock)
+      st.amax = max(st.amax, mag(p.hidden_max[row * p.ldm + k / kHiddenBlock]));
+  } else {
 #pragma unroll 4
-  for (int k = threadIdx.x; k < p.K; k += blockDim.x) {
-    float s = value(k);
-    if (KIND == kInt8RowsNorm) {
-      st.ss = fmaf(s, s, st.ss);
-      s = __fmul_rn(s, in_value<kInt8RowsQuant>(g[k]));
+    for (int k = threadIdx.x; k < p.K; k += blockDim.x) {
+      float s = value(k);
+      if (KIND == kInt8RowsNorm) {
+        st.ss = fmaf(s, s, st.ss);
+        s = __fmul_rn(s, in_value<KIND>(g[k]));
+      }
+      st.amax = max(st.amax, mag(s));
     }
-    st.amax = max(st.amax, mag(s));
   }
   st = block_stat(st, KIND == kInt8RowsNorm);
   const RowScale sc = row_scale<KIND>(p, st);
   if (threadIdx.x == 0) p.scale[row] = sc.scale;
-  const bool zero = sc.u.r == 0.0f;
   // A thread reads a value of x again before it writes the sum, which may be x.
 #pragma unroll 4
   for (int k = threadIdx.x; k < p.K; k += blockDim.x) {
     float s = value(k);
     if (RES) p.sum[row * p.lds + k] = __float2bfloat16_rn(s);
-    if (KIND == kInt8RowsNorm) s = __fmul_rn(s, in_value<kInt8RowsQuant>(g[k]));
-    p.q[row * p.ldq + k] = zero ? 0 : static_cast<int8_t>(q_bits(s, sc) & 0xFFu);
+    if (KIND == kInt8RowsNorm) s = __fmul_rn(s, in_value<KIND>(g[k]));
+    uint32_t b;
+    if (KIND == kInt8RowsHidden)
+      b = round_bits(s * (p.hidden_max[row * p.ldm + k / kHiddenBlock] * sc.u.up * sc.u.r * (1.0f / 32767.0f)));
+    else
+      b = round_bits(__fmul_rn(__fmul_rn(s, sc.u.up), sc.u.r));
+    p.q[row * p.ldq + k] = sc.u.r == 0.0f ? 0 : static_cast<int8_t>(b & 0xFFu);
   }
 }
 
 template <int KIND, bool RES>
 cudaError_t launch_rows(const RowsParams& p, bool vec, cudaStream_t s) {
-  const bool warp = p.K <= 32 * kPer;
+  constexpr bool kV = KIND == kInt8RowsHidden;  // the hidden block is always aligned
+  vec = vec || kV;
+  const bool warp = p.K <= 32 * 32, wide = p.K > 32 * kMaxT, longer = p.K > kMaxRow || (wide && !vec);
+  // The smallest block that holds the row; with few rows, one that gives every
+  // thread as few values as it can.
   int T = 128;
-  while (!warp && T < 1024 && T * kPer < p.K) T *= 2;
-  if (p.K > kMaxRow) T = 1024;
+  const int per = p.M <= 148 ? 8 : 32;
+  while (!warp && T < kMaxT && T * per < p.K) T *= 2;
+  if (longer) T = 1024;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(warp ? (p.M + 3) / 4 : p.M), 1, 1);
   cfg.blockDim = dim3(static_cast<unsigned>(T), 1, 1);
@@ -300,12 +349,12 @@ cudaError_t launch_rows(const RowsParams& p, bool vec, cudaStream_t s) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  constexpr bool kAny = KIND != kInt8RowsHidden;  // the hidden block is always aligned
-  cudaError_t e = p.K > kMaxRow ? cudaLaunchKernelEx(&cfg, k_int8_rows_long<KIND, RES>, p)
-                  : warp ? (vec ? cudaLaunchKernelEx(&cfg, k_int8_rows<KIND, RES, true, true>, p)
-                                : cudaLaunchKernelEx(&cfg, k_int8_rows<KIND, RES, !kAny, true>, p))
-                         : (vec ? cudaLaunchKernelEx(&cfg, k_int8_rows<KIND, RES, true, false>, p)
-                                : cudaLaunchKernelEx(&cfg, k_int8_rows<KIND, RES, !kAny, false>, p));
+  void (*kernel)(const RowsParams) =
+      longer ? k_int8_rows_long<KIND, RES>
+      : wide ? k_int8_rows<KIND, RES, true, false, 64>
+      : warp ? (vec ? k_int8_rows<KIND, RES, true, true, 32> : k_int8_rows<KIND, RES, kV, true, 32>)
+             : (vec ? k_int8_rows<KIND, RES, true, false, 32> : k_int8_rows<KIND, RES, kV, false, 32>);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
   return e == cudaSuccess ? cudaGetLastError() : e;
 }
 
