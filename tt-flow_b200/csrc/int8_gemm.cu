@@ -431,29 +431,33 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
           }
         }
         const uint32_t buf = bufs + (p.e.out == kInt8OutF32 ? 0u : static_cast<uint32_t>(c & 1) * kStageOut);
-        float f[32];
+        uint64_t v2[16];  // fp32 pairs
         {
-          const float4* sb = reinterpret_cast<const float4*>(ctl->sb + c * 32);
+          const ulonglong2* sb = reinterpret_cast<const ulonglong2*>(ctl->sb + c * 32);
           const uint4* bias = reinterpret_cast<const uint4*>(ctl->bias + c * 32);
+          const uint64_t sa2 = f2(sa, sa);
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
-            const float4 s0 = sb[2 * u], s1 = sb[2 * u + 1];
+            const ulonglong2 s0 = sb[2 * u], s1 = sb[2 * u + 1];
             const uint4 b = bias[u];
-            const float s8[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
-            const uint32_t b8[4] = {b.x, b.y, b.z, b.w};
+            const uint64_t s4[4] = {s0.x, s0.y, s1.x, s1.y};
+            const uint32_t b4[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              f[u * 8 + j] = int8_scaled(static_cast<int32_t>(v[u * 8 + j]), sa, s8[j],
-                                         (j & 1) ? bf16_hi(b8[j >> 1]) : bf16_lo(b8[j >> 1]));
+            for (int j = 0; j < 4; ++j)
+              v2[u * 4 + j] =
+                  int8_scaled(v[u * 8 + 2 * j], v[u * 8 + 2 * j + 1], sa2, s4[j], f2_from_bf16x2(b4[j]));
           }
         }
         if (p.e.gelu == kGeluErf) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) f[j] = int8_gelu(f[j], kGeluErf);
+          for (int j = 0; j < 16; ++j) v2[j] = int8_gelu_erf(v2[j]);
         } else if (p.e.gelu == kGeluTanh) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) f[j] = int8_gelu(f[j], kGeluTanh);
+          for (int j = 0; j < 16; ++j) v2[j] = int8_gelu_tanh(v2[j]);
         }
+        float f[32];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) f2_split(v2[j], f[2 * j], f[2 * j + 1]);
         if (!HIDDEN && !p.fast) {
           // The residual or C is not laid out in 16-byte steps: the block goes
           // through shared memory (as fp32 in both buffers, unit j ^ row of a row)
@@ -516,21 +520,22 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
         }
         __syncwarp();
         if (HIDDEN) {
-          uint32_t amax = 0;
+          float amax = 0.0f;
 #pragma unroll
-          for (int j = 0; j < 32; ++j) amax = max(amax, mag(f[j]));
-          const UpScale us = up_scale(amax, 32767.0f);
+          for (int j = 0; j < 32; ++j) amax = max_abs(amax, f[j]);
+          const UpScale us = up_scale(mag(amax), 32767.0f);
 #pragma unroll
           for (int k = 0; k < kChunks; ++k)
-            if (k == c - c0) hmax[k] = hidden_max(amax);
+            if (k == c - c0) hmax[k] = hidden_max(mag(amax));
+          if (us.up != 1.0f) {  // blocks of the smallest fp32 values
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            uint32_t w2[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              w2[j] = __byte_perm(hidden_bits(f[u * 8 + 2 * j], us), hidden_bits(f[u * 8 + 2 * j + 1], us), 0x5410);
-            stage16(buf, lane, u, w2[0], w2[1], w2[2], w2[3]);
+            for (int j = 0; j < 16; ++j) v2[j] = f2_mul(v2[j], f2(us.up, us.up));
           }
+          const uint64_t r2 = f2(us.r, us.r);
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            stage16(buf, lane, u, hidden_pair(v2[u * 4], r2), hidden_pair(v2[u * 4 + 1], r2),
+                    hidden_pair(v2[u * 4 + 2], r2), hidden_pair(v2[u * 4 + 3], r2));
         } else if (p.e.out == kInt8OutF32) {
           // Two blocks of 32 x 16 fp32 values.
 #pragma unroll

@@ -47,19 +47,37 @@ inline Int8Epi int8_epi(const Int8Gemm& g) {
   return e;
 }
 
-// GELU in fp32. The int8 hidden block is quantised again right after it, so its
-// error has to stay well under an int8 step of the row's largest value: the
-// hardware tanh (error 2^-11 of the tanh) moved about 1 % of the hidden values
-// by a step, so the tanh form is written with a sigmoid instead,
-// 0.5 (1 + tanh z) = 1 / (1 + exp(-2z)), whose exponential and division are a
-// few fp32 roundings off.
-__device__ __forceinline__ float int8_gelu(float x, int mode) {
-  if (mode == kGeluErf) return 0.5f * x * (1.0f + erff(x * 0.70710678118654752f));
-  if (mode == kGeluTanh) {
-    const float z = 0.7978845608028654f * fmaf(0.044715f * x, x * x, x);
-    return __fdividef(x, 1.0f + __expf(-2.0f * z));
-  }
-  return x;
+// GELU in fp32, on packed pairs. The int8 hidden block is quantised again right
+// after it, so its error has to stay well under an int8 step of the row's largest
+// value: the hardware tanh (error 2^-11 of the tanh) moved about 1 % of the
+// hidden values by a step. The tanh form is written with a sigmoid instead,
+//   0.5 x (1 + tanh z) = x / (1 + exp(-2z)),  -2z log2(e) = x (k1 + k2 x^2),
+// whose exponential (ex2.approx, 2^-22) and reciprocal (1 ulp) cost as many
+// special-function instructions as the tanh and one more.
+__device__ __forceinline__ float ex2_approx(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ uint64_t int8_gelu_tanh(uint64_t x) {
+  // k1 = -2 log2(e) sqrt(2 / pi), k2 = 0.044715 k1
+  const uint64_t k1 = f2(-2.3022081985f, -2.3022081985f), k2 = f2(-0.10294323960f, -0.10294323960f);
+  float a, b;
+  f2_split(f2_mul(x, f2_fma(f2_mul(x, x), k2, k1)), a, b);
+  f2_split(f2_add(f2(ex2_approx(a), ex2_approx(b)), f2(1.0f, 1.0f)), a, b);
+  return f2_mul(x, f2(rcp_approx(a), rcp_approx(b)));
+}
+__device__ __forceinline__ uint64_t int8_gelu_erf(uint64_t x) {
+  float a, b;
+  f2_split(x, a, b);
+  a = 0.5f * a * (1.0f + erff(a * 0.70710678118654752f));
+  b = 0.5f * b * (1.0f + erff(b * 0.70710678118654752f));
+  return f2(a, b);
 }
 
 // Largest |value| as its bits: unsigned order puts infinities and NaN on top.
@@ -88,21 +106,32 @@ __device__ __forceinline__ UpScale up_scale(uint32_t amax_bits, float limit) {
 __device__ __forceinline__ float hidden_max(uint32_t amax_bits) {
   return __uint_as_float(amax_bits >= 0x7F800000u ? 0x7FC00000u : amax_bits);
 }
-// One hidden value in the low 16 bits; s = up_scale(its block's maximum, 32767).
-__device__ __forceinline__ uint32_t hidden_bits(float h, UpScale s) {
-  return s.r == 0.0f ? 0u : round_bits(h * s.up * s.r);
+// Two hidden values in a word; r = up_scale(their block's maximum, 32767).r, and
+// h has been taken up by its `up`. (What a block with a NaN maximum holds is not
+// read as values.)
+__device__ __forceinline__ uint32_t hidden_pair(uint64_t h, uint64_t r) {
+  const uint64_t b = f2_add(f2_mul(h, r), f2(12582912.0f, 12582912.0f));
+  return __byte_perm(static_cast<uint32_t>(b), static_cast<uint32_t>(b >> 32), 0x5410);
+}
+// max(a, |b|), NaN if one is.
+__device__ __forceinline__ float max_abs(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
+  return r;
 }
 
-// acc * sa * sb + bias: the same roundings in every kernel and layout (without a
-// bias it is 0).
-__device__ __forceinline__ float int8_scaled(int32_t acc, float sa, float sb, float bias) {
-  return __fmaf_rn(__fmul_rn(__int2float_rn(acc), sa), sb, bias);
+// acc * sa * sb + bias of two columns: the same roundings in every kernel and
+// layout (without a bias it is 0).
+__device__ __forceinline__ uint64_t int8_scaled(uint32_t acc0, uint32_t acc1, uint64_t sa, uint64_t sb,
+                                                uint64_t bias) {
+  const uint64_t v = f2(__int2float_rn(static_cast<int32_t>(acc0)), __int2float_rn(static_cast<int32_t>(acc1)));
+  return f2_fma(f2_mul(v, sa), sb, bias);
 }
 
 // Eight neighbouring columns n .. n + 7 of the epilogue's operands. `vec` says
 // that scales and bias start on 16-byte boundaries (n is a multiple of 8).
 struct Cols8 {
-  float sb[8], bias[8];
+  uint64_t sb[4], bias[4];  // fp32 pairs
 };
 __device__ __forceinline__ Cols8 int8_cols(const Int8Epi& e, int n, bool vec) {
   Cols8 c;
@@ -110,18 +139,20 @@ __device__ __forceinline__ Cols8 int8_cols(const Int8Epi& e, int n, bool vec) {
     const float4 s0 = *reinterpret_cast<const float4*>(e.b_scale + n);
     const float4 s1 = *reinterpret_cast<const float4*>(e.b_scale + n + 4);
     const uint4 b = e.bias ? *reinterpret_cast<const uint4*>(e.bias + n) : make_uint4(0u, 0u, 0u, 0u);
-    const float s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
-    const uint32_t w[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      c.sb[j] = s[j];
-      c.bias[j] = (j & 1) ? bf16_hi(w[j >> 1]) : bf16_lo(w[j >> 1]);
-    }
+    c.sb[0] = f2(s0.x, s0.y), c.sb[1] = f2(s0.z, s0.w), c.sb[2] = f2(s1.x, s1.y), c.sb[3] = f2(s1.z, s1.w);
+    c.bias[0] = f2_from_bf16x2(b.x), c.bias[1] = f2_from_bf16x2(b.y);
+    c.bias[2] = f2_from_bf16x2(b.z), c.bias[3] = f2_from_bf16x2(b.w);
   } else {
+    float sb[8], bias[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      c.sb[j] = n + j < e.N ? e.b_scale[n + j] : 0.0f;
-      c.bias[j] = e.bias && n + j < e.N ? __bfloat162float(e.bias[n + j]) : 0.0f;
+      sb[j] = n + j < e.N ? e.b_scale[n + j] : 0.0f;
+      bias[j] = e.bias && n + j < e.N ? __bfloat162float(e.bias[n + j]) : 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      c.sb[j] = f2(sb[2 * j], sb[2 * j + 1]);
+      c.bias[j] = f2(bias[2 * j], bias[2 * j + 1]);
     }
   }
   return c;
@@ -133,15 +164,18 @@ __device__ __forceinline__ Cols8 int8_cols(const Int8Epi& e, int n, bool vec) {
 // 4096 x 4096: 40 us, of which the weights' stream is 3).
 __device__ __forceinline__ void int8_values(const Int8Epi& e, const uint32_t (&acc)[8], float sa, const Cols8& c,
                                             float (&f)[8]) {
+  uint64_t v[4];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) f[j] = int8_scaled(static_cast<int32_t>(acc[j]), sa, c.sb[j], c.bias[j]);
+  for (int j = 0; j < 4; ++j) v[j] = int8_scaled(acc[2 * j], acc[2 * j + 1], f2(sa, sa), c.sb[j], c.bias[j]);
   if (e.gelu == kGeluErf) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = int8_gelu(f[j], kGeluErf);
+    for (int j = 0; j < 4; ++j) v[j] = int8_gelu_erf(v[j]);
   } else if (e.gelu == kGeluTanh) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = int8_gelu(f[j], kGeluTanh);
+    for (int j = 0; j < 4; ++j) v[j] = int8_gelu_tanh(v[j]);
   }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) f2_split(v[j], f[2 * j], f[2 * j + 1]);
 }
 
 __device__ __forceinline__ void add8_bf16(const uint4& b, float (&f)[8]) {
@@ -179,7 +213,8 @@ __device__ __forceinline__ void int8_store_hidden(const Int8Epi& e, int64_t m, i
   const UpScale us = up_scale(amax, 32767.0f);
   uint32_t w[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) w[j] = __byte_perm(hidden_bits(f[2 * j], us), hidden_bits(f[2 * j + 1], us), 0x5410);
+  for (int j = 0; j < 4; ++j)
+    w[j] = hidden_pair(f2_mul(f2(f[2 * j], f[2 * j + 1]), f2(us.up, us.up)), f2(us.r, us.r));
   // The block's row stride is a multiple of 16 values, so eight at a multiple of
   // eight stay in the row.
   *reinterpret_cast<uint4*>(static_cast<int16_t*>(e.C) + m * e.ldc + n) = make_uint4(w[0], w[1], w[2], w[3]);

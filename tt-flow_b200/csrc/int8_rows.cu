@@ -74,12 +74,6 @@ __device__ __forceinline__ uint64_t in_pair(uint32_t w) {
   return f2_from_bf16x2(w);
 }
 
-// max(a, |b|), NaN if one is.
-__device__ __forceinline__ float max_abs(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
-  return r;
-}
 __device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
   uint32_t r;
   asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
@@ -157,8 +151,12 @@ __global__ void __launch_bounds__(WARP ? 128 : kMaxT, !WARP && PER == 32 && KIND
   clear_words(p.zero, p.zero_vecs);
   const int T = WARP ? 32 : blockDim.x;
   const int t = WARP ? threadIdx.x & 31 : threadIdx.x;
-  const int64_t row = WARP ? static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5) : blockIdx.x;
-  if (WARP && row >= p.M) return;
+  // The hidden block is read from its last row, which the up projection wrote
+  // last (what is left of it in L2 is read first), to its first, which the down
+  // projection reads first.
+  const int64_t at = WARP ? static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5) : blockIdx.x;
+  const int64_t row = KIND == kInt8RowsHidden ? p.M - 1 - at : at;
+  if (WARP && at >= p.M) return;
   const uint16_t* x = static_cast<const uint16_t*>(p.x) + row * p.ldx;
   const uint16_t* r = RES ? reinterpret_cast<const uint16_t*>(p.residual) + row * p.ldr : nullptr;
   const uint16_t* g = reinterpret_cast<const uint16_t*>(p.gamma);
