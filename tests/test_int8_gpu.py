@@ -96,6 +96,25 @@ def test_rmsnorm(ops, m, k, residual):
         assert len(res) == 2
 
 
+@pytest.mark.parametrize("k", [256, 259, 4096, 20000, 40008])
+def test_quantize_ties(ops, k):
+    """Values halfway between two steps go to the even one, whatever the row's scale: x = j / 2 * 2^e * c with amax
+    127 * 2^e * c, all exact in bf16, lies j / 2 steps from zero."""
+    j = torch.arange(k, device="cuda") % 255 - 127
+    for e in (-100, -3, 0, 5, 90):
+        x = (j.double() / 2 * 2.0 ** e).bfloat16()
+        x[0] = 127 * 2.0 ** e
+        q, scale = ops.quantize_int8(x.repeat(3, 1))
+        want = torch.round(j.double() / 2)  # half to even
+        want[0] = 127
+        assert torch.equal(q[1].double(), want) and scale[1].double() == 2.0 ** e
+    # amax = 4.03125: 127 / amax is not exact, 2.015625 is half of amax
+    x = torch.full((2, k), 2.015625, device="cuda").bfloat16()
+    x[:, 1] = -4.03125
+    q, _ = ops.quantize_int8(x)
+    assert (q[:, 0] == 64).all() and (q[:, 1] == -127).all()
+
+
 @pytest.mark.parametrize("k", [64, 1000, 1001, 5000, 33000])
 @pytest.mark.parametrize("offset,pad", [(0, 0), (1, 0), (8, 8), (3, 5)])
 def test_rows_strides_and_surroundings(ops, k, offset, pad):

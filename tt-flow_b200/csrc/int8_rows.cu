@@ -45,6 +45,7 @@ struct RowsParams {
   float* scale;
   const float* hidden_max;
   int64_t ldm;
+  float one;  // 1 (q_pair)
   uint4* zero;
   int64_t zero_vecs;
 };
@@ -127,9 +128,13 @@ __device__ __forceinline__ RowScale row_scale(const RowsParams& p, RowStat s) {
   return o;
 }
 
-// rn of two values in the low bytes of a pair's halves.
-__device__ __forceinline__ uint64_t q_pair(uint64_t v, uint64_t r) {
-  return f2_add(f2_mul(v, r), f2(12582912.0f, 12582912.0f));
+// rn of two values in the low bytes of a pair's halves. The product is rounded to
+// fp32 before the integer: bf16 rows hold many values halfway between two steps,
+// and 127 / amax rounded down would take them off the tie. ptxas contracts a
+// packed product and sum into one rounding, so the sum is a multiply-add by a 1
+// that only the launch knows.
+__device__ __forceinline__ uint64_t q_pair(uint64_t v, uint64_t r, uint64_t one) {
+  return f2_fma(f2_mul(v, r), one, f2(12582912.0f, 12582912.0f));
 }
 __device__ __forceinline__ uint32_t pack4(uint64_t a, uint64_t b) {
   const uint32_t lo = __byte_perm(static_cast<uint32_t>(a), static_cast<uint32_t>(a >> 32), 0x0040);
@@ -252,7 +257,7 @@ __global__ void __launch_bounds__(WARP ? 128 : kMaxT, !WARP && PER == 32 && KIND
   int8_t* q = p.q + row * p.ldq;
   // A row of zeros, or one that is not finite, is stored as zeros.
   const uint32_t keep = sc.u.r == 0.0f ? 0u : 0xFFFFFFFFu;
-  const uint64_t rr = f2(sc.u.r, sc.u.r), up = f2(sc.u.up, sc.u.up);
+  const uint64_t rr = f2(sc.u.r, sc.u.r), up = f2(sc.u.up, sc.u.up), one = f2(p.one, p.one);
 #pragma unroll
   for (int i = 0; i < G; ++i) {
     const int k = first(i);
@@ -264,7 +269,7 @@ __global__ void __launch_bounds__(WARP ? 128 : kMaxT, !WARP && PER == 32 && KIND
     for (int j = 0; j < 4; ++j) {
       uint64_t s = KIND == kInt8RowsNorm ? v[KIND == kInt8RowsNorm ? i : 0][j] : in_pair<KIND>(xw[i][j]);
       if (KIND != kInt8RowsHidden && sc.u.up != 1.0f) s = f2_mul(s, up);
-      b[j] = q_pair(s, KIND == kInt8RowsHidden ? f2(hr, hr) : rr);
+      b[j] = q_pair(s, KIND == kInt8RowsHidden ? f2(hr, hr) : rr, one);
     }
     const uint2 o = make_uint2(pack4(b[0], b[1]) & keep, pack4(b[2], b[3]) & keep);
     if (VEC && k + 8 <= K) {
@@ -401,6 +406,7 @@ int run_int8_rows(const Int8Rows& r, cudaStream_t stream, std::string* err) {
   p.ldq = r.ldq;
   p.scale = r.scale;
   p.hidden_max = r.hidden_max;
+  p.one = 1.0f;
   p.ldm = r.ldm;
   p.zero = static_cast<uint4*>(r.zero);
   p.zero_vecs = static_cast<int64_t>(r.zero_bytes / 16);
