@@ -37,6 +37,7 @@ def test_quantize_refusals(lib):
     refused(lib, L.TFB200_EINVAL, "negative", fn, R(mat(-1, 64, L.TFB200_BF16)), R(q), 4096, None)
     refused(lib, L.TFB200_EINVAL, "2^30", fn, R(mat((1 << 30) + 1, 64, L.TFB200_BF16)), R(q), 4096, None)
     refused(lib, L.TFB200_EINVAL, "null scale", fn, R(x), R(q), None, None)
+    refused(lib, L.TFB200_EINVAL, "scale: not aligned", fn, R(x), R(q), 4098, None)
     assert lib.tfb200_quantize_int8(R(mat(0, 64, L.TFB200_BF16)), R(mat(0, 64, L.TFB200_I8)), None, None) == 0
 
 
@@ -45,6 +46,7 @@ def test_rmsnorm_refusals(lib):
     fn = "tfb200_rmsnorm_int8"
     refused(lib, L.TFB200_EINVAL, "null gamma", fn, R(x), None, None, 1e-5, None, R(q), 4096, None)
     refused(lib, L.TFB200_EINVAL, "eps", fn, R(x), None, 4096, -1.0, None, R(q), 4096, None)
+    refused(lib, L.TFB200_EINVAL, "gamma: not aligned", fn, R(x), None, 4097, 1e-5, None, R(q), 4096, None)
     refused(lib, L.TFB200_EINVAL, "eps", fn, R(x), None, 4096, float("nan"), None, R(q), 4096, None)
     refused(lib, L.TFB200_EINVAL, "sum", fn, R(x), R(x), 4096, 1e-5, None, R(q), 4096, None)
     refused(lib, L.TFB200_EINVAL, "without a residual", fn, R(x), None, 4096, 1e-5, R(x), R(q), 4096, None)
@@ -69,6 +71,7 @@ def test_matmul_refusals(lib):
     refused(lib, L.TFB200_EINVAL, "gelu_mode", fn, *call(gelu=3))
     refused(lib, L.TFB200_EINVAL, "null scales", fn, *call(sa=None))
     refused(lib, L.TFB200_EINVAL, "null scales", fn, *call(sb=None))
+    refused(lib, L.TFB200_EINVAL, "b_scale: not aligned", fn, *call(sb=4098))
     refused(lib, L.TFB200_EINVAL, "not aligned", fn, *call(c=mat(4, 8, L.TFB200_F32, data=4098)))
     k = 131072
     refused(lib, L.TFB200_EUNSUPPORTED, "131071", fn, *call(a=mat(4, k, L.TFB200_I8), b=mat(8, k, L.TFB200_I8)))

@@ -141,6 +141,33 @@ def test_rows_strides_and_surroundings(ops, k, offset, pad):
     assert t2 is x2 and torch.equal(x2, want[2]) and torch.equal(q2, want[0])
 
 
+@pytest.mark.parametrize("m,k", [(3000, 1), (3000, 9), (2500, 1001), (2500, 1032), (700, 4099), (700, 4104), (300, 16383)])
+@pytest.mark.parametrize("offset", [0, 1, 5])
+def test_rows_many_in_place(ops, m, k, offset):
+    """Many rows of odd width, starting anywhere, the sum written over x; q in its usual layout."""
+    g = gen(m + k)
+    x, r = normal(g, m, k).bfloat16(), normal(g, m, k).bfloat16()
+    gamma = (torch.rand(k, generator=g, device="cuda") + 0.5).bfloat16()
+    s = x.float() + r.float()
+    t = s * gamma.float()
+    amax = t.abs().amax(1, keepdim=True)
+    want = torch.where(amax > 0, torch.round(t * (127.0 / amax)), amax)  # the same fp32 roundings
+    xv, xbuf = rows_at(x, offset, k)
+    rv, _ = rows_at(r, offset, k)
+    qp = torch.full((m, (k + 15) // 16 * 16), 77, dtype=torch.int8, device="cuda")
+    scale = torch.empty(m, device="cuda")
+    ops.rmsnorm_int8(xv, gamma, EPS, residual=rv, out=(qp[:, :k], scale, xv))
+    assert torch.equal(qp[:, :k].float(), want) and torch.equal(xv, s.bfloat16())
+    assert (qp[:, k:] == 77).all()
+    assert (xbuf[:offset] == 77).all() and (xbuf[offset + m * k:] == 77).all()
+    ref = amax[:, 0].double() / torch.sqrt(s.double().pow(2).mean(1) + EPS) / 127
+    assert ((scale.double() - ref).abs() <= 60 * U32 * ref).all()
+    xv.copy_(x)
+    q, _ = ops.quantize_int8(xv)
+    xa = x.float().abs().amax(1, keepdim=True)
+    assert torch.equal(q.float(), torch.where(xa > 0, torch.round(x.float() * (127.0 / xa)), xa))
+
+
 @pytest.mark.parametrize("k", [5, 256, 3001, 40000])
 def test_rows_special_values(ops, k):
     x = normal(gen(k), 8, k).bfloat16()

@@ -53,6 +53,13 @@ bool mat_ok(const tfb200_mat* m, const char* name, int32_t dtype, std::string* e
   return false;
 }
 
+// gamma and bias (2 bytes), scales (4): null is the caller's to judge.
+bool vec_ok(const void* p, unsigned bytes, const char* name, std::string* err) {
+  if (!(reinterpret_cast<uintptr_t>(p) & (bytes - 1))) return true;
+  *err = std::string(name) + ": not aligned to its element";
+  return false;
+}
+
 bool same_shape(const tfb200_mat* a, const tfb200_mat* b) { return a->rows == b->rows && a->cols == b->cols; }
 
 const bf16* as_bf16(const void* p) { return static_cast<const bf16*>(p); }
@@ -121,7 +128,8 @@ int tfb200_quantize_int8(const tfb200_mat* x, tfb200_mat* q, float* scale, void*
   static const char fn[] = "tfb200_quantize_int8";
   return guarded([&] {
     std::string err;
-    if (!mat_ok(x, "x", TFB200_BF16, &err) || !mat_ok(q, "q", TFB200_I8, &err)) return fail(TFB200_EINVAL, fn, err);
+    if (!mat_ok(x, "x", TFB200_BF16, &err) || !mat_ok(q, "q", TFB200_I8, &err) || !vec_ok(scale, 4, "scale", &err))
+      return fail(TFB200_EINVAL, fn, err);
     if (!same_shape(x, q)) return fail(TFB200_EINVAL, fn, "q must have the shape of x");
     if (x->rows == 0) return static_cast<int>(TFB200_OK);
     if (!scale) return fail(TFB200_EINVAL, fn, "null scale");
@@ -144,6 +152,7 @@ int tfb200_rmsnorm_int8(const tfb200_mat* x, const tfb200_mat* residual, const v
   return guarded([&] {
     std::string err;
     if (!mat_ok(x, "x", TFB200_BF16, &err) || !mat_ok(q, "q", TFB200_I8, &err) ||
+        !vec_ok(gamma, 2, "gamma", &err) || !vec_ok(scale, 4, "scale", &err) ||
         (residual && (!mat_ok(residual, "residual", TFB200_BF16, &err) || !mat_ok(sum, "sum", TFB200_BF16, &err))))
       return fail(TFB200_EINVAL, fn, err);
     if (!same_shape(x, q) || (residual && (!same_shape(x, residual) || !same_shape(x, sum))))
@@ -189,7 +198,8 @@ int tfb200_matmul_int8(const tfb200_mat* a, const float* a_scale, const tfb200_m
     std::string err;
     const bool f32 = c && c->dtype == TFB200_F32;
     if (!mat_ok(a, "a", TFB200_I8, &err) || !mat_ok(b, "b", TFB200_I8, &err) ||
-        !mat_ok(c, "c", f32 ? TFB200_F32 : TFB200_BF16, &err) ||
+        !vec_ok(a_scale, 4, "a_scale", &err) || !vec_ok(b_scale, 4, "b_scale", &err) ||
+        !vec_ok(bias, 2, "bias", &err) || !mat_ok(c, "c", f32 ? TFB200_F32 : TFB200_BF16, &err) ||
         (residual && !mat_ok(residual, "residual", TFB200_BF16, &err)))
       return fail(TFB200_EINVAL, fn, err);
     if (a->cols != b->cols || c->rows != a->rows || c->cols != b->rows || (residual && !same_shape(residual, c)))
@@ -245,7 +255,8 @@ int tfb200_fused_rmsnorm_matmul_int8(const tfb200_mat* x, const void* gamma, con
   static const char fn[] = "tfb200_fused_rmsnorm_matmul_int8";
   return guarded([&] {
     std::string err;
-    if (!mat_ok(x, "x", TFB200_BF16, &err) || !mat_ok(w, "w", TFB200_I8, &err) || !mat_ok(y, "y", TFB200_BF16, &err))
+    if (!mat_ok(x, "x", TFB200_BF16, &err) || !mat_ok(w, "w", TFB200_I8, &err) ||
+        !mat_ok(y, "y", TFB200_BF16, &err) || !vec_ok(gamma, 2, "gamma", &err) || !vec_ok(w_scale, 4, "w_scale", &err))
       return fail(TFB200_EINVAL, fn, err);
     const int64_t M = x->rows, K = x->cols, N = w->rows;
     if (w->cols != K || y->rows != M || y->cols != N)
@@ -308,7 +319,8 @@ int tfb200_fused_mlp_int8(const tfb200_mat* x, const void* gamma, const tfb200_m
     std::string err;
     if (!mat_ok(x, "x", TFB200_BF16, &err) || !mat_ok(w1, "w1", TFB200_I8, &err) ||
         !mat_ok(w2, "w2", TFB200_I8, &err) || !mat_ok(residual, "residual", TFB200_BF16, &err) ||
-        !mat_ok(y, "y", TFB200_BF16, &err))
+        !mat_ok(y, "y", TFB200_BF16, &err) || !vec_ok(gamma, 2, "gamma", &err) || !vec_ok(b1, 2, "b1", &err) ||
+        !vec_ok(w1_scale, 4, "w1_scale", &err) || !vec_ok(w2_scale, 4, "w2_scale", &err))
       return fail(TFB200_EINVAL, fn, err);
     const int64_t M = x->rows, K = x->cols, H = w1->rows, N = w2->rows;
     if (w1->cols != K || w2->cols != H || y->rows != M || y->cols != N || !same_shape(residual, y))

@@ -46,6 +46,8 @@ struct RowsParams {
   const float* hidden_max;
   int64_t ldm;
   float one;  // 1 (q_pair)
+  int ahead;  // prefetch_row
+  int64_t span_x, span_r;  // values from the first row's start to the last row's end
   uint4* zero;
   int64_t zero_vecs;
 };
@@ -75,6 +77,13 @@ __device__ __forceinline__ uint64_t in_pair(uint32_t w) {
   return f2_from_bf16x2(w);
 }
 
+// max(a, |b|, |c|), NaN if one is (a is not negative).
+__device__ __forceinline__ float max_abs(float a, uint64_t bc) {
+  float b, c, r;
+  f2_split(bc, b, c);
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 __device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
   uint32_t r;
   asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
@@ -111,21 +120,20 @@ __device__ __forceinline__ RowStat block_stat(RowStat s, bool squares) {
   return warp_stat(s, squares);
 }
 
-struct RowScale {
-  UpScale u;  // q = rn(t * u.up * u.r)
-  float scale;
-};
-
+// The scale of a row; only the thread that stores it computes it (its root and
+// divisions are as long as a warp's share of a 4096-wide row).
 template <int KIND>
-__device__ __forceinline__ RowScale row_scale(const RowsParams& p, RowStat s) {
-  RowScale o;
-  if (KIND == kInt8RowsNorm && !(s.ss <= 3.402823466e38f)) s.amax = 0x7FC00000u;
-  o.u = up_scale(s.amax, 127.0f);
+__device__ __forceinline__ float row_scale(const RowsParams& p, RowStat s) {
+  if (s.amax >= 0x7F800000u) return __uint_as_float(0x7FC00000u);
   const float amax = __uint_as_float(s.amax);
-  o.scale = KIND == kInt8RowsNorm ? amax * (1.0f / sqrtf(s.ss / static_cast<float>(p.K) + p.eps) / 127.0f)
-                                  : amax / 127.0f;
-  if (s.amax >= 0x7F800000u) o.scale = __uint_as_float(0x7FC00000u);
-  return o;
+  return KIND == kInt8RowsNorm ? amax * (1.0f / sqrtf(s.ss / static_cast<float>(p.K) + p.eps) / 127.0f)
+                               : amax / 127.0f;
+}
+// Marks a row whose sum of squares left fp32 as not finite.
+template <int KIND>
+__device__ __forceinline__ RowStat checked(RowStat s) {
+  if (KIND == kInt8RowsNorm && !(s.ss <= 3.402823466e38f)) s.amax = 0x7FC00000u;
+  return s;
 }
 
 // rn of two values in the low bytes of a pair's halves. The product is rounded to
@@ -142,12 +150,44 @@ __device__ __forceinline__ uint32_t pack4(uint64_t a, uint64_t b) {
   return __byte_perm(lo, hi, 0x5410);
 }
 
-// VEC: rows start on 16-byte boundaries (8 for q); a thread takes 8 neighbouring
-// values at a time. Otherwise a thread takes single values, T apart.
+// The 16 bytes that start `half` 16-bit values into the 32 bytes w.
+__device__ __forceinline__ void from_half(const uint32_t (&w)[8], int half, uint32_t (&o)[4]) {
+  uint32_t a[7], b[5];
+#pragma unroll
+  for (int i = 0; i < 7; ++i) a[i] = half & 2 ? w[i + 1] : w[i];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) b[i] = half & 4 ? a[i + 2] : a[i];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = __funnelshift_r(b[i], b[i + 1], 16 * (half & 1));
+}
+
+// How a row's values reach its threads.
+//   kScalar: one at a time, T apart (any layout).
+//   kVec:    8 neighbours at a time; x, residual and sum start every row on a
+//            16-byte boundary, gamma and q (8) as well.
+//   kShift:  8 neighbours at a time; the rows of x, residual and sum start
+//            anywhere, but all three at the same place of their 16-byte granules
+//            (odd widths). A thread reads two neighbouring granules and takes
+//            its 8 values from them; the sum is formed on granules. Single loads
+//            took 7 times as long (8192 x 4099: 117 us against 16).
+enum Mode : int { kScalar, kVec, kShift };
+
+// Rows ahead that are brought into L2: about 12 MB of them, so that HBM is kept
+// busy while blocks reduce and store.
+constexpr int64_t kAheadBytes = 12 << 20;
+
+__device__ __forceinline__ void prefetch_row(const uint16_t* row, int K) {
+  const uint64_t lo = (reinterpret_cast<uint64_t>(row) + 15) & ~uint64_t(15);
+  const uint64_t hi = reinterpret_cast<uint64_t>(row + K) & ~uint64_t(15);
+  if (hi > lo)
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(lo), "r"(static_cast<uint32_t>(hi - lo))
+                 : "memory");
+}
+
 // WARP: a warp per row (T = 32), else a block per row (T = blockDim.x).
 // PER: values per thread.
-template <int KIND, bool RES, bool VEC, bool WARP, int PER>
-__global__ void __launch_bounds__(WARP ? 128 : kMaxT, !WARP && PER == 32 && KIND == kInt8RowsHidden ? 3 : 1)
+template <int KIND, bool RES, Mode MODE, bool WARP, int PER>
+__global__ void __launch_bounds__(WARP ? 128 : kMaxT, !WARP && PER == 32 && MODE == kVec && KIND != kInt8RowsNorm ? 3 : 1)
     k_int8_rows(const RowsParams p) {
   // Launched with programmatic serialization: wait for the grid before (it may
   // write x or still read q), then let the next grid start its prologue.
@@ -162,18 +202,27 @@ __global__ void __launch_bounds__(WARP ? 128 : kMaxT, !WARP && PER == 32 && KIND
   const int64_t at = WARP ? static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5) : blockIdx.x;
   const int64_t row = KIND == kInt8RowsHidden ? p.M - 1 - at : at;
   if (WARP && at >= p.M) return;
-  const uint16_t* x = static_cast<const uint16_t*>(p.x) + row * p.ldx;
-  const uint16_t* r = RES ? reinterpret_cast<const uint16_t*>(p.residual) + row * p.ldr : nullptr;
+  const uint16_t* const x0 = static_cast<const uint16_t*>(p.x);
+  const uint16_t* const r0 = reinterpret_cast<const uint16_t*>(p.residual);
+  const uint16_t* x = x0 + row * p.ldx;
+  const uint16_t* r = RES ? r0 + row * p.ldr : nullptr;
   const uint16_t* g = reinterpret_cast<const uint16_t*>(p.gamma);
   const int K = p.K;
+  if (t == 0 && at + p.ahead < p.M) {
+    const int64_t next = KIND == kInt8RowsHidden ? row - p.ahead : row + p.ahead;
+    prefetch_row(x0 + next * p.ldx, K);
+    if (RES) prefetch_row(r0 + next * p.ldr, K);
+  }
   // Groups of 8 values: the first of group i, and the distance between them.
   constexpr int G = PER / 8;
-  const int step = VEC ? 1 : T;
-  auto first = [&](int i) { return VEC ? (t + i * T) * 8 : t + i * 8 * T; };
+  const int step = MODE == kScalar ? T : 1;
+  auto first = [&](int i) { return MODE == kScalar ? t + i * 8 * T : (t + i * T) * 8; };
+  // kShift: granule i holds values 8i - phase ..
+  const int phase = MODE == kShift ? static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15u) / 2) : 0;
 
   // Plain loads: the sum may be written over x or the residual.
   auto load8 = [&](const uint16_t* src, int k, uint32_t (&w)[4]) {
-    if (VEC && k + 8 <= K) {
+    if (MODE != kScalar && k + 8 <= K) {
       const uint4 v = *reinterpret_cast<const uint4*>(src + k);
       w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
     } else {
@@ -185,15 +234,65 @@ __global__ void __launch_bounds__(WARP ? 128 : kMaxT, !WARP && PER == 32 && KIND
       }
     }
   };
-  uint32_t xw[G][4], rw[RES ? G : 1][4], gw[KIND == kInt8RowsNorm && VEC ? G : 1][4];
+  // A granule from value k (k may be negative) of a row of [base, base + span);
+  // one that reaches past the matrix is read value by value.
+  auto granule = [&](const uint16_t* src, int k, const uint16_t* base, int64_t span, uint32_t* w) {
+    const uint16_t* s = src + k;
+    if (k >= K) {
+      w[0] = w[1] = w[2] = w[3] = 0u;
+    } else if (s >= base && s + 8 <= base + span) {
+      const uint4 v = *reinterpret_cast<const uint4*>(s);
+      w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t lo = k + 2 * j >= 0 && k + 2 * j < K ? s[2 * j] : 0u;
+        const uint32_t hi = k + 2 * j + 1 >= 0 && k + 2 * j + 1 < K ? s[2 * j + 1] : 0u;
+        w[j] = lo | hi << 16;
+      }
+    }
+  };
+  // The row's values k .. k + 7 (0 past its end) from its granules; raw gets the
+  // first of these.
+  auto load_shifted = [&](const uint16_t* src, int k, const uint16_t* base, int64_t span, uint32_t (&w)[4],
+                          uint32_t (&raw)[4]) {
+    uint32_t b[8];
+    granule(src, k - phase, base, span, b);
+    granule(src, k - phase + 8, base, span, b + 4);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) raw[j] = b[j];
+    from_half(b, phase, w);
+    if (k + 8 > K) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        w[j] &= (k + 2 * j < K ? 0xFFFFu : 0u) | (k + 2 * j + 1 < K ? 0xFFFF0000u : 0u);
+    }
+  };
+  uint32_t xw[G][4], rw[RES ? G : 1][4], gw[KIND == kInt8RowsNorm && MODE == kVec ? G : 1][4];
+  uint32_t sums[RES ? G : 1][4];  // bf16(x + residual); kShift: of the granule
   float hm[KIND == kInt8RowsHidden ? G : 1];
 #pragma unroll
   for (int i = 0; i < G; ++i) {
-    load8(x, first(i), xw[i]);
-    if (RES) load8(r, first(i), rw[i]);
-    if (KIND == kInt8RowsNorm && VEC) load8(g, first(i), gw[VEC ? i : 0]);
+    const int k = first(i);
+    if (MODE == kShift) {
+      uint32_t xg[4], rg[4];
+      load_shifted(x, k, x0, p.span_x, xw[i], xg);
+      if (RES) {
+        load_shifted(r, k, r0, p.span_r, rw[i], rg);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float lo, hi;
+          f2_split(f2_add(in_pair<KIND>(xg[j]), in_pair<KIND>(rg[j])), lo, hi);
+          sums[i][j] = pack_bf16(lo, hi);
+        }
+      }
+    } else {
+      load8(x, k, xw[i]);
+      if (RES) load8(r, k, rw[i]);
+    }
+    if (KIND == kInt8RowsNorm && MODE == kVec) load8(g, k, gw[MODE == kVec ? i : 0]);
     // Eight hidden values lie in one block of 32.
-    if (KIND == kInt8RowsHidden) hm[i] = first(i) < K ? p.hidden_max[row * p.ldm + first(i) / kHiddenBlock] : 0.0f;
+    if (KIND == kInt8RowsHidden) hm[i] = k < K ? p.hidden_max[row * p.ldm + k / kHiddenBlock] : 0.0f;
   }
   RowStat st{0.0f, 0u};
   uint64_t v[KIND == kInt8RowsNorm ? G : 1][4];  // kInt8RowsNorm: t
@@ -214,34 +313,19 @@ __global__ void __launch_bounds__(WARP ? 128 : kMaxT, !WARP && PER == 32 && KIND
     for (int i = 0; i < G; ++i) {
       const int k = first(i);
       if (k < K) {
-        uint64_t s[4];
-        if (!VEC) load8(g, k, gw[0]);  // single loads: all of them at once would not fit the registers
+        // Gamma beside the values only where it is read with them.
+        if (MODE != kVec) load8(g, k, gw[0]);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          s[j] = in_pair<KIND>(xw[i][j]);
-          if (RES) s[j] = f2_add(s[j], in_pair<KIND>(rw[RES ? i : 0][j]));
-          ss = f2_fma(s[j], s[j], ss);
-          v[i][j] = f2_mul(s[j], in_pair<KIND>(gw[VEC ? i : 0][j]));
-          float lo, hi;
-          f2_split(v[i][j], lo, hi);
-          amax = max_abs(max_abs(amax, lo), hi);
-        }
-        if (RES) {
-          bf16* sum = p.sum + row * p.lds;
-          uint32_t o[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
+          uint64_t s = in_pair<KIND>(xw[i][j]);
+          if (RES) s = f2_add(s, in_pair<KIND>(rw[RES ? i : 0][j]));
+          ss = f2_fma(s, s, ss);
+          v[i][j] = f2_mul(s, in_pair<KIND>(gw[MODE == kVec ? i : 0][j]));
+          amax = max_abs(amax, v[i][j]);
+          if (RES && MODE != kShift) {
             float lo, hi;
-            f2_split(s[j], lo, hi);
-            o[j] = pack_bf16(lo, hi);
-          }
-          if (VEC && k + 8 <= K) {
-            *reinterpret_cast<uint4*>(sum + k) = make_uint4(o[0], o[1], o[2], o[3]);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              if (k + j * step < K)
-                reinterpret_cast<uint16_t*>(sum)[k + j * step] = static_cast<uint16_t>(o[j >> 1] >> (16 * (j & 1)));
+            f2_split(s, lo, hi);
+            sums[RES ? i : 0][j] = pack_bf16(lo, hi);
           }
         }
       }
@@ -252,27 +336,47 @@ __global__ void __launch_bounds__(WARP ? 128 : kMaxT, !WARP && PER == 32 && KIND
     st.amax = mag(amax);
   }
   st = WARP ? warp_stat(st, KIND == kInt8RowsNorm) : block_stat(st, KIND == kInt8RowsNorm);
-  const RowScale sc = row_scale<KIND>(p, st);
-  if (t == 0) p.scale[row] = sc.scale;
+  if (RES) {
+    // After the row's last load: a thread's granules are its neighbour's too, and
+    // the sum may be written over x or the residual.
+    uint16_t* sum = reinterpret_cast<uint16_t*>(p.sum + row * p.lds);
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      const int k = first(i) - phase;
+      if (k >= K) break;
+      const uint32_t(&o)[4] = sums[RES ? i : 0];
+      if (MODE != kScalar && k >= 0 && k + 8 <= K) {
+        *reinterpret_cast<uint4*>(sum + k) = make_uint4(o[0], o[1], o[2], o[3]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (k + j * step >= 0 && k + j * step < K)
+            sum[k + j * step] = static_cast<uint16_t>(o[j >> 1] >> (16 * (j & 1)));
+      }
+    }
+  }
+  st = checked<KIND>(st);
+  const UpScale u = up_scale(st.amax, 127.0f);  // q = rn(t * u.up * u.r)
+  if (t == 0) p.scale[row] = row_scale<KIND>(p, st);
   int8_t* q = p.q + row * p.ldq;
   // A row of zeros, or one that is not finite, is stored as zeros.
-  const uint32_t keep = sc.u.r == 0.0f ? 0u : 0xFFFFFFFFu;
-  const uint64_t rr = f2(sc.u.r, sc.u.r), up = f2(sc.u.up, sc.u.up), one = f2(p.one, p.one);
+  const uint32_t keep = u.r == 0.0f ? 0u : 0xFFFFFFFFu;
+  const uint64_t rr = f2(u.r, u.r), up = f2(u.up, u.up), one = f2(p.one, p.one);
 #pragma unroll
   for (int i = 0; i < G; ++i) {
     const int k = first(i);
     if (k >= K) break;
     uint64_t b[4];
     // A hidden value and its factor: h = value * block, q = rn(value * block * r).
-    const float hr = KIND == kInt8RowsHidden ? hm[i] * sc.u.up * sc.u.r * (1.0f / 32767.0f) : 0.0f;
+    const float hr = KIND == kInt8RowsHidden ? hm[i] * u.up * u.r * (1.0f / 32767.0f) : 0.0f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       uint64_t s = KIND == kInt8RowsNorm ? v[KIND == kInt8RowsNorm ? i : 0][j] : in_pair<KIND>(xw[i][j]);
-      if (KIND != kInt8RowsHidden && sc.u.up != 1.0f) s = f2_mul(s, up);
+      if (KIND != kInt8RowsHidden && u.up != 1.0f) s = f2_mul(s, up);
       b[j] = q_pair(s, KIND == kInt8RowsHidden ? f2(hr, hr) : rr, one);
     }
     const uint2 o = make_uint2(pack4(b[0], b[1]) & keep, pack4(b[2], b[3]) & keep);
-    if (VEC && k + 8 <= K) {
+    if (MODE != kScalar && k + 8 <= K) {
       *reinterpret_cast<uint2*>(q + k) = o;
     } else {
 #pragma unroll
@@ -315,8 +419,9 @@ __global__ void __launch_bounds__(1024) k_int8_rows_long(const RowsParams p) {
     }
   }
   st = block_stat(st, KIND == kInt8RowsNorm);
-  const RowScale sc = row_scale<KIND>(p, st);
-  if (threadIdx.x == 0) p.scale[row] = sc.scale;
+  st = checked<KIND>(st);
+  const UpScale u = up_scale(st.amax, 127.0f);  // q = rn(t * u.up * u.r)
+  if (threadIdx.x == 0) p.scale[row] = row_scale<KIND>(p, st);
   // A thread reads a value of x again before it writes the sum, which may be x.
 #pragma unroll 4
   for (int k = threadIdx.x; k < p.K; k += blockDim.x) {
@@ -325,26 +430,29 @@ __global__ void __launch_bounds__(1024) k_int8_rows_long(const RowsParams p) {
     if (KIND == kInt8RowsNorm) s = __fmul_rn(s, in_value<KIND>(g[k]));
     uint32_t b;
     if (KIND == kInt8RowsHidden)
-      b = round_bits(s * (p.hidden_max[row * p.ldm + k / kHiddenBlock] * sc.u.up * sc.u.r * (1.0f / 32767.0f)));
+      b = round_bits(s * (p.hidden_max[row * p.ldm + k / kHiddenBlock] * u.up * u.r * (1.0f / 32767.0f)));
     else
-      b = round_bits(__fmul_rn(__fmul_rn(s, sc.u.up), sc.u.r));
-    p.q[row * p.ldq + k] = sc.u.r == 0.0f ? 0 : static_cast<int8_t>(b & 0xFFu);
+      b = round_bits(__fmul_rn(__fmul_rn(s, u.up), u.r));
+    p.q[row * p.ldq + k] = u.r == 0.0f ? 0 : static_cast<int8_t>(b & 0xFFu);
   }
 }
 
 template <int KIND, bool RES>
-cudaError_t launch_rows(const RowsParams& p, bool vec, cudaStream_t s) {
-  constexpr bool kV = KIND == kInt8RowsHidden;  // the hidden block is always aligned
-  vec = vec || kV;
-  const bool warp = p.K <= 32 * 32, wide = p.K > 32 * kMaxT, longer = p.K > kMaxRow || (wide && !vec);
+cudaError_t launch_rows(RowsParams p, Mode mode, cudaStream_t s) {
+  const bool hidden = KIND == kInt8RowsHidden;  // always aligned
+  if (hidden) mode = kVec;
+  // kShift: a granule more than the values fill.
+  const int K = p.K + (mode == kShift && RES ? 8 : 0);
+  const bool warp = K <= 32 * 32, wide = K > 32 * kMaxT, longer = K > kMaxRow || (wide && mode != kVec);
   // The smallest block that holds the row; with few rows, one that gives every
   // thread as few values as it can.
-  int T = 128;
   const int per = p.M <= 148 ? 8 : 32;
-  while (!warp && T < kMaxT && T * per < p.K) T *= 2;
+  int T = std::min(kMaxT, std::max(128, (K + 32 * per - 1) / (32 * per) * 32));
+  if (warp) T = 128;
   if (longer) T = 1024;
+  p.ahead = static_cast<int>(std::max<int64_t>(148, kAheadBytes / (p.K * (RES ? 4 : 2) + 1)));
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(warp ? (p.M + 3) / 4 : p.M), 1, 1);
+  cfg.gridDim = dim3(static_cast<unsigned>(warp && !longer ? (p.M + 3) / 4 : p.M), 1, 1);
   cfg.blockDim = dim3(static_cast<unsigned>(T), 1, 1);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
@@ -352,11 +460,20 @@ cudaError_t launch_rows(const RowsParams& p, bool vec, cudaStream_t s) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  void (*kernel)(const RowsParams) =
-      longer ? k_int8_rows_long<KIND, RES>
-      : wide ? k_int8_rows<KIND, RES, true, false, 64>
-      : warp ? (vec ? k_int8_rows<KIND, RES, true, true, 32> : k_int8_rows<KIND, RES, kV, true, 32>)
-             : (vec ? k_int8_rows<KIND, RES, true, false, 32> : k_int8_rows<KIND, RES, kV, false, 32>);
+  constexpr Mode kA = KIND == kInt8RowsHidden ? kVec : kScalar, kB = KIND == kInt8RowsHidden ? kVec : kShift;
+  void (*kernel)(const RowsParams) = nullptr;
+  if (longer)
+    kernel = k_int8_rows_long<KIND, RES>;
+  else if (wide)
+    kernel = k_int8_rows<KIND, RES, kVec, false, 64>;
+  else if (warp)
+    kernel = mode == kVec     ? k_int8_rows<KIND, RES, kVec, true, 32>
+             : mode == kShift ? k_int8_rows<KIND, RES, kB, true, 32>
+                              : k_int8_rows<KIND, RES, kA, true, 32>;
+  else
+    kernel = mode == kVec     ? k_int8_rows<KIND, RES, kVec, false, 32>
+             : mode == kShift ? k_int8_rows<KIND, RES, kB, false, 32>
+                              : k_int8_rows<KIND, RES, kA, false, 32>;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
   return e == cudaSuccess ? cudaGetLastError() : e;
 }
@@ -413,12 +530,23 @@ int run_int8_rows(const Int8Rows& r, cudaStream_t stream, std::string* err) {
   const bool norm = r.kind == kInt8RowsNorm, res = norm && r.residual;
   // One row alone has no stride to keep aligned.
   auto rows_ok = [&](const void* b, int64_t ld) { return al(b, 16) && (ld % 8 == 0 || r.M == 1); };
-  const bool vec = rows_ok(r.x, r.ldx) && al(r.q, 8) && (r.ldq % 8 == 0 || r.M == 1) && (!norm || al(r.gamma, 16)) &&
-                   (!res || (rows_ok(r.residual, r.ldr) && rows_ok(r.sum, r.lds)));
-  const cudaError_t e = r.kind == kInt8RowsHidden ? launch_rows<kInt8RowsHidden, false>(p, vec, stream)
-                        : !norm                   ? launch_rows<kInt8RowsQuant, false>(p, vec, stream)
-                        : res                     ? launch_rows<kInt8RowsNorm, true>(p, vec, stream)
-                                                  : launch_rows<kInt8RowsNorm, false>(p, vec, stream);
+  auto same_place = [&](const void* b, int64_t ld) {
+    return ((reinterpret_cast<uintptr_t>(b) ^ reinterpret_cast<uintptr_t>(r.x)) & 15u) == 0 &&
+           ((ld - r.ldx) % 8 == 0 || r.M == 1);
+  };
+  Mode mode = kScalar;
+  if (al(r.q, 8) && (r.ldq % 8 == 0 || r.M == 1) && (!norm || al(r.gamma, 16))) {
+    if (rows_ok(r.x, r.ldx) && (!res || (rows_ok(r.residual, r.ldr) && rows_ok(r.sum, r.lds))))
+      mode = kVec;
+    else if (!res || (same_place(r.residual, r.ldr) && same_place(r.sum, r.lds)))
+      mode = kShift;
+  }
+  p.span_x = (r.M - 1) * r.ldx + r.K;
+  p.span_r = (r.M - 1) * r.ldr + r.K;
+  const cudaError_t e = r.kind == kInt8RowsHidden ? launch_rows<kInt8RowsHidden, false>(p, mode, stream)
+                        : !norm                   ? launch_rows<kInt8RowsQuant, false>(p, mode, stream)
+                        : res                     ? launch_rows<kInt8RowsNorm, true>(p, mode, stream)
+                                                  : launch_rows<kInt8RowsNorm, false>(p, mode, stream);
   if (e != cudaSuccess) {
     *err = std::string("int8 rows launch: ") + cudaGetErrorString(e);
     return -3;
