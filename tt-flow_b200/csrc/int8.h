@@ -58,6 +58,7 @@ struct Int8Gemm {
   // b_scale (it is this library's own staging launch), so their first tiles may
   // be requested before it has completed.
   bool b_stable = false;
+  bool a_stable = false;  // nor A (a bare product behind the clear of its counters)
   // Few rows only: the weights [next_n, next_k] of the product that follows on
   // the stream, the first of which are brought into L2 while this one drains.
   const int8_t* next_b = nullptr;

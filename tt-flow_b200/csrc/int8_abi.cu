@@ -236,7 +236,7 @@ int tfb200_matmul_int8(const tfb200_mat* a, const float* a_scale, const tfb200_m
     if (clear) {
       const int rc = run_int8_clear(workspace, clear, s, &err);
       if (rc) return fail(rc, fn, err);
-      g.b_stable = true;  // the clear touches only the workspace
+      g.a_stable = g.b_stable = true;  // the clear touches only the workspace
     }
     const int rc = run_int8_gemm(g, s, &err);
     return rc ? fail(rc, fn, err) : static_cast<int>(TFB200_OK);

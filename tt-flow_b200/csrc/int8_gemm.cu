@@ -130,7 +130,7 @@ static_assert(kPairSmem <= 227 * 1024, "shared memory of one CTA");
 struct PairParams {
   Int8Epi e;
   int fast;  // the residual and C are laid out in 16-byte steps; C is stored with TMA
-  int b_prefetch;
+  int b_prefetch, a_early;
   sched::PairSched ps;
   int32_t* slots;
   int* flags;
@@ -238,7 +238,8 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
       uint32_t phase = 0;
       bool ok = true;
       // The first stages of B, if the preceding kernel does not write it, are
-      // requested while that kernel finishes; A follows after the wait.
+      // requested while that kernel finishes; A follows after the wait, unless
+      // that kernel does not write it either.
       int npre = 0;
       if (p.b_prefetch && nwork > 0) {
         const Work w = item_at(ps, pair, 0);
@@ -252,7 +253,7 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
                            tn * kBN + static_cast<int>(rank) * kBM);
         }
       }
-      grid_dep_wait();
+      if (!p.a_early) grid_dep_wait();
       for (int i = 0; i < nwork && ok; ++i) {
         const Work w = item_at(ps, pair, i);
         int tm, tn;
@@ -670,6 +671,7 @@ int launch_pair(const Int8Gemm& g, cudaStream_t s, std::string* err) {
   const int esz = g.out == kInt8OutF32 ? 4 : 2;
   p.fast = al(g.C, 16) && g.ldc * esz % 16 == 0 && (!g.residual || p.e.vec_res);
   p.b_prefetch = g.b_stable;
+  p.a_early = g.a_stable;
   CUtensorMap ta{}, tb{}, tc{};
   if (!int8_map(&ta, g.A, g.M, g.K, g.lda, kBM, err) || !int8_map(&tb, g.B, g.N, g.K, g.ldb, kBM, err)) return -3;
   if (p.fast && !make_map_box(&tc, g.C, g.M, g.N, g.ldc, static_cast<uint32_t>(64 / esz), 32,

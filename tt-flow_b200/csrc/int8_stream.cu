@@ -55,14 +55,17 @@ struct StreamParams {
   uint32_t acc_cols, tmem_cols;
   int32_t* slots;
   int* counters;
-  int b_prefetch;
-  int pf_units, pf_kblocks, pf_total;  // L2 prefetch of the next product's B
+  int b_prefetch, a_early;
+  int pf_units, pf_kblocks, pf_total, pf_grid;  // L2 prefetch of the next product's B
   int* status;
   uint64_t timeout_ns;
 };
 
+__device__ __forceinline__ int64_t unit_start(int c, int units, int grid) {
+  return static_cast<int64_t>(c) * units / grid;
+}
 __device__ __forceinline__ int64_t unit_start(int c, int units) {
-  return static_cast<int64_t>(c) * units / static_cast<int>(gridDim.x);
+  return unit_start(c, units, static_cast<int>(gridDim.x));
 }
 // The CTA whose range holds unit u.
 __device__ __forceinline__ int cta_of(int64_t u, int units) {
@@ -220,7 +223,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tma_load_2d_hint(smem_u32(sB + s * kUnit), &tmB, smem_u32(&ctl->full[s]),
                          static_cast<int>(u % p.kblocks) * kK, static_cast<int>(u / p.kblocks) * kN, evict_first);
       }
-      grid_dep_wait();
+      if (!p.a_early) grid_dep_wait();
       for (int64_t u = u0; u < u1; ++u) {
         const uint32_t fb = smem_u32(&ctl->full[stage]);
         if (u - u0 >= pre) {
@@ -245,11 +248,26 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       if (ok && p.pf_units > 0) {
-        // The first units of the range this CTA streams in the next product.
-        const int64_t n0 = unit_start(blockIdx.x, p.pf_total);
-        const int64_t n1 = min(unit_start(blockIdx.x + 1, p.pf_total), n0 + p.pf_units);
-        for (int64_t u = n0; u < n1; ++u)
-          tma_prefetch_l2_2d(&tmNext, static_cast<int>(u % p.pf_kblocks) * kK, static_cast<int>(u / p.pf_kblocks) * kN);
+        // This CTA's share of the first units of the next product's ranges. The
+        // divisions stay out of the inner loop: the thread holds up the CTA's exit.
+        const int all = p.pf_units * p.pf_grid;
+        int i = static_cast<int>(unit_start(blockIdx.x, all));
+        const int i1 = static_cast<int>(unit_start(blockIdx.x + 1, all));
+        while (i < i1) {
+          const int c = i / p.pf_units, end = min(i1, (c + 1) * p.pf_units);
+          const int first = static_cast<int>(unit_start(c, p.pf_total, p.pf_grid));
+          const int last = static_cast<int>(unit_start(c + 1, p.pf_total, p.pf_grid));
+          const int u = first + (i - c * p.pf_units);
+          int kn = u % p.pf_kblocks, nn = u / p.pf_kblocks;
+          for (int n = min(last - u, end - i); n > 0; --n) {
+            tma_prefetch_l2_2d(&tmNext, kn * kK, nn * kN);
+            if (++kn == p.pf_kblocks) {
+              kn = 0;
+              ++nn;
+            }
+          }
+          i = end;
+        }
       }
       if (!ok) {
         // Let the copies already issued land before shared memory goes away.
@@ -334,13 +352,23 @@ cudaError_t ready() {
 
 int64_t units_of(int64_t n, int64_t k) { return (n + kN - 1) / kN * ((k + kK - 1) / kK); }
 
-int grid_of(int64_t units) {
+// CTAs of a product: one per SM, or up to a quarter fewer when that makes every
+// CTA's range end on a channel block's border or cut it into equal parts, which
+// spares slots, arrivals and finishes (148 CTAs against the number chosen, us:
+// 1 x 4096 x 4096 11.0 / 128 CTAs 9.7; 16 x 4096 x 6144 13.4 / 144 CTAs 12.3;
+// 128 x 8192 x 28672 53.7 / 112 CTAs 49.7; with 96 CTAs the stream itself slows
+// down).
+int grid_of(int64_t n, int64_t k) {
+  const int64_t blocks = (n + kN - 1) / kN, units = units_of(n, k);
   const int most = sm_count() < kMaxGrid ? sm_count() : kMaxGrid;
-  return units < most ? static_cast<int>(units) : most;
+  if (units <= most) return static_cast<int>(units);
+  for (int g = most; g >= most - most / 4; --g)
+    if (blocks % g == 0 || g % blocks == 0) return g;
+  return most;
 }
 
-// Units of the next product's B that each CTA brings into L2 at its end.
-constexpr int kPrefetchUnits = 32;
+// Units of the next product's B that are brought into L2 at the end: 78 MB.
+constexpr int kPrefetchUnits = 4736;
 
 }  // namespace
 
@@ -379,17 +407,18 @@ int run_int8_stream(const Int8Gemm& g, cudaStream_t stream, std::string* err) {
   p.counters = static_cast<int*>(g.ws);
   p.slots = reinterpret_cast<int32_t*>(static_cast<char*>(g.ws) + int8_stream_ws(g.M, g.N).clear_bytes);
   p.b_prefetch = g.b_stable;
-  const int grid = grid_of(units);
+  p.a_early = g.a_stable;
+  const int grid = grid_of(g.N, g.K);
   CUtensorMap tb{}, ta{}, tn{};
   if (!int8_map(&tb, g.B, g.N, g.K, g.ldb, kN, err) ||
       !int8_map(&ta, g.A, g.M, g.K, g.lda, static_cast<uint32_t>(p.mpad), err))
     return -3;
-  // The CTAs' ranges of the next product are known if it gets the same grid.
   const int64_t next = g.next_b ? units_of(g.next_n, g.next_k) : 0;
-  if (next > 0 && next <= (int64_t(1) << 30) && grid_of(next) == grid && g.next_ld % 16 == 0 &&
+  if (next > 0 && next <= (int64_t(1) << 30) && g.next_ld % 16 == 0 &&
       (reinterpret_cast<uintptr_t>(g.next_b) & 15u) == 0) {
     if (!int8_map(&tn, g.next_b, g.next_n, g.next_k, g.next_ld, kN, err)) return -3;
-    p.pf_units = kPrefetchUnits;
+    p.pf_grid = grid_of(g.next_n, g.next_k);
+    p.pf_units = kPrefetchUnits / p.pf_grid;
     p.pf_kblocks = static_cast<int>((g.next_k + kK - 1) / kK);
     p.pf_total = static_cast<int>(next);
   } else {
