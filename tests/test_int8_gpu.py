@@ -282,7 +282,9 @@ def aligned(t):
 SHAPES = [(1, 1, 1), (1, 4096, 4096), (1, 130, 127), (2, 5, 300), (17, 129, 128), (31, 1000, 129), (32, 512, 4096),
           (33, 257, 1000), (64, 300, 2049), (65, 520, 384), (100, 100, 50), (128, 384, 1024), (129, 700, 640),
           (200, 64, 16), (255, 513, 4100), (256, 256, 128), (257, 1023, 511), (1000, 517, 333), (1024, 2304, 768),
-          (64, 8192, 512), (40, 96, 16384), (600, 4096, 2048)]
+          (64, 8192, 512), (40, 96, 16384), (600, 4096, 2048),
+          # a long inner dimension: a short last wave of tiles is split over idle CTA pairs
+          (130, 300, 16384), (300, 520, 9000), (1200, 4000, 10001)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
@@ -419,7 +421,8 @@ def mlp64(q, scale, w1, s1, b1, w2, s2, res, gelu):
 
 
 MLPS = [(1, 256, 1024, 256), (7, 100, 333, 50), (32, 512, 2048, 512), (64, 257, 515, 129), (65, 512, 1024, 512),
-        (200, 384, 1000, 384), (1024, 1024, 4096, 1024)]
+        (200, 384, 1000, 384), (1024, 1024, 4096, 1024),
+        (200, 9008, 520, 256)]
 
 
 @pytest.mark.parametrize("m,k,h,n", MLPS)

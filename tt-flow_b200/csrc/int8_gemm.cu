@@ -595,10 +595,13 @@ int64_t pair_tiles(int64_t m, int64_t n) { return (m + 2 * kBM - 1) / (2 * kBM) 
 
 // The schedule over all the pairs of a B200. A last wave of R < 74 tiles is split
 // when that shortens it: each of its tiles keeps k-blocks [0, kc) on one pair, and
-// S parts of the rest go to idle pairs, one each. Times in k-blocks (0.3 us): a
-// part costs kPartCost for writing its sums and the hand-over, and the finishing
-// pair kReadCost per part.
-constexpr int kPartCost = 8, kReadCost = 3;
+// S parts of the rest go to idle pairs, one each. Costs in k-blocks of 0.3 us: a
+// split costs kSplitCost (writing and handing over the sums, clearing the flags)
+// and kReadCost per part, which the finishing pair reads. Measured, us without a
+// split / with 1 / 2 / 3 parts: 256 x 16384 x 4096 42.6 / 34.5 / 31.8 / 32.3,
+// 1200 x 16384 x 4096 79.8 / 72.0 / 67.8 / 66.8, and where it does not pay,
+// 256 x 4096 x 4096 16.1 / 20.2 / 20.9 / 22.6.
+constexpr int kSplitCost = 30, kReadCost = 8;
 sched::PairSched pair_plan(int64_t m, int64_t n, int64_t k) {
   sched::PairSched s;
   s.tiles = static_cast<int>(pair_tiles(m, n));
@@ -610,7 +613,7 @@ sched::PairSched pair_plan(int64_t m, int64_t n, int64_t k) {
     // Equal pieces: kc = ceil(KB / (parts + 1)), the parts share the rest.
     const int kc = (s.kblocks + parts) / (parts + 1);
     if (s.kblocks - kc < parts) break;
-    const int cost = kc + kPartCost + kReadCost * parts;
+    const int cost = kc + kSplitCost + kReadCost * parts;
     if (cost < best) {
       best = cost;
       s.waves = s.tiles / kSmPairs;
