@@ -2,14 +2,14 @@
 // both running along K, int32 sums (exact up to K = 131071), one fp32 scale per
 // token and per channel applied to the finished sum.
 //
-// k_int8_pair: the tensor-core kernel, persistent over 256 x 256 output tiles,
-// one tile per pair of CTAs (tcgen05.mma.cta_group::2.kind::i8, 256 x 256 x 32).
-// Both operands run along k, so a stage is 128 rows of A and 128 rows of B per
-// CTA, 128 k values (128 bytes) each, in the 128-byte swizzle: 32 KiB a stage,
-// six stages. The int32 accumulator is double-buffered in TMEM, so that the
-// epilogue of one tile runs beside the next tile's products. The work schedule
-// (full waves, then a last wave split over idle pairs) is pair_sched.h; the
-// parts of a split tile are int32, so adding them is exact in any order.
+// k_int8_pair: the tensor-core kernel, persistent over 256 x BN output tiles, one
+// tile per pair of CTAs (tcgen05.mma.cta_group::2.kind::i8, 256 x BN x 32). Both
+// operands run along k, so a stage is 128 rows of A and BN / 2 rows of B per CTA,
+// 128 k values (128 bytes) each, in the 128-byte swizzle. The int32 accumulator
+// is double-buffered in TMEM, so that the epilogue of one tile runs beside the
+// next tile's products. BN is 256 where the tiles fill the GPU and 128 or 64
+// where they do not (pair_plan); a short last wave of long tiles is split along k
+// over idle pairs, whose int32 parts are exact in any order.
 // k_int8_gemm_any: operands that TMA cannot describe.
 #include <atomic>
 #include <mutex>
@@ -98,19 +98,24 @@ __global__ void __launch_bounds__(256) k_int8_gemm_any(const int8_t* A, int64_t 
 // ------------------------------------------------------------ CTA-pair kernel
 
 constexpr int kBM = 128;                   // rows of A, and rows of B, per CTA
-constexpr int kBN = 256;                   // columns of a pair's tile
 constexpr int kBK = 128;                   // k values per stage (128 bytes)
-constexpr int kStages = cfg::kPairStages;
-constexpr uint32_t kTileBytes = kBM * kBK;  // one operand's stage: 16 KiB
+constexpr uint32_t kABytes = kBM * kBK;    // A's share of a stage: 16 KiB
 constexpr int kEpiWarps = cfg::kPairEpiWarps;
-constexpr int kChunks = kBN / 32 / (kEpiWarps / 4);  // 32-column chunks per epilogue warp
-constexpr uint32_t kStageOut = 32 * 64;              // one staged block: 32 rows of 64 bytes
-constexpr int kGroup = cfg::kGroupM;                 // row tiles per raster group
-constexpr int kSmPairs = 74;                         // CTA pairs of a B200
+constexpr uint32_t kStageOut = 32 * 64;    // one staged block: 32 rows of 64 bytes
+constexpr int kGroup = cfg::kGroupM;       // row tiles per raster group
+constexpr int kSmPairs = 74;               // CTA pairs of a B200
+constexpr int kMaxBN = 256, kMaxStages = 9;
+
+template <int BN>
+struct Geo {
+  static constexpr uint32_t kBBytes = BN / 2 * kBK;
+  static constexpr int kStages = BN == 256 ? 6 : BN == 128 ? 8 : 9;
+  static constexpr int kChunks = BN / 64;  // 32-column chunks per epilogue warp
+};
 
 struct PairCtl {
-  uint64_t full[kStages];
-  uint64_t empty[kStages];
+  uint64_t full[kMaxStages];
+  uint64_t empty[kMaxStages];
   uint64_t tfull[2];
   uint64_t tempty[2];
   uint64_t drain;
@@ -119,13 +124,17 @@ struct PairCtl {
   // Scales and bias of the tile's columns, for the epilogue. Read from global
   // memory chunk by chunk they cost an L2 round trip each behind the operands'
   // traffic, longer than the products of a 4096-deep tile.
-  alignas(16) float sb[kBN];
-  alignas(16) uint16_t bias[kBN];
+  alignas(16) float sb[kMaxBN];
+  alignas(16) uint16_t bias[kMaxBN];
 };
 
-constexpr size_t kPairSmem =
-    1024 + 2 * kStages * kTileBytes + static_cast<size_t>(kEpiWarps) * 2 * kStageOut + sizeof(PairCtl);
-static_assert(kPairSmem <= 227 * 1024, "shared memory of one CTA");
+template <int BN>
+constexpr size_t pair_smem() {
+  return 1024 + Geo<BN>::kStages * (kABytes + Geo<BN>::kBBytes) + static_cast<size_t>(kEpiWarps) * 2 * kStageOut +
+         sizeof(PairCtl);
+}
+static_assert(pair_smem<256>() <= 227 * 1024 && pair_smem<128>() <= 227 * 1024 && pair_smem<64>() <= 227 * 1024,
+              "shared memory of one CTA");
 
 struct PairParams {
   Int8Epi e;
@@ -182,15 +191,17 @@ __device__ __forceinline__ void stage16(uint32_t buf, int lane, int u, uint32_t 
 __device__ __forceinline__ void half_bar(int half) { asm volatile("bar.sync %0, 128;" ::"r"(half + 1) : "memory"); }
 
 // HIDDEN: C is the hidden block of an MLP (Int8Hidden), else bf16 or fp32.
-template <bool HIDDEN>
+template <bool HIDDEN, int BN>
 __global__ void __launch_bounds__(cfg::kPairThreads, 1)
     k_int8_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                 const __grid_constant__ CUtensorMap tmC, const PairParams p) {
+  constexpr int kStages = Geo<BN>::kStages, kChunks = Geo<BN>::kChunks;
+  constexpr uint32_t kBBytes = Geo<BN>::kBBytes;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint8_t* sA = smem;
-  uint8_t* sB = sA + kStages * kTileBytes;
-  uint8_t* sC = sB + kStages * kTileBytes;
+  uint8_t* sB = sA + kStages * kABytes;
+  uint8_t* sC = sB + kStages * kBBytes;
   PairCtl* ctl = reinterpret_cast<PairCtl*>(sC + kEpiWarps * 2 * kStageOut);
 
   const int warp = threadIdx.x >> 5;
@@ -215,7 +226,7 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
     if (p.fast) tma_prefetch_desc(&tmC);
   }
   if (warp == 2) {
-    tmem_alloc_pair(smem_u32(&ctl->tmem_base), 2 * kBN);
+    tmem_alloc_pair(smem_u32(&ctl->tmem_base), 2 * BN);
     tmem_relinquish_pair();
   }
   tc_fence_before();
@@ -229,7 +240,7 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
   const sched::PairSched& ps = p.ps;
   const int nwork = item_count(ps, pair);
   const int num_m = (p.e.M + 2 * kBM - 1) / (2 * kBM);
-  const int num_n = (p.e.N + kBN - 1) / kBN;
+  const int num_n = (p.e.N + BN - 1) / BN;
 
   if (warp == 0) {
     // ------------------------------------------------ TMA producer (both CTAs)
@@ -248,9 +259,9 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
         npre = min(kStages, w.k1 - w.k0);
         for (int s = 0; s < npre; ++s) {
           const uint32_t fb = mapa_shared(smem_u32(&ctl->full[s]), 0);
-          if (leader) mbar_arrive_expect_tx(smem_u32(&ctl->full[s]), 4 * kTileBytes);
-          tma_load_2d_pair(smem_u32(sB + s * kTileBytes), &tmB, fb, (w.k0 + s) * kBK,
-                           tn * kBN + static_cast<int>(rank) * kBM);
+          if (leader) mbar_arrive_expect_tx(smem_u32(&ctl->full[s]), 2 * (kABytes + kBBytes));
+          tma_load_2d_pair(smem_u32(sB + s * kBBytes), &tmB, fb, (w.k0 + s) * kBK,
+                           tn * BN + static_cast<int>(rank) * (BN / 2));
         }
       }
       if (!p.a_early) grid_dep_wait();
@@ -266,12 +277,12 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
             break;
           }
           const uint32_t fb = mapa_shared(smem_u32(&ctl->full[stage]), 0);
-          if (leader && !pre) mbar_arrive_expect_tx(smem_u32(&ctl->full[stage]), 4 * kTileBytes);
-          tma_load_2d_pair(smem_u32(sA + stage * kTileBytes), &tmA, fb, kb * kBK,
+          if (leader && !pre) mbar_arrive_expect_tx(smem_u32(&ctl->full[stage]), 2 * (kABytes + kBBytes));
+          tma_load_2d_pair(smem_u32(sA + stage * kABytes), &tmA, fb, kb * kBK,
                            tm * 2 * kBM + static_cast<int>(rank) * kBM);
           if (!pre)
-            tma_load_2d_pair(smem_u32(sB + stage * kTileBytes), &tmB, fb, kb * kBK,
-                             tn * kBN + static_cast<int>(rank) * kBM);
+            tma_load_2d_pair(smem_u32(sB + stage * kBBytes), &tmB, fb, kb * kBK,
+                             tn * BN + static_cast<int>(rank) * (BN / 2));
           if (++stage == kStages) {
             stage = 0;
             phase ^= 1u;
@@ -289,7 +300,7 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
   } else if (warp == 1) {
     // --------------------------------------------------- MMA issuer (leader)
     if (lane == 0 && leader) {
-      constexpr uint32_t idesc = idesc_i8(2 * kBM, kBN);
+      constexpr uint32_t idesc = idesc_i8(2 * kBM, BN);
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -303,7 +314,7 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
           break;
         }
         tc_fence_after();
-        const uint32_t d = tmem_base + static_cast<uint32_t>(acc * kBN);
+        const uint32_t d = tmem_base + static_cast<uint32_t>(acc * BN);
         for (int kb = w.k0; kb < w.k1; ++kb) {
           if (!mbar_wait(smem_u32(&ctl->full[stage]), phase, &ctl->abort, p.timeout_ns)) {
             give_up(ctl, p.status);
@@ -311,8 +322,8 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
             break;
           }
           tc_fence_after();
-          const uint32_t a0 = smem_u32(sA + stage * kTileBytes);
-          const uint32_t b0 = smem_u32(sB + stage * kTileBytes);
+          const uint32_t a0 = smem_u32(sA + stage * kABytes);
+          const uint32_t b0 = smem_u32(sB + stage * kBBytes);
 #pragma unroll
           for (int k = 0; k < kBK / 32; ++k)
             mma_i8_pair(d, sdesc_sw128(a0 + k * 32, 16, 1024), sdesc_sw128(b0 + k * 32, 16, 1024), idesc,
@@ -350,21 +361,24 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
       const bool row_in = row < p.e.M;
       const bool part = w.role == sched::kPart, fix = w.role == sched::kMain;
       // While the tile's products run: the row's scale, a column's scale and bias
-      // per thread (four warps share a half's 128 columns), the residual into L2.
+      // per thread (four warps share a half of the columns), the residual into L2.
       float sa = 0.0f;
       if (!part) {
-        const int n = tn * kBN + c0 * 32 + r;
-        const float sb = n < p.e.N ? p.e.b_scale[n] : 0.0f;
-        const uint16_t bias = p.e.bias && n < p.e.N ? reinterpret_cast<const uint16_t*>(p.e.bias)[n] : uint16_t(0);
+        const int n = tn * BN + c0 * 32 + r;
+        const bool col_in = r < BN / 2 && n < p.e.N;
+        const float sb = col_in ? p.e.b_scale[n] : 0.0f;
+        const uint16_t bias = p.e.bias && col_in ? reinterpret_cast<const uint16_t*>(p.e.bias)[n] : uint16_t(0);
         if (row_in) {
           sa = p.e.a_scale[row];
           if (!HIDDEN && p.e.residual)
-            for (int c = c0; c < c0 + kChunks && tn * kBN + c * 32 < p.e.N; c += 2)
-              prefetch_l2(p.e.residual + row * p.e.ldr + tn * kBN + c * 32);
+            for (int c = c0; c < c0 + kChunks && tn * BN + c * 32 < p.e.N; c += 2)
+              prefetch_l2(p.e.residual + row * p.e.ldr + tn * BN + c * 32);
         }
         half_bar(ew >> 2);  // the half's warps are done with the last tile's columns
-        ctl->sb[c0 * 32 + r] = sb;
-        ctl->bias[c0 * 32 + r] = bias;
+        if (r < BN / 2) {
+          ctl->sb[c0 * 32 + r] = sb;
+          ctl->bias[c0 * 32 + r] = bias;
+        }
         half_bar(ew >> 2);
       }
       bool ok = mbar_wait(smem_u32(&ctl->tfull[acc]), use & 1u, &ctl->abort, p.timeout_ns);
@@ -376,7 +390,7 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
         continue;
       }
       tc_fence_after();
-      const uint32_t tacc = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * kBN);
+      const uint32_t tacc = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * BN);
       // A split tile's flags: one per part and epilogue warp.
       int* const flag = p.flags + (w.slot * 2 + static_cast<int>(rank)) * kEpiWarps + ew;
       if (fix && row0 < p.e.M) {
@@ -394,11 +408,11 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
       }
       float hmax[kChunks] = {};
       for (int c = c0; c < c0 + kChunks; ++c) {
-        const int col0 = tn * kBN + c * 32;
+        const int col0 = tn * BN + c * 32;
         if (col0 >= p.e.N || row0 >= p.e.M) break;  // warp-uniform: nothing of this block is in the matrix
         // Slots: [chunk][column / 4][row][4], so that a warp's 16-byte accesses
         // cover 512 contiguous bytes.
-        int4* slot = reinterpret_cast<int4*>(p.slots + (static_cast<int64_t>(w.slot) * 2 + rank) * (kBM * kBN)) +
+        int4* slot = reinterpret_cast<int4*>(p.slots + (static_cast<int64_t>(w.slot) * 2 + rank) * (kBM * BN)) +
                      c * 8 * kBM + r;
         uint4 res[4];
         const bool whole = col0 + 32 <= p.e.N;
@@ -423,7 +437,7 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
           for (int j = 0; j < ps.parts; ++j) {
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-              const int4 add = __ldcg(slot + j * (kBM * kBN / 2) + k * kBM);
+              const int4 add = __ldcg(slot + j * (kBM * BN / 2) + k * kBM);
               v[4 * k] += static_cast<uint32_t>(add.x);
               v[4 * k + 1] += static_cast<uint32_t>(add.y);
               v[4 * k + 2] += static_cast<uint32_t>(add.z);
@@ -564,10 +578,16 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
         __syncwarp();
         if (lane == 0) st_release_gpu(flag, 1);
       }
-      // The maxima of this warp's 128 columns.
-      if (HIDDEN && !part && row_in && tn * kBN + c0 * 32 < p.e.N)
-        *reinterpret_cast<float4*>(p.e.hidden_max + row * p.e.ldm + tn * (kBN / kHiddenBlock) + c0) =
-            make_float4(hmax[0], hmax[1], hmax[2], hmax[3]);
+      // The maxima of this warp's columns (a row of them is padded to 128 columns).
+      if (HIDDEN && !part && row_in && tn * BN + c0 * 32 < p.e.N) {
+        float* at = p.e.hidden_max + row * p.e.ldm + tn * (BN / kHiddenBlock) + c0;
+        if constexpr (kChunks == 4)
+          *reinterpret_cast<float4*>(at) = make_float4(hmax[0], hmax[1], hmax[2], hmax[3]);
+        else if constexpr (kChunks == 2)
+          *reinterpret_cast<float2*>(at) = make_float2(hmax[0], hmax[1]);
+        else
+          *at = hmax[0];
+      }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
@@ -585,45 +605,79 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
   cluster_sync();  // no CTA leaves while its peer may still touch its barriers or shared memory
   if (warp == 2) {
     tc_fence_after();
-    tmem_dealloc_pair(tmem_base, 2 * kBN);
+    tmem_dealloc_pair(tmem_base, 2 * BN);
   }
 }
 
 bool al(const void* p, unsigned b) { return (reinterpret_cast<uintptr_t>(p) & (b - 1)) == 0; }
 
-int64_t pair_tiles(int64_t m, int64_t n) { return (m + 2 * kBM - 1) / (2 * kBM) * ((n + kBN - 1) / kBN); }
+int64_t pair_tiles(int64_t m, int64_t n, int bn) { return (m + 2 * kBM - 1) / (2 * kBM) * ((n + bn - 1) / bn); }
 
-// The schedule over all the pairs of a B200. A last wave of R < 74 tiles is split
-// when that shortens it: each of its tiles keeps k-blocks [0, kc) on one pair, and
-// S parts of the rest go to idle pairs, one each. Costs in k-blocks of 0.3 us: a
-// split costs kSplitCost (writing and handing over the sums, clearing the flags)
-// and kReadCost per part, which the finishing pair reads. Measured, us without a
-// split / with 1 / 2 / 3 parts: 256 x 16384 x 4096 42.6 / 34.5 / 31.8 / 32.3,
-// 1200 x 16384 x 4096 79.8 / 72.0 / 67.8 / 66.8, and where it does not pay,
-// 256 x 4096 x 4096 16.1 / 20.2 / 20.9 / 22.6.
-constexpr int kSplitCost = 30, kReadCost = 8;
-sched::PairSched pair_plan(int64_t m, int64_t n, int64_t k) {
+struct PairPlan {
+  int bn = kMaxBN;
   sched::PairSched s;
-  s.tiles = static_cast<int>(pair_tiles(m, n));
-  s.kblocks = static_cast<int>((k + kBK - 1) / kBK);
-  s.pairs = kSmPairs;
-  const int rem = s.tiles % kSmPairs, idle = kSmPairs - rem;
-  int best = s.kblocks;
-  for (int parts = 1; rem > 0 && parts <= sched::kMaxParts && rem * parts <= idle; ++parts) {
-    // Equal pieces: kc = ceil(KB / (parts + 1)), the parts share the rest.
-    const int kc = (s.kblocks + parts) / (parts + 1);
-    if (s.kblocks - kc < parts) break;
-    const int cost = kc + kSplitCost + kReadCost * parts;
-    if (cost < best) {
-      best = cost;
-      s.waves = s.tiles / kSmPairs;
-      s.rem = rem;
-      s.parts = parts;
-      s.kc = kc;
+};
+
+// The tile width and schedule over all the pairs of a B200, by an estimate in
+// k-blocks of a 256-wide tile (0.3 us). A narrower tile's k-block is hardly
+// shorter (A's share of a stage stays, and comes out of L2 for every pair), but
+// its epilogue is, so narrow tiles pay where the wide ones leave pairs idle in a
+// single short wave; measured, us with 256 / 128 / 64 columns: 256 x 4096 x 4096
+// 16.2 / 14.6 / 13.9, 512 x 4096 x 4096 16.5 / 15.5 / 22.5, 200 x 512 x 2048 7.3 /
+// 5.7 / 4.8, 1024 x 4096 x 4096 17.7 / 24.8 / 40.0.
+// A last wave of R < 74 wide tiles is split when that shortens it: each of its
+// tiles keeps k-blocks [0, kc) on one pair, and S parts of the rest go to idle
+// pairs, one each. A split costs kSplitCost (writing and handing over the sums,
+// clearing the flags) and kReadCost per part, which the finishing pair reads.
+// Measured, us without a split / with 1 / 2 / 3 parts: 256 x 16384 x 4096 42.6 /
+// 34.5 / 31.8 / 32.3, 1200 x 16384 x 4096 79.8 / 72.0 / 67.8 / 66.8, and where it
+// does not pay, 256 x 4096 x 4096 16.1 / 20.2 / 20.9 / 22.6.
+constexpr int kSplitCost = 30, kReadCost = 8;
+PairPlan pair_plan(int64_t m, int64_t n, int64_t k) {
+  const int kb = static_cast<int>((k + kBK - 1) / kBK);
+  PairPlan best;
+  double best_cost = 0.0;
+  for (const int bn : {256, 128, 64}) {
+    const int64_t tiles = pair_tiles(m, n, bn);
+    if (bn < kMaxBN && tiles > 4 * kSmPairs) break;
+    const double block = bn == 256 ? 1.0 : bn == 128 ? 0.96 : 0.92, fixed = bn == 256 ? 10.0 : bn == 128 ? 6.0 : 4.0;
+    const double cost = static_cast<double>((tiles + kSmPairs - 1) / kSmPairs) * kb * block + fixed;
+    if (bn == kMaxBN || cost < best_cost) {
+      best_cost = cost;
+      best.bn = bn;
+      best.s = sched::PairSched();
+      best.s.tiles = static_cast<int>(tiles);
+      best.s.kblocks = kb;
+      best.s.pairs = kSmPairs;
+    }
+    if (bn < kMaxBN) continue;
+    const int rem = best.s.tiles % kSmPairs, idle = kSmPairs - rem;
+    for (int parts = 1; rem > 0 && parts <= sched::kMaxParts && rem * parts <= idle; ++parts) {
+      // Equal pieces: kc = ceil(KB / (parts + 1)), the parts share the rest.
+      const int kc = (kb + parts) / (parts + 1);
+      if (kb - kc < parts) break;
+      const double split = static_cast<double>(best.s.tiles / kSmPairs) * kb + kc + kSplitCost + kReadCost * parts + fixed;
+      if (split < best_cost) {
+        best_cost = split;
+        best.s.waves = best.s.tiles / kSmPairs;
+        best.s.rem = rem;
+        best.s.parts = parts;
+        best.s.kc = kc;
+      }
     }
   }
-  return s;
+  return best;
 }
+
+using PairKernel = void (*)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const PairParams);
+template <int BN>
+PairKernel pair_kernel(bool hidden) {
+  return hidden ? k_int8_pair<true, BN> : k_int8_pair<false, BN>;
+}
+PairKernel pair_kernel(bool hidden, int bn) {
+  return bn == 256 ? pair_kernel<256>(hidden) : bn == 128 ? pair_kernel<128>(hidden) : pair_kernel<64>(hidden);
+}
+size_t pair_smem(int bn) { return bn == 256 ? pair_smem<256>() : bn == 128 ? pair_smem<128>() : pair_smem<64>(); }
 
 // Per-device set-up of the first call; calls may come from several host
 // threads. *pairs: how many pairs are resident at once.
@@ -637,21 +691,23 @@ cudaError_t pair_ready(int* pairs) {
   *pairs = resident[dev].load(std::memory_order_acquire);
   if (*pairs > 0) return cudaSuccess;
   std::lock_guard<std::mutex> lock(mu);
-  e = cudaFuncSetAttribute(k_int8_pair<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kPairSmem));
-  if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(k_int8_pair<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kPairSmem));
-  if (e != cudaSuccess) return e;
+  for (const int bn : {64, 128, 256})
+    for (const bool hidden : {false, true}) {
+      e = cudaFuncSetAttribute(pair_kernel(hidden, bn), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               static_cast<int>(pair_smem(bn)));
+      if (e != cudaSuccess) return e;
+    }
   cudaLaunchConfig_t q{};
   q.gridDim = dim3(static_cast<unsigned>(sm_count()), 1, 1);
   q.blockDim = dim3(cfg::kPairThreads, 1, 1);
-  q.dynamicSmemBytes = kPairSmem;
+  q.dynamicSmemBytes = pair_smem(kMaxBN);  // one CTA per SM in every form
   cudaLaunchAttribute a[1];
   a[0].id = cudaLaunchAttributeClusterDimension;
   a[0].val.clusterDim = {2, 1, 1};
   q.attrs = a;
   q.numAttrs = 1;
   int n = 0;
-  e = cudaOccupancyMaxActiveClusters(&n, k_int8_pair<false>, &q);
+  e = cudaOccupancyMaxActiveClusters(&n, pair_kernel(false, kMaxBN), &q);
   if (e == cudaSuccess && n <= 0) e = cudaErrorLaunchOutOfResources;
   if (e != cudaSuccess) return e;
   resident[dev].store(n, std::memory_order_release);
@@ -675,8 +731,10 @@ int launch_pair(const Int8Gemm& g, cudaStream_t s, std::string* err) {
   p.fast = al(g.C, 16) && g.ldc * esz % 16 == 0 && (!g.residual || p.e.vec_res);
   p.b_prefetch = g.b_stable;
   p.a_early = g.a_stable;
+  const PairPlan plan = pair_plan(g.M, g.N, g.K);
   CUtensorMap ta{}, tb{}, tc{};
-  if (!int8_map(&ta, g.A, g.M, g.K, g.lda, kBM, err) || !int8_map(&tb, g.B, g.N, g.K, g.ldb, kBM, err)) return -3;
+  if (!int8_map(&ta, g.A, g.M, g.K, g.lda, kBM, err) || !int8_map(&tb, g.B, g.N, g.K, g.ldb, static_cast<uint32_t>(plan.bn / 2), err))
+    return -3;
   if (p.fast && !make_map_box(&tc, g.C, g.M, g.N, g.ldc, static_cast<uint32_t>(64 / esz), 32,
                                    CU_TENSOR_MAP_SWIZZLE_64B, err,
                                    g.out == kInt8OutF32      ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
@@ -684,7 +742,7 @@ int launch_pair(const Int8Gemm& g, cudaStream_t s, std::string* err) {
                                                              : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
                                    esz))
     return -3;
-  p.ps = pair_plan(g.M, g.N, g.K);
+  p.ps = plan.s;
   if (p.ps.rem > 0 && resident >= kSmPairs) {
     p.flags = static_cast<int*>(g.ws);
     p.slots = reinterpret_cast<int32_t*>(static_cast<char*>(g.ws) + int8_gemm_ws(g.M, g.N, g.K).clear_bytes);
@@ -694,7 +752,7 @@ int launch_pair(const Int8Gemm& g, cudaStream_t s, std::string* err) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(2 * p.ps.pairs), 1, 1);
   cfg.blockDim = dim3(cfg::kPairThreads, 1, 1);
-  cfg.dynamicSmemBytes = kPairSmem;
+  cfg.dynamicSmemBytes = pair_smem(plan.bn);
   cfg.stream = s;
   cudaLaunchAttribute a[2];
   a[0].id = cudaLaunchAttributeClusterDimension;
@@ -703,7 +761,7 @@ int launch_pair(const Int8Gemm& g, cudaStream_t s, std::string* err) {
   a[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = a;
   cfg.numAttrs = 2;
-  e = cudaLaunchKernelEx(&cfg, g.out == kInt8OutHidden ? k_int8_pair<true> : k_int8_pair<false>, ta, tb, tc, p);
+  e = cudaLaunchKernelEx(&cfg, pair_kernel(g.out == kInt8OutHidden, plan.bn), ta, tb, tc, p);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) {
     *err = std::string("int8 pair gemm launch: ") + cudaGetErrorString(e);
@@ -724,8 +782,8 @@ bool int8_map(CUtensorMap* m, const int8_t* base, int64_t rows, int64_t cols, in
 Int8GemmWs int8_gemm_ws(int64_t m, int64_t n, int64_t k) {
   Int8GemmWs w;
   if (k > 0 && m <= kInt8StreamRows) return int8_stream_ws(m, n);
-  if (k <= 0 || pair_tiles(m, n) > (1 << 30)) return w;
-  const sched::PairSched ps = pair_plan(m, n, k);
+  if (k <= 0 || pair_tiles(m, n, kMaxBN) > (1 << 30)) return w;
+  const sched::PairSched ps = pair_plan(m, n, k).s;
   if (ps.rem > 0) {
     w.clear_bytes = (static_cast<size_t>(ps.rem) * ps.parts * 2 * kEpiWarps * sizeof(int) + 255) / 256 * 256;
     w.total = w.clear_bytes + static_cast<size_t>(ps.rem) * ps.parts * sched::kSlotBytes;
@@ -741,7 +799,7 @@ int run_int8_gemm(const Int8Gemm& g, cudaStream_t stream, std::string* err) {
   // TMA describes operands that start on 16-byte boundaries with row strides
   // that are multiples of 16 bytes (one row has no stride).
   if (g.K > 0 && al(g.A, 16) && al(g.B, 16) && (g.lda % 16 == 0 || g.M == 1) && (g.ldb % 16 == 0 || g.N == 1) &&
-      pair_tiles(g.M, g.N) <= (1 << 30))
+      pair_tiles(g.M, g.N, kMaxBN) <= (1 << 30))
     return g.M <= kInt8StreamRows ? run_int8_stream(g, stream, err) : launch_pair(g, stream, err);
   const int64_t by = (g.N + kAnyTile - 1) / kAnyTile;
   const dim3 grid(static_cast<unsigned>((g.M + kAnyTile - 1) / kAnyTile), static_cast<unsigned>(by < 65535 ? by : 65535));
