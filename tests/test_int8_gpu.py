@@ -288,15 +288,66 @@ SHAPES = [(1, 1, 1), (1, 4096, 4096), (1, 130, 127), (2, 5, 300), (17, 129, 128)
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
-@pytest.mark.parametrize("align", [True, False])
-def test_matmul(ops, m, n, k, align):
+def test_matmul(ops, m, n, k):
     a, sa, b, sb, bias, res = operands(m + 7 * n + 13 * k, m, n, k)
-    if align:
-        a, b = aligned(a), aligned(b)
+    a, b = aligned(a), aligned(b)
     check(ops.matmul_int8(a, sa, b, sb), product64(a, sa, b, sb))
     check(ops.matmul_int8(a, sa, b, sb, bias=bias, gelu="tanh"), product64(a, sa, b, sb, bias, "tanh"))
     check(ops.matmul_int8(a, sa, b, sb, bias=bias, residual=res, out_dtype=torch.float32),
           product64(a, sa, b, sb, bias, None, res, torch.float32))
+    # Over the residual: an element is read before it is written.
+    check(ops.matmul_int8(a, sa, b, sb, residual=res, out=res.clone()), product64(a, sa, b, sb, None, None, res))
+    y = res.clone()
+    check(ops.matmul_int8(a, sa, b, sb, residual=y, out=y), product64(a, sa, b, sb, None, None, res))
+
+
+def c_call(ops, fn, *args):
+    """A C entry point on operands as they are laid out (the Python functions copy unaligned int8 ones)."""
+    from tfb200 import _lib as L
+
+    ops._call(torch.device("cuda", torch.cuda.current_device()), getattr(L.lib(), fn), *args)
+
+
+@pytest.mark.parametrize("m,n,k", SHAPES[:-3])
+@pytest.mark.parametrize("off_a,pad_a,off_b,pad_b", [(1, 0, 0, 3), (16, 16, 5, 0), (0, 1, 16, 16)])
+def test_matmul_unaligned(ops, m, n, k, off_a, pad_a, off_b, pad_b):
+    import ctypes
+
+    a, sa, b, sb, bias, res = operands(m + 7 * n + 13 * k, m, n, k)
+    av, _ = rows_at(a, off_a, k + pad_a)
+    bv, _ = rows_at(b, off_b, k + pad_b)
+    y = torch.empty(m, n, dtype=torch.bfloat16, device="cuda")
+    need = ops.matmul_int8_workspace_bytes(m, k, n)
+    ws = torch.empty(max(need, 1), dtype=torch.uint8, device="cuda")
+    mats = [ops._rows(t, "t", t.dtype)[2] for t in (av, bv, res, y)]
+    ra, rb, rr, ry = (ctypes.byref(x) for x in mats)
+    assert mats[0].data == av.data_ptr() and mats[1].data == bv.data_ptr()
+    c_call(ops, "tfb200_matmul_int8", ra, sa.data_ptr(), rb, sb.data_ptr(), bias.data_ptr(), 1, rr, ry, ops._call,
+           ws.data_ptr(), need)
+    check(y, product64(a, sa, b, sb, bias, "tanh", res))
+    # The same bits as on aligned operands.
+    assert torch.equal(y, ops.matmul_int8(av, sa, bv, sb, bias=bias, gelu="tanh", residual=res))
+
+
+@pytest.mark.parametrize("m,k,h,n", [(3, 50, 333, 20), (70, 100, 70, 64), (300, 129, 515, 130)])
+def test_mlp_unaligned(ops, m, k, h, n):
+    import ctypes
+
+    g = gen(k)
+    x, gamma = normal(g, m, k).bfloat16(), torch.ones(k, dtype=torch.bfloat16, device="cuda")
+    w1, s1 = weight(ops, g, h, k)
+    w2, s2 = weight(ops, g, n, h)
+    res = normal(g, m, n).bfloat16()
+    w1v, _ = rows_at(w1, 3, k + 1)
+    w2v, _ = rows_at(w2, 1, h)
+    y = torch.empty(m, n, dtype=torch.bfloat16, device="cuda")
+    need = ops.mlp_int8_workspace_bytes(m, k, h, n)
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    mats = [ops._rows(t, "t", t.dtype)[2] for t in (x, w1v, w2v, res, y)]
+    rx, r1, r2, rr, ry = (ctypes.byref(t) for t in mats)
+    c_call(ops, "tfb200_fused_mlp_int8", rx, gamma.data_ptr(), r1, s1.data_ptr(), None, r2, s2.data_ptr(), rr, EPS, 1,
+           ry, ops._call, ws.data_ptr(), need)
+    assert torch.equal(y, ops.fused_mlp_int8(x, gamma, w1, s1, None, w2, s2, res, EPS, gelu="tanh"))
 
 
 @pytest.mark.parametrize("m,n,k", [(1, 300, 256), (48, 200, 129), (150, 333, 400), (300, 512, 1024)])
@@ -343,9 +394,8 @@ def test_matmul_extremes(ops, m):
     b = torch.full((n, k), -128, dtype=torch.int8, device="cuda")
     b[1::2] = 127
     sa, sb = torch.full((m,), 2.0 ** -20, device="cuda"), torch.ones(n, device="cuda")
-    for a_, b_ in ((a, b), (aligned(a), aligned(b))):
-        y = ops.matmul_int8(a_, sa, b_, sb, out_dtype=torch.float32)
-        check(y, product64(a, sa, b, sb, dtype=torch.float32))
+    y = ops.matmul_int8(a, sa, b, sb, out_dtype=torch.float32)
+    check(y, product64(a, sa, b, sb, dtype=torch.float32))
     # NaN and infinite scales stay in their rows and columns.
     a, sa, b, sb, bias, res = operands(m, m, 300, 512)
     sa[0], sb[5], sb[299] = float("nan"), float("inf"), float("nan")

@@ -450,7 +450,7 @@ cudaError_t launch_rows(RowsParams p, Mode mode, cudaStream_t s) {
   int T = std::min(kMaxT, std::max(128, (K + 32 * per - 1) / (32 * per) * 32));
   if (warp) T = 128;
   if (longer) T = 1024;
-  p.ahead = static_cast<int>(std::max<int64_t>(148, kAheadBytes / (p.K * (RES ? 4 : 2) + 1)));
+  p.ahead = static_cast<int>(std::max<int64_t>(148, kAheadBytes / (static_cast<int64_t>(p.K) * (RES ? 4 : 2) + 1)));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(warp && !longer ? (p.M + 3) / 4 : p.M), 1, 1);
   cfg.blockDim = dim3(static_cast<unsigned>(T), 1, 1);

@@ -294,6 +294,17 @@ def _rows(t: torch.Tensor, name: str, dtype: torch.dtype, dev: torch.device | No
     return rows, cols, L.Mat(t.data_ptr(), rows, cols, ld if rows > 1 and ld > 0 else max(cols, 1), _DTYPES[dtype]), t
 
 
+def _rows_int8(t: torch.Tensor, name: str, dev: torch.device | None = None, two_d: bool = False):
+    """``_rows`` of a product's int8 operand. The tensor cores' copies need rows on 16-byte boundaries; an operand laid
+    out otherwise is copied so, which takes a fraction of the time the product would take on it as it is."""
+    r = _rows(t, name, torch.int8, dev, two_d)
+    rows, cols, mat, t = r
+    if rows and cols and ((mat.data & 15) or (rows > 1 and mat.ld & 15)):
+        q, r = _new_int8((rows, cols), rows, t.device)
+        q.copy_(t)
+    return r
+
+
 def _out(t: torch.Tensor, name: str, dtype: torch.dtype, shape, dev: torch.device):
     """``_rows`` of a caller's output, which is written in place: nothing is copied."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != dtype or t.device != dev:
@@ -377,8 +388,8 @@ def quantize_int8(x: torch.Tensor, out: tuple | None = None) -> tuple[torch.Tens
     leading dimensions, ``amax`` the largest magnitude of each row (last dimension), halves to even.
 
     A weight ``w [in, out]`` is laid out for the products once: ``w_q, w_scale = quantize_int8(w.t())``. The rows of
-    a returned ``q`` start 16 bytes apart or a multiple of it (its row stride may exceed its width); the products
-    accept other strides but run slower on them. ``out = (q, scale)`` takes the results in place.
+    a returned ``q`` start 16 bytes apart or a multiple of it (its row stride may exceed its width); the products copy
+    an operand laid out otherwise on every call. ``out = (q, scale)`` takes the results in place.
     """
     xr = _rows(x, "x", torch.bfloat16)
     rows, dev = xr[0], x.device
@@ -447,9 +458,9 @@ def matmul_int8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale
     per row of each; exact integer sums, the rest in fp32, rounded once to ``out_dtype`` (bf16 or fp32). ``bias`` is
     bf16 ``[N]``, ``gelu`` "erf", "tanh" or None, ``residual`` bf16 ``[..., N]``. K is at most 131071.
     """
-    ar = _rows(a, "a", torch.int8)
+    ar = _rows_int8(a, "a")
     M, K, dev = ar[0], ar[1], a.device
-    br = _rows(b, "b", torch.int8, dev, True)
+    br = _rows_int8(b, "b", dev, True)
     N = br[0]
     if br[1] != K:
         raise ValueError(f"matmul_int8: a has K={K} but b has {br[1]} columns")
@@ -484,7 +495,7 @@ def fused_rmsnorm_matmul_int8(x: torch.Tensor, gamma: torch.Tensor, w: torch.Ten
     normalised rows quantised per token (``rmsnorm_int8``, then ``matmul_int8``)."""
     xr = _rows(x, "x", torch.bfloat16)
     M, K, dev = xr[0], xr[1], x.device
-    wr = _rows(w, "w", torch.int8, dev, True)
+    wr = _rows_int8(w, "w", dev, True)
     N = wr[0]
     if wr[1] != K:
         raise ValueError(f"fused_rmsnorm_matmul_int8: x has K={K} but w has {wr[1]} columns")
@@ -510,7 +521,7 @@ def fused_mlp_int8(x: torch.Tensor, gamma: torch.Tensor, w1: torch.Tensor, w1_sc
     block are quantised per token. ``b1`` is a bf16 ``[H]`` bias or None."""
     xr = _rows(x, "x", torch.bfloat16)
     M, K, dev = xr[0], xr[1], x.device
-    w1r, w2r = _rows(w1, "w1", torch.int8, dev, True), _rows(w2, "w2", torch.int8, dev, True)
+    w1r, w2r = _rows_int8(w1, "w1", dev, True), _rows_int8(w2, "w2", dev, True)
     H, N = w1r[0], w2r[0]
     if w1r[1] != K or w2r[1] != H:
         raise ValueError("fused_mlp_int8: shapes do not chain (x[M,K], w1[H,K], w2[N,H])")
