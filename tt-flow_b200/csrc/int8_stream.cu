@@ -357,10 +357,14 @@ int64_t units_of(int64_t n, int64_t k) { return (n + kN - 1) / kN * ((k + kK - 1
 // spares slots, arrivals and finishes (148 CTAs against the number chosen, us:
 // 1 x 4096 x 4096 11.0 / 128 CTAs 9.7; 16 x 4096 x 6144 13.4 / 144 CTAs 12.3;
 // 128 x 8192 x 28672 53.7 / 112 CTAs 49.7; with 96 CTAs the stream itself slows
-// down).
-int grid_of(int64_t n, int64_t k) {
+// down). A block is cut into 8 ranges at most (16 up to 16 rows), because its
+// finisher reads them all (at most 8 / all CTAs, us: 32 x 16384 x 96 13.4 / 37.6,
+// 128 x 8192 x 1024 18.8 / 29.8, 32 x 16384 x 2048 15.2 / 16.3; 1 x 16384 x 96 with
+// at most 16 / 8 / all 10.0 / 11.6 / 16.7).
+int grid_of(int64_t m, int64_t n, int64_t k) {
   const int64_t blocks = (n + kN - 1) / kN, units = units_of(n, k);
-  const int most = sm_count() < kMaxGrid ? sm_count() : kMaxGrid;
+  const int64_t sms = sm_count() < kMaxGrid ? sm_count() : kMaxGrid, cuts = blocks * (m <= 16 ? 16 : 8);
+  const int most = static_cast<int>(sms < cuts ? sms : cuts);
   if (units <= most) return static_cast<int>(units);
   for (int g = most; g >= most - most / 4; --g)
     if (blocks % g == 0 || g % blocks == 0) return g;
@@ -408,7 +412,7 @@ int run_int8_stream(const Int8Gemm& g, cudaStream_t stream, std::string* err) {
   p.slots = reinterpret_cast<int32_t*>(static_cast<char*>(g.ws) + int8_stream_ws(g.M, g.N).clear_bytes);
   p.b_prefetch = g.b_stable;
   p.a_early = g.a_stable;
-  const int grid = grid_of(g.N, g.K);
+  const int grid = grid_of(g.M, g.N, g.K);
   CUtensorMap tb{}, ta{}, tn{};
   if (!int8_map(&tb, g.B, g.N, g.K, g.ldb, kN, err) ||
       !int8_map(&ta, g.A, g.M, g.K, g.lda, static_cast<uint32_t>(p.mpad), err))
@@ -417,7 +421,7 @@ int run_int8_stream(const Int8Gemm& g, cudaStream_t stream, std::string* err) {
   if (next > 0 && next <= (int64_t(1) << 30) && g.next_ld % 16 == 0 &&
       (reinterpret_cast<uintptr_t>(g.next_b) & 15u) == 0) {
     if (!int8_map(&tn, g.next_b, g.next_n, g.next_k, g.next_ld, kN, err)) return -3;
-    p.pf_grid = grid_of(g.next_n, g.next_k);
+    p.pf_grid = grid_of(g.M, g.next_n, g.next_k);
     p.pf_units = kPrefetchUnits / p.pf_grid;
     p.pf_kblocks = static_cast<int>((g.next_k + kK - 1) / kK);
     p.pf_total = static_cast<int>(next);
