@@ -283,6 +283,9 @@ SHAPES = [(1, 1, 1), (1, 4096, 4096), (1, 130, 127), (2, 5, 300), (17, 129, 128)
           (33, 257, 1000), (64, 300, 2049), (65, 520, 384), (100, 100, 50), (128, 384, 1024), (129, 700, 640),
           (200, 64, 16), (255, 513, 4100), (256, 256, 128), (257, 1023, 511), (1000, 517, 333), (1024, 2304, 768),
           (64, 8192, 512), (40, 96, 16384), (600, 4096, 2048),
+          # few rows before large weights: the weight-streaming kernel, with one and many ranges to a channel block
+          (1, 2500, 5000), (2, 130, 20000), (17, 3000, 4100), (33, 4097, 4111), (48, 6144, 2048), (64, 2500, 8200),
+          (65, 3001, 8000), (100, 3000, 9001), (113, 28672, 1024), (128, 2000, 16384),
           # a long inner dimension: a short last wave of tiles is split over idle CTA pairs
           (130, 300, 16384), (300, 520, 9000), (1200, 4000, 10001)]
 
@@ -308,7 +311,7 @@ def c_call(ops, fn, *args):
     ops._call(torch.device("cuda", torch.cuda.current_device()), getattr(L.lib(), fn), *args)
 
 
-@pytest.mark.parametrize("m,n,k", SHAPES[:-3])
+@pytest.mark.parametrize("m,n,k", SHAPES[:-13])
 @pytest.mark.parametrize("off_a,pad_a,off_b,pad_b", [(1, 0, 0, 3), (16, 16, 5, 0), (0, 1, 16, 16)])
 def test_matmul_unaligned(ops, m, n, k, off_a, pad_a, off_b, pad_b):
     import ctypes
@@ -350,7 +353,7 @@ def test_mlp_unaligned(ops, m, k, h, n):
     assert torch.equal(y, ops.fused_mlp_int8(x, gamma, w1, s1, None, w2, s2, res, EPS, gelu="tanh"))
 
 
-@pytest.mark.parametrize("m,n,k", [(1, 300, 256), (48, 200, 129), (150, 333, 400), (300, 512, 1024)])
+@pytest.mark.parametrize("m,n,k", [(1, 300, 256), (48, 200, 129), (37, 2500, 6000), (150, 333, 400), (300, 512, 1024)])
 @pytest.mark.parametrize("gelu", [None, "erf", "tanh"])
 @pytest.mark.parametrize("with_bias", [False, True])
 @pytest.mark.parametrize("with_res", [False, True])
@@ -365,9 +368,8 @@ def test_matmul_epilogues(ops, m, n, k, gelu, with_bias, with_res, dtype):
     check(y, product64(a, sa, b, sb, bias, gelu, res, dtype))
 
 
-@pytest.mark.parametrize("m,n", [(3, 200), (70, 300), (300, 520)])
-def test_matmul_strides_and_surroundings(ops, m, n):
-    k = 272
+@pytest.mark.parametrize("m,n,k", [(3, 200, 272), (70, 300, 272), (300, 520, 272), (19, 2500, 6000)])
+def test_matmul_strides_and_surroundings(ops, m, n, k):
     a, sa, b, sb, bias, res = operands(m, m, n, k)
     want = product64(a, sa, b, sb, bias, None, res)
     first = None
@@ -386,7 +388,7 @@ def test_matmul_strides_and_surroundings(ops, m, n):
         assert (buf == 77).all(), "wrote outside the rows"
 
 
-@pytest.mark.parametrize("m", [1, 40, 100, 300])
+@pytest.mark.parametrize("m", [1, 40, 100, 300])  # 131071 deep: streamed up to 128 rows
 def test_matmul_extremes(ops, m):
     # The longest inner dimension with the largest products: the sums reach 2147467264 of 2147483647.
     k, n = 131071, 20
@@ -472,7 +474,7 @@ def mlp64(q, scale, w1, s1, b1, w2, s2, res, gelu):
 
 MLPS = [(1, 256, 1024, 256), (7, 100, 333, 50), (32, 512, 2048, 512), (64, 257, 515, 129), (65, 512, 1024, 512),
         (200, 384, 1000, 384), (1024, 1024, 4096, 1024),
-        (200, 9008, 520, 256)]
+        (200, 9008, 520, 256), (1, 2100, 9001, 2000), (40, 3000, 8001, 2800), (100, 4096, 8200, 3000)]
 
 
 @pytest.mark.parametrize("m,k,h,n", MLPS)
@@ -541,11 +543,11 @@ def test_mlp_bad_rows_stay_apart(ops):
 # ------------------------------------------------------- streams and graphs
 
 
-@pytest.mark.parametrize("m", [8, 64, 100, 512])
-def test_a_layer_in_a_graph(ops, m):
+@pytest.mark.parametrize("m,d", [(8, 512), (8, 2560), (64, 512), (100, 512), (100, 4096), (512, 512)])
+def test_a_layer_in_a_graph(ops, m, d):
     """norm + QKV, output projection with the residual, MLP block: captured together and replayed with new inputs."""
     g = gen(m)
-    d, h = 512, 1536
+    h = 3 * d
     gamma = (torch.rand(d, generator=g, device="cuda") + 0.5).bfloat16()
     wq, sq = weight(ops, g, 3 * d, d)
     wo, so = weight(ops, g, d, d)
@@ -575,7 +577,7 @@ def test_a_layer_in_a_graph(ops, m):
 
 def test_two_streams_at_once(ops):
     g = gen(9)
-    k, n = 1024, 2048
+    k, n = 4096, 4096
     w, ws = weight(ops, g, n, k)
     gamma = torch.ones(k, dtype=torch.bfloat16, device="cuda")
     xs = {m: normal(g, m, k).bfloat16() for m in (4, 64, 90, 700)}
@@ -611,10 +613,11 @@ def test_weights_written_just_before(ops, m):
 
 def test_workspace_reuse_and_checks(ops):
     g = gen(2)
-    for m in (8, 100, 400):
-        a, sa, b, sb, _, _ = operands(m, m, 1000, 2048)
+    for m, n, k in ((8, 1000, 8192), (100, 3000, 8192), (400, 1000, 2048), (200, 300, 16384)):
+        a, sa, b, sb, _, _ = operands(m, m, n, k)
         a, b = aligned(a), aligned(b)
-        need = ops.matmul_int8_workspace_bytes(m, 2048, 1000)
+        need = ops.matmul_int8_workspace_bytes(m, k, n)
+        assert (need > 0) == (m != 400)
         ws = torch.full((need + 256,), 255, dtype=torch.uint8, device="cuda")  # whatever it held before
         y = ops.matmul_int8(a, sa, b, sb, workspace=ws)
         assert torch.equal(y, ops.matmul_int8(a, sa, b, sb))

@@ -616,6 +616,7 @@ int64_t pair_tiles(int64_t m, int64_t n, int bn) { return (m + 2 * kBM - 1) / (2
 struct PairPlan {
   int bn = kMaxBN;
   sched::PairSched s;
+  double cost = 0.0;  // k-blocks
 };
 
 // The tile width and schedule over all the pairs of a B200, by an estimate in
@@ -636,14 +637,13 @@ constexpr int kSplitCost = 30, kReadCost = 8;
 PairPlan pair_plan(int64_t m, int64_t n, int64_t k) {
   const int kb = static_cast<int>((k + kBK - 1) / kBK);
   PairPlan best;
-  double best_cost = 0.0;
   for (const int bn : {256, 128, 64}) {
     const int64_t tiles = pair_tiles(m, n, bn);
     if (bn < kMaxBN && tiles > 4 * kSmPairs) break;
     const double block = bn == 256 ? 1.0 : bn == 128 ? 0.96 : 0.92, fixed = bn == 256 ? 10.0 : bn == 128 ? 6.0 : 4.0;
     const double cost = static_cast<double>((tiles + kSmPairs - 1) / kSmPairs) * kb * block + fixed;
-    if (bn == kMaxBN || cost < best_cost) {
-      best_cost = cost;
+    if (bn == kMaxBN || cost < best.cost) {
+      best.cost = cost;
       best.bn = bn;
       best.s = sched::PairSched();
       best.s.tiles = static_cast<int>(tiles);
@@ -657,8 +657,8 @@ PairPlan pair_plan(int64_t m, int64_t n, int64_t k) {
       const int kc = (kb + parts) / (parts + 1);
       if (kb - kc < parts) break;
       const double split = static_cast<double>(best.s.tiles / kSmPairs) * kb + kc + kSplitCost + kReadCost * parts + fixed;
-      if (split < best_cost) {
-        best_cost = split;
+      if (split < best.cost) {
+        best.cost = split;
         best.s.waves = best.s.tiles / kSmPairs;
         best.s.rem = rem;
         best.s.parts = parts;
@@ -779,10 +779,24 @@ bool int8_map(CUtensorMap* m, const int8_t* base, int64_t rows, int64_t cols, in
                       CU_TENSOR_MAP_SWIZZLE_128B, err, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1);
 }
 
+// Few rows go to the weight-streaming kernel, unless the whole product is so
+// small that its per-call costs outweigh the weights' stream: by estimates in us,
+//   stream  5.6 + 0.075 per row (slots, arrivals, finish) + weights at 6 TB/s
+//   pair    2.5 + 0.29 per k-block of its plan + weights at 12 TB/s.
+// Measured, us, stream / pair: 2 x 1024 x 1024 6.3 / 5.5, 2 x 4096 x 4096 9.7 /
+// 14.3, 32 x 2048 x 2048 8.8 / 7.8, 32 x 4096 x 4096 11.3 / 13.4, 128 x 1024 x 1024
+// 16.1 / 5.8, 128 x 4096 x 4096 15.7 / 13.6, 128 x 16384 x 4096 23.3 / 30.8,
+// 128 x 8192 x 28672 50.0 / 53.4.
+static bool use_stream(int64_t m, int64_t n, int64_t k) {
+  if (m > kInt8StreamRows) return false;
+  const double mb = static_cast<double>(n) * static_cast<double>(k) * 1e-6;
+  return 5.6 + 0.075 * static_cast<double>(m) + mb / 6.0 <= 2.5 + 0.29 * pair_plan(m, n, k).cost + mb / 12.0;
+}
+
 Int8GemmWs int8_gemm_ws(int64_t m, int64_t n, int64_t k) {
   Int8GemmWs w;
-  if (k > 0 && m <= kInt8StreamRows) return int8_stream_ws(m, n);
   if (k <= 0 || pair_tiles(m, n, kMaxBN) > (1 << 30)) return w;
+  if (use_stream(m, n, k)) return int8_stream_ws(m, n);
   const sched::PairSched ps = pair_plan(m, n, k).s;
   if (ps.rem > 0) {
     w.clear_bytes = (static_cast<size_t>(ps.rem) * ps.parts * 2 * kEpiWarps * sizeof(int) + 255) / 256 * 256;
@@ -800,7 +814,7 @@ int run_int8_gemm(const Int8Gemm& g, cudaStream_t stream, std::string* err) {
   // that are multiples of 16 bytes (one row has no stride).
   if (g.K > 0 && al(g.A, 16) && al(g.B, 16) && (g.lda % 16 == 0 || g.M == 1) && (g.ldb % 16 == 0 || g.N == 1) &&
       pair_tiles(g.M, g.N, kMaxBN) <= (1 << 30))
-    return g.M <= kInt8StreamRows ? run_int8_stream(g, stream, err) : launch_pair(g, stream, err);
+    return use_stream(g.M, g.N, g.K) ? run_int8_stream(g, stream, err) : launch_pair(g, stream, err);
   const int64_t by = (g.N + kAnyTile - 1) / kAnyTile;
   const dim3 grid(static_cast<unsigned>((g.M + kAnyTile - 1) / kAnyTile), static_cast<unsigned>(by < 65535 ? by : 65535));
   k_int8_gemm_any<<<grid, 256, 0, stream>>>(g.A, g.lda, g.B, g.ldb, int8_epi(g));
