@@ -352,12 +352,13 @@ cudaError_t ready() {
 
 int64_t units_of(int64_t n, int64_t k) { return (n + kN - 1) / kN * ((k + kK - 1) / kK); }
 
-// CTAs of a product: one per SM, or up to a quarter fewer when that makes every
-// CTA's range end on a channel block's border or cut it into equal parts, which
-// spares slots, arrivals and finishes (148 CTAs against the number chosen, us:
-// 1 x 4096 x 4096 11.0 / 128 CTAs 9.7; 16 x 4096 x 6144 13.4 / 144 CTAs 12.3;
-// 128 x 8192 x 28672 53.7 / 112 CTAs 49.7; with 96 CTAs the stream itself slows
-// down). A block is cut into 8 ranges at most (16 up to 16 rows), because its
+// CTAs of a product: one per SM, or up to a seventh fewer (a quarter over 64 rows,
+// where slots weigh more) when that makes every CTA's range end on a channel
+// block's border or cut it into equal parts, which spares slots, arrivals and
+// finishes. 148 CTAs against fewer, us: 1 x 4096 x 4096 11.0 / 128 CTAs 9.7;
+// 16 x 4096 x 6144 13.4 / 144 CTAs 12.3; 128 x 8192 x 28672 53.7 / 112 CTAs 49.7;
+// 32 x 8192 x 28672 43.9 / 112 CTAs 44.9; with 96 CTAs the stream itself slows
+// down. A block is cut into 8 ranges at most (16 up to 16 rows), because its
 // finisher reads them all (at most 8 / all CTAs, us: 32 x 16384 x 96 13.4 / 37.6,
 // 128 x 8192 x 1024 18.8 / 29.8, 32 x 16384 x 2048 15.2 / 16.3; 1 x 16384 x 96 with
 // at most 16 / 8 / all 10.0 / 11.6 / 16.7).
@@ -366,7 +367,7 @@ int grid_of(int64_t m, int64_t n, int64_t k) {
   const int64_t sms = sm_count() < kMaxGrid ? sm_count() : kMaxGrid, cuts = blocks * (m <= 16 ? 16 : 8);
   const int most = static_cast<int>(sms < cuts ? sms : cuts);
   if (units <= most) return static_cast<int>(units);
-  for (int g = most; g >= most - most / 4; --g)
+  for (int g = most; g >= most - most / (m <= 64 ? 7 : 4); --g)
     if (blocks % g == 0 || g % blocks == 0) return g;
   return most;
 }
