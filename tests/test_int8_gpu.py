@@ -304,11 +304,15 @@ def test_matmul(ops, m, n, k):
     check(ops.matmul_int8(a, sa, b, sb, residual=y, out=y), product64(a, sa, b, sb, None, None, res))
 
 
+STREAM = object()
+
+
 def c_call(ops, fn, *args):
     """A C entry point on operands as they are laid out (the Python functions copy unaligned int8 ones)."""
     from tfb200 import _lib as L
 
-    ops._call(torch.device("cuda", torch.cuda.current_device()), getattr(L.lib(), fn), *args)
+    stream = torch.cuda.current_stream().cuda_stream
+    ops._call(torch.cuda.current_device(), getattr(L.lib(), fn), *(stream if a is STREAM else a for a in args))
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES[:-13])
@@ -322,10 +326,10 @@ def test_matmul_unaligned(ops, m, n, k, off_a, pad_a, off_b, pad_b):
     y = torch.empty(m, n, dtype=torch.bfloat16, device="cuda")
     need = ops.matmul_int8_workspace_bytes(m, k, n)
     ws = torch.empty(max(need, 1), dtype=torch.uint8, device="cuda")
-    mats = [ops._rows(t, "t", t.dtype)[2] for t in (av, bv, res, y)]
+    mats = [ops._rows(t, "t", t.dtype, t.get_device())[2] for t in (av, bv, res, y)]
     ra, rb, rr, ry = (ctypes.byref(x) for x in mats)
     assert mats[0].data == av.data_ptr() and mats[1].data == bv.data_ptr()
-    c_call(ops, "tfb200_matmul_int8", ra, sa.data_ptr(), rb, sb.data_ptr(), bias.data_ptr(), 1, rr, ry, ops._call,
+    c_call(ops, "tfb200_matmul_int8", ra, sa.data_ptr(), rb, sb.data_ptr(), bias.data_ptr(), 1, rr, ry, STREAM,
            ws.data_ptr(), need)
     check(y, product64(a, sa, b, sb, bias, "tanh", res))
     # The same bits as on aligned operands.
@@ -346,10 +350,10 @@ def test_mlp_unaligned(ops, m, k, h, n):
     y = torch.empty(m, n, dtype=torch.bfloat16, device="cuda")
     need = ops.mlp_int8_workspace_bytes(m, k, h, n)
     ws = torch.empty(need, dtype=torch.uint8, device="cuda")
-    mats = [ops._rows(t, "t", t.dtype)[2] for t in (x, w1v, w2v, res, y)]
+    mats = [ops._rows(t, "t", t.dtype, t.get_device())[2] for t in (x, w1v, w2v, res, y)]
     rx, r1, r2, rr, ry = (ctypes.byref(t) for t in mats)
     c_call(ops, "tfb200_fused_mlp_int8", rx, gamma.data_ptr(), r1, s1.data_ptr(), None, r2, s2.data_ptr(), rr, EPS, 1,
-           ry, ops._call, ws.data_ptr(), need)
+           ry, STREAM, ws.data_ptr(), need)
     assert torch.equal(y, ops.fused_mlp_int8(x, gamma, w1, s1, None, w2, s2, res, EPS, gelu="tanh"))
 
 

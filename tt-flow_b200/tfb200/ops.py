@@ -263,23 +263,33 @@ def residual_add(partial: torch.Tensor, residual: torch.Tensor, out: torch.Tenso
 _GELU_INT8 = {**_GELU, "none": L.TFB200_GELU_NONE, None: L.TFB200_GELU_NONE}
 _DTYPES = {torch.bfloat16: L.TFB200_BF16, torch.float32: L.TFB200_F32, torch.int8: L.TFB200_I8}
 
-# A decode step makes these calls while the GPU waits for them, so each looks at a tensor once: ``_rows`` and ``_out``
-# return the operand's C descriptor beside its shape, and the device and stream are read without building the objects
-# torch.cuda's accessors return (25 us a product with them, 13 us without).
+# A decode step makes these calls while the GPU waits for them, so each looks at a tensor once, through the accessors
+# that build no Python objects: ``_rows`` and ``_out`` return the operand's C descriptor beside its shape, devices are
+# compared by index (25 us of host time a product with torch.cuda's accessors, 11 us without).
+_Tensor = torch.Tensor
+_stream = torch._C._cuda_getCurrentRawStream
+_BF16, _F32, _I8 = torch.bfloat16, torch.float32, torch.int8
 
 
-def _bad(t, name: str, dtype: torch.dtype, dev: torch.device | None):
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+def _bad(t, name: str, dtype: torch.dtype, dev: int):
+    if not isinstance(t, _Tensor) or not t.is_cuda:
         return TypeError(f"{name} must be a CUDA tensor")
     if t.dtype != dtype:
         return TypeError(f"{name} must be {dtype} (got {t.dtype})")
-    return ValueError(f"{name} is on {t.device}; the other operands are on {dev}")
+    return ValueError(f"{name} is on {t.device}; the other operands are on cuda:{dev}")
 
 
-def _rows(t: torch.Tensor, name: str, dtype: torch.dtype, dev: torch.device | None = None, two_d: bool = False):
+def _first(t, name: str) -> int:
+    """The device index of a call's first operand."""
+    if not isinstance(t, _Tensor) or not t.is_cuda:
+        raise TypeError(f"{name} must be a CUDA tensor")
+    return t.get_device()
+
+
+def _rows(t: torch.Tensor, name: str, dtype: torch.dtype, dev: int, two_d: bool = False):
     """(rows, columns, tfb200_mat, tensor) of an operand: leading dimensions flattened, unit column stride, rows that
     do not overlap. A view that is not so is copied; the tensor keeps the memory alive."""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != dtype or (dev is not None and t.device != dev):
+    if not isinstance(t, _Tensor) or t.dtype is not dtype or t.get_device() != dev:
         raise _bad(t, name, dtype, dev)
     n = t.dim()
     if n != 2:
@@ -291,13 +301,13 @@ def _rows(t: torch.Tensor, name: str, dtype: torch.dtype, dev: torch.device | No
     if (unit != 1 and cols > 1) or (ld < cols and rows > 1):
         t = t.contiguous()
         ld = cols
-    return rows, cols, L.Mat(t.data_ptr(), rows, cols, ld if rows > 1 and ld > 0 else max(cols, 1), _DTYPES[dtype]), t
+    return rows, cols, L.Mat(t.data_ptr(), rows, cols, ld if rows > 1 and ld > 0 else cols or 1, _DTYPES[dtype]), t
 
 
-def _rows_int8(t: torch.Tensor, name: str, dev: torch.device | None = None, two_d: bool = False):
+def _rows_int8(t: torch.Tensor, name: str, dev: int, two_d: bool = False):
     """``_rows`` of a product's int8 operand. The tensor cores' copies need rows on 16-byte boundaries; an operand laid
     out otherwise is copied so, which takes a fraction of the time the product would take on it as it is."""
-    r = _rows(t, name, torch.int8, dev, two_d)
+    r = _rows(t, name, _I8, dev, two_d)
     rows, cols, mat, t = r
     if rows and cols and ((mat.data & 15) or (rows > 1 and mat.ld & 15)):
         q, r = _new_int8((rows, cols), rows, t.device)
@@ -305,9 +315,9 @@ def _rows_int8(t: torch.Tensor, name: str, dev: torch.device | None = None, two_
     return r
 
 
-def _out(t: torch.Tensor, name: str, dtype: torch.dtype, shape, dev: torch.device):
+def _out(t: torch.Tensor, name: str, dtype: torch.dtype, shape, dev: int):
     """``_rows`` of a caller's output, which is written in place: nothing is copied."""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != dtype or t.device != dev:
+    if not isinstance(t, _Tensor) or t.dtype != dtype or t.get_device() != dev:
         raise _bad(t, name, dtype, dev)
     if tuple(t.shape) != tuple(shape):
         raise ValueError(f"{name} must be {list(shape)} (got {list(t.shape)})")
@@ -316,45 +326,47 @@ def _out(t: torch.Tensor, name: str, dtype: torch.dtype, shape, dev: torch.devic
             t = t.view(math.prod(shape[:-1]), shape[-1])
         except RuntimeError:
             raise ValueError(f"{name}: the leading dimensions must flatten into rows without a copy") from None
-    r = _rows(t, name, dtype)
+    r = _rows(t, name, dtype, dev)
     if r[3].data_ptr() != t.data_ptr():
         raise ValueError(f"{name} must have unit column stride and rows that do not overlap")
     return r
 
 
-def _out_scale(t: torch.Tensor, n: int, dev: torch.device) -> int:
-    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.float32 or t.device != dev:
-        raise _bad(t, "scale", torch.float32, dev)
+def _out_scale(t: torch.Tensor, n: int, dev: int) -> int:
+    if not isinstance(t, _Tensor) or t.dtype != _F32 or t.get_device() != dev:
+        raise _bad(t, "scale", _F32, dev)
     if t.numel() != n or not t.is_contiguous():
         raise ValueError(f"scale must be contiguous and have {n} elements (got {list(t.shape)})")
     return t.data_ptr()
 
 
-def _vec1(t, n: int, name: str, dtype: torch.dtype, dev: torch.device):
-    """A contiguous vector of n elements (any shape), or None."""
+def _vec1(t, n: int, name: str, dtype: torch.dtype, dev: int):
+    """(address, tensor) of a contiguous vector of n elements (any shape); (None, None) for None."""
     if t is None:
-        return None
-    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != dtype or t.device != dev:
+        return None, None
+    if not isinstance(t, _Tensor) or t.dtype is not dtype or t.get_device() != dev:
         raise _bad(t, name, dtype, dev)
     if t.numel() != n:
         raise ValueError(f"{name} has {t.numel()} elements, expected {n}")
-    return t if t.is_contiguous() else t.reshape(-1).contiguous()
+    if not t.is_contiguous():
+        t = t.reshape(-1).contiguous()
+    return t.data_ptr(), t
 
 
-def _space(need: int, ws: torch.Tensor | None, dev: torch.device):
-    """(tensor, address, bytes) of the workspace of a call that needs `need` bytes."""
-    if ws is None and need == 0:
-        return None, None, 0
-    ws = _workspace(need, ws, dev)
+def _space(need: int, ws: torch.Tensor | None, x: torch.Tensor):
+    """(tensor, address, bytes) of the workspace of a call on x's device that needs `need` bytes."""
+    if ws is None:
+        if need == 0:
+            return None, None, 0
+        ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+        return ws, ws.data_ptr(), need
+    ws = _workspace(need, ws, x.device)
     return ws, ws.data_ptr(), ws.numel() * ws.element_size()
 
 
-def _call(dev: torch.device, fn, *args) -> None:
-    """One C call with ``dev`` current; a ``_call`` among ``args`` stands for dev's current stream."""
-    i = dev.index
-    s = torch._C._cuda_getCurrentRawStream(i)
-    args = [s if a is _call else a for a in args]
-    if torch._C._cuda_getDevice() == i:
+def _call(dev: int, fn, *args) -> None:
+    """One C call with device ``dev`` current."""
+    if torch._C._cuda_getDevice() == dev:
         rc = fn(*args)
     else:
         with torch.cuda.device(dev):
@@ -363,12 +375,11 @@ def _call(dev: torch.device, fn, *args) -> None:
         L.check(rc)
 
 
+_byref = ctypes.byref
+
+
 def _ref(r):
-    return None if r is None else ctypes.byref(r[2])
-
-
-def _ptr(t: torch.Tensor | None):
-    return None if t is None else t.data_ptr()
+    return None if r is None else _byref(r[2])
 
 
 def _new_int8(shape, rows: int, dev):
@@ -376,8 +387,8 @@ def _new_int8(shape, rows: int, dev):
     read best."""
     k = shape[-1]
     ld = (k + 15) // 16 * 16
-    q = torch.empty(rows, ld, dtype=torch.int8, device=dev)
-    mat = L.Mat(q.data_ptr(), rows, k, max(ld, 1), L.TFB200_I8)
+    q = torch.empty(rows, ld, dtype=_I8, device=dev)
+    mat = L.Mat(q.data_ptr(), rows, k, ld or 1, L.TFB200_I8)
     if ld != k:
         q = q[:, :k]
     return (q if len(shape) == 2 else q.unflatten(0, shape[:-1])), (rows, k, mat, q)
@@ -391,16 +402,18 @@ def quantize_int8(x: torch.Tensor, out: tuple | None = None) -> tuple[torch.Tens
     a returned ``q`` start 16 bytes apart or a multiple of it (its row stride may exceed its width); the products copy
     an operand laid out otherwise on every call. ``out = (q, scale)`` takes the results in place.
     """
-    xr = _rows(x, "x", torch.bfloat16)
-    rows, dev = xr[0], x.device
+    dev = _first(x, "x")
+    xr = _rows(x, "x", _BF16, dev)
+    rows = xr[0]
     if out is None:
-        q, qr = _new_int8(x.shape, rows, dev)
-        scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
+        device = x.device
+        q, qr = _new_int8(x.shape, rows, device)
+        scale = torch.empty(x.shape[:-1], dtype=_F32, device=device)
         sp = scale.data_ptr()
     else:
         q, scale = out
-        qr, sp = _out(q, "q", torch.int8, x.shape, dev), _out_scale(scale, rows, dev)
-    _call(dev, L.lib().tfb200_quantize_int8, _ref(xr), _ref(qr), sp, _call)
+        qr, sp = _out(q, "q", _I8, x.shape, dev), _out_scale(scale, rows, dev)
+    _call(dev, L.lib().tfb200_quantize_int8, _byref(xr[2]), _byref(qr[2]), sp, _stream(dev))
     return q, scale
 
 
@@ -410,40 +423,42 @@ def rmsnorm_int8(x: torch.Tensor, gamma: torch.Tensor, eps: float = 1e-6, residu
     ``(q, scale, sum)`` of ``rmsnorm(x + residual, gamma, eps)`` and ``sum = bf16(x + residual)``. The norm and ``q``
     are taken from the unrounded sum. ``out`` takes the results in place; its ``sum`` may be ``x`` or ``residual``.
     """
-    xr = _rows(x, "x", torch.bfloat16)
-    rows, K, dev = xr[0], xr[1], x.device
-    g = _vec1(gamma, K, "gamma", torch.bfloat16, dev)
+    dev = _first(x, "x")
+    xr = _rows(x, "x", _BF16, dev)
+    rows, K = xr[:2]
+    g, gk = _vec1(gamma, K, "gamma", _BF16, dev)
     rr = tr = total = None
     if residual is not None:
-        rr = _rows(residual, "residual", torch.bfloat16, dev)
+        rr = _rows(residual, "residual", _BF16, dev)
         if residual.shape != x.shape:
             raise ValueError(f"residual must have the shape of x (got {list(residual.shape)})")
     if out is None:
-        q, qr = _new_int8(x.shape, rows, dev)
-        scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
+        device = x.device
+        q, qr = _new_int8(x.shape, rows, device)
+        scale = torch.empty(x.shape[:-1], dtype=_F32, device=device)
         sp = scale.data_ptr()
         if rr is not None:
-            total = torch.empty(x.shape, dtype=torch.bfloat16, device=dev)
-            tr = (rows, K, L.Mat(total.data_ptr(), rows, K, max(K, 1), L.TFB200_BF16), total)
+            total = torch.empty(x.shape, dtype=_BF16, device=device)
+            tr = (rows, K, L.Mat(total.data_ptr(), rows, K, K or 1, L.TFB200_BF16), total)
     else:
         if len(out) != (2 if residual is None else 3):
             raise ValueError("out must be (q, scale), and (q, scale, sum) with a residual")
         q, scale = out[:2]
-        qr, sp = _out(q, "q", torch.int8, x.shape, dev), _out_scale(scale, rows, dev)
+        qr, sp = _out(q, "q", _I8, x.shape, dev), _out_scale(scale, rows, dev)
         if rr is not None:
             total = out[2]
-            tr = _out(total, "sum", torch.bfloat16, x.shape, dev)
-    _call(dev, L.lib().tfb200_rmsnorm_int8, _ref(xr), _ref(rr), _ptr(g), eps, _ref(tr), _ref(qr), sp, _call)
+            tr = _out(total, "sum", _BF16, x.shape, dev)
+    _call(dev, L.lib().tfb200_rmsnorm_int8, _byref(xr[2]), _ref(rr), g, eps, _ref(tr), _byref(qr[2]), sp, _stream(dev))
     return (q, scale) if residual is None else (q, scale, total)
 
 
-def _result(x: torch.Tensor, rows: int, n: int, dtype: torch.dtype, out: torch.Tensor | None):
+def _result(x: torch.Tensor, rows: int, n: int, dtype: torch.dtype, out: torch.Tensor | None, dev: int):
     """A product's output, [..., N] for an input [..., K] (a caller's may also be given as [rows, N])."""
     if out is None:
         y = torch.empty(rows, n, dtype=dtype, device=x.device)
-        r = (rows, n, L.Mat(y.data_ptr(), rows, n, max(n, 1), _DTYPES[dtype]), y)
+        r = (rows, n, L.Mat(y.data_ptr(), rows, n, n or 1, _DTYPES[dtype]), y)
         return (y if x.dim() == 2 else y.view(*x.shape[:-1], n)), r
-    return out, _out(out, "out", dtype, (rows, n) if out.dim() == 2 else (*x.shape[:-1], n), x.device)
+    return out, _out(out, "out", dtype, (rows, n) if out.dim() == 2 else (*x.shape[:-1], n), dev)
 
 
 def matmul_int8_workspace_bytes(m: int, k: int, n: int) -> int:
@@ -458,29 +473,30 @@ def matmul_int8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale
     per row of each; exact integer sums, the rest in fp32, rounded once to ``out_dtype`` (bf16 or fp32). ``bias`` is
     bf16 ``[N]``, ``gelu`` "erf", "tanh" or None, ``residual`` bf16 ``[..., N]``. K is at most 131071.
     """
-    ar = _rows_int8(a, "a")
-    M, K, dev = ar[0], ar[1], a.device
+    dev = _first(a, "a")
+    ar = _rows_int8(a, "a", dev)
+    M, K = ar[:2]
     br = _rows_int8(b, "b", dev, True)
     N = br[0]
     if br[1] != K:
         raise ValueError(f"matmul_int8: a has K={K} but b has {br[1]} columns")
-    if out_dtype is not torch.bfloat16 and out_dtype is not torch.float32:
+    if out_dtype is not _BF16 and out_dtype is not _F32:
         raise TypeError(f"out_dtype must be bfloat16 or float32 (got {out_dtype})")
     if gelu not in _GELU_INT8:
         raise ValueError(f"gelu must be 'erf', 'tanh' or None (got {gelu!r})")
-    sa = _vec1(a_scale, M, "a_scale", torch.float32, dev)
-    sb = _vec1(b_scale, N, "b_scale", torch.float32, dev)
-    bv = _vec1(bias, N, "bias", torch.bfloat16, dev)
+    sa, sak = _vec1(a_scale, M, "a_scale", _F32, dev)
+    sb, sbk = _vec1(b_scale, N, "b_scale", _F32, dev)
+    bv, bvk = _vec1(bias, N, "bias", _BF16, dev)
     rr = None
     if residual is not None:
-        rr = _rows(residual, "residual", torch.bfloat16, dev)
+        rr = _rows(residual, "residual", _BF16, dev)
         if rr[0] != M or rr[1] != N:
             raise ValueError(f"residual must be [{M},{N}] (got {list(residual.shape)})")
-    y, yr = _result(a, M, N, out_dtype, out)
+    y, yr = _result(a, M, N, out_dtype, out, dev)
     lib = L.lib()
-    ws, wp, wn = _space(lib.tfb200_matmul_int8_workspace_size(M, K, N), workspace, dev)
-    _call(dev, lib.tfb200_matmul_int8, _ref(ar), _ptr(sa), _ref(br), _ptr(sb), _ptr(bv), _GELU_INT8[gelu], _ref(rr),
-          _ref(yr), _call, wp, wn)
+    ws, wp, wn = _space(lib.tfb200_matmul_int8_workspace_size(M, K, N), workspace, a)
+    _call(dev, lib.tfb200_matmul_int8, _byref(ar[2]), sa, _byref(br[2]), sb, bv, _GELU_INT8[gelu], _ref(rr),
+          _byref(yr[2]), _stream(dev), wp, wn)
     return y
 
 
@@ -493,19 +509,20 @@ def fused_rmsnorm_matmul_int8(x: torch.Tensor, gamma: torch.Tensor, w: torch.Ten
                               workspace: torch.Tensor | None = None) -> torch.Tensor:
     """``rmsnorm(x, gamma, eps) @ w`` on int8 ``w [N, K]`` with ``w_scale [N]``: ``fused_rmsnorm_matmul`` with the
     normalised rows quantised per token (``rmsnorm_int8``, then ``matmul_int8``)."""
-    xr = _rows(x, "x", torch.bfloat16)
-    M, K, dev = xr[0], xr[1], x.device
+    dev = _first(x, "x")
+    xr = _rows(x, "x", _BF16, dev)
+    M, K = xr[:2]
     wr = _rows_int8(w, "w", dev, True)
     N = wr[0]
     if wr[1] != K:
         raise ValueError(f"fused_rmsnorm_matmul_int8: x has K={K} but w has {wr[1]} columns")
-    g = _vec1(gamma, K, "gamma", torch.bfloat16, dev)
-    sw = _vec1(w_scale, N, "w_scale", torch.float32, dev)
-    y, yr = _result(x, M, N, torch.bfloat16, out)
+    g, gk = _vec1(gamma, K, "gamma", _BF16, dev)
+    sw, swk = _vec1(w_scale, N, "w_scale", _F32, dev)
+    y, yr = _result(x, M, N, _BF16, out, dev)
     lib = L.lib()
-    ws, wp, wn = _space(lib.tfb200_fused_rmsnorm_matmul_int8_workspace_size(M, K, N), workspace, dev)
-    _call(dev, lib.tfb200_fused_rmsnorm_matmul_int8, _ref(xr), _ptr(g), _ref(wr), _ptr(sw), eps, _ref(yr), _call, wp,
-          wn)
+    ws, wp, wn = _space(lib.tfb200_fused_rmsnorm_matmul_int8_workspace_size(M, K, N), workspace, x)
+    _call(dev, lib.tfb200_fused_rmsnorm_matmul_int8, _byref(xr[2]), g, _byref(wr[2]), sw, eps, _byref(yr[2]),
+          _stream(dev), wp, wn)
     return y
 
 
@@ -519,24 +536,25 @@ def fused_mlp_int8(x: torch.Tensor, gamma: torch.Tensor, w1: torch.Tensor, w1_sc
                    workspace: torch.Tensor | None = None) -> torch.Tensor:
     """``fused_mlp`` on int8 ``w1 [H, K]`` and ``w2 [N, H]`` with a scale per row: the normalised rows and the hidden
     block are quantised per token. ``b1`` is a bf16 ``[H]`` bias or None."""
-    xr = _rows(x, "x", torch.bfloat16)
-    M, K, dev = xr[0], xr[1], x.device
+    dev = _first(x, "x")
+    xr = _rows(x, "x", _BF16, dev)
+    M, K = xr[:2]
     w1r, w2r = _rows_int8(w1, "w1", dev, True), _rows_int8(w2, "w2", dev, True)
     H, N = w1r[0], w2r[0]
     if w1r[1] != K or w2r[1] != H:
         raise ValueError("fused_mlp_int8: shapes do not chain (x[M,K], w1[H,K], w2[N,H])")
-    rr = _rows(residual, "residual", torch.bfloat16, dev)
+    rr = _rows(residual, "residual", _BF16, dev)
     if rr[0] != M or rr[1] != N:
         raise ValueError(f"fused_mlp_int8: residual must be [{M},{N}] (got {list(residual.shape)})")
     if gelu not in _GELU:
         raise ValueError(f"gelu must be 'erf' or 'tanh' (got {gelu!r})")
-    g = _vec1(gamma, K, "gamma", torch.bfloat16, dev)
-    b = _vec1(b1, H, "b1", torch.bfloat16, dev)
-    s1 = _vec1(w1_scale, H, "w1_scale", torch.float32, dev)
-    s2 = _vec1(w2_scale, N, "w2_scale", torch.float32, dev)
-    y, yr = _result(x, M, N, torch.bfloat16, out)
+    g, gk = _vec1(gamma, K, "gamma", _BF16, dev)
+    b, bk = _vec1(b1, H, "b1", _BF16, dev)
+    s1, s1k = _vec1(w1_scale, H, "w1_scale", _F32, dev)
+    s2, s2k = _vec1(w2_scale, N, "w2_scale", _F32, dev)
+    y, yr = _result(x, M, N, _BF16, out, dev)
     lib = L.lib()
-    ws, wp, wn = _space(lib.tfb200_fused_mlp_int8_workspace_size(M, K, H, N), workspace, dev)
-    _call(dev, lib.tfb200_fused_mlp_int8, _ref(xr), _ptr(g), _ref(w1r), _ptr(s1), _ptr(b), _ref(w2r), _ptr(s2),
-          _ref(rr), eps, _GELU[gelu], _ref(yr), _call, wp, wn)
+    ws, wp, wn = _space(lib.tfb200_fused_mlp_int8_workspace_size(M, K, H, N), workspace, x)
+    _call(dev, lib.tfb200_fused_mlp_int8, _byref(xr[2]), g, _byref(w1r[2]), s1, b, _byref(w2r[2]), s2, _byref(rr[2]),
+          eps, _GELU[gelu], _byref(yr[2]), _stream(dev), wp, wn)
     return y
