@@ -219,6 +219,9 @@ int tfb200_fused_mlp_noalloc(const tfb200_mat* x, const void* gamma, const tfb20
  * 8-bit forms of golden.fused_rmsnorm_matmul and golden.fused_mlp
  * (golden.py:97-122).
  *
+ * A workspace belongs to one call at a time: calls on one stream may share it,
+ * calls that may overlap on the GPU each need their own.
+ *
  * A row that holds an infinity or a NaN gets scale NaN (and q = 0), so every
  * value computed from it is NaN; the other rows are not touched by it. A row of
  * zeros gets scale 0. RMSNorm's sum of squares is held in fp32: a row where it
@@ -241,8 +244,8 @@ int tfb200_rmsnorm_int8(const tfb200_mat* x, const tfb200_mat* residual, const v
  * gelu_mode any of enum tfb200_gelu, residual [M,N] bf16 or NULL, C [M,N] bf16 or
  * fp32. The sums are exact in int32, which bounds K to 131071
  * (TFB200_EUNSUPPORTED above); scales, bias, GELU and residual are applied in
- * fp32 and rounded once. K == 0 gives gelu(bias) + R. Equal calls give equal
- * bits. workspace: tfb200_matmul_int8_workspace_size bytes, 256-byte aligned. */
+ * fp32 and rounded once. K == 0 gives gelu(bias) + R. C may be R. Equal calls
+ * give equal bits. workspace: tfb200_matmul_int8_workspace_size bytes, 256-byte aligned. */
 size_t tfb200_matmul_int8_workspace_size(int64_t m, int64_t k, int64_t n);
 int tfb200_matmul_int8(const tfb200_mat* a, const float* a_scale, const tfb200_mat* b, const float* b_scale,
                        const void* bias, int gelu_mode, const tfb200_mat* residual, tfb200_mat* c, void* stream,

@@ -598,6 +598,26 @@ def test_two_streams_at_once(ops):
         assert all(torch.equal(y, want[m]) for y in got[m])
 
 
+def test_split_products_on_two_streams(ops):
+    """Products whose last wave is split over idle CTA pairs, several at once: finishing pairs wait for helpers."""
+    g = gen(10)
+    k, n = 16384, 2048
+    a, sa, b, sb, _, _ = operands(3, 300, n, k)
+    assert ops.matmul_int8_workspace_bytes(300, k, n) > 0
+    want = ops.matmul_int8(a, sa, b, sb)
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(4)], []
+    for _ in range(15):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(ops.matmul_int8(a, sa, b, sb))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want) for y in got)
+    from tfb200 import _lib as L
+
+    assert L.lib().tfb200_device_status() == L.TFB200_OK
+
+
 @pytest.mark.parametrize("m", [16, 80, 384])
 def test_weights_written_just_before(ops, m):
     """A product right behind the launch that writes its weights and scales."""

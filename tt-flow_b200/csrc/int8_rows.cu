@@ -359,23 +359,9 @@ __global__ void __launch_bounds__(WARP ? 128 : kMaxT, !WARP && PER == 32 && MODE
   const UpScale u = up_scale(st.amax, 127.0f);  // q = rn(t * u.up * u.r)
   if (t == 0) p.scale[row] = row_scale<KIND>(p, st);
   int8_t* q = p.q + row * p.ldq;
-  // A row of zeros, or one that is not finite, is stored as zeros.
-  const uint32_t keep = u.r == 0.0f ? 0u : 0xFFFFFFFFu;
-  const uint64_t rr = f2(u.r, u.r), up = f2(u.up, u.up), one = f2(p.one, p.one);
-#pragma unroll
-  for (int i = 0; i < G; ++i) {
+  const uint64_t rr = f2(u.r, u.r), one = f2(p.one, p.one);
+  auto store = [&](int i, const uint2& o) {
     const int k = first(i);
-    if (k >= K) break;
-    uint64_t b[4];
-    // A hidden value and its factor: h = value * block, q = rn(value * block * r).
-    const float hr = KIND == kInt8RowsHidden ? hm[i] * u.up * u.r * (1.0f / 32767.0f) : 0.0f;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint64_t s = KIND == kInt8RowsNorm ? v[KIND == kInt8RowsNorm ? i : 0][j] : in_pair<KIND>(xw[i][j]);
-      if (KIND != kInt8RowsHidden && u.up != 1.0f) s = f2_mul(s, up);
-      b[j] = q_pair(s, KIND == kInt8RowsHidden ? f2(hr, hr) : rr, one);
-    }
-    const uint2 o = make_uint2(pack4(b[0], b[1]) & keep, pack4(b[2], b[3]) & keep);
     if (MODE != kScalar && k + 8 <= K) {
       *reinterpret_cast<uint2*>(q + k) = o;
     } else {
@@ -383,6 +369,35 @@ __global__ void __launch_bounds__(WARP ? 128 : kMaxT, !WARP && PER == 32 && MODE
       for (int j = 0; j < 8; ++j)
         if (k + j * step < K) q[k + j * step] = static_cast<int8_t>(((j < 4 ? o.x : o.y) >> (8 * (j & 3))) & 0xFFu);
     }
+  };
+  auto quantise = [&](auto&& value) {
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      if (first(i) >= K) break;
+      uint64_t b[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) b[j] = value(i, j);
+      store(i, make_uint2(pack4(b[0], b[1]), pack4(b[2], b[3])));
+    }
+  };
+  // A row of zeros, one that is not finite (both are stored as zeros) and one of
+  // the smallest fp32 values go apart, so that the usual row costs nothing for
+  // them.
+  auto t_of = [&](int i, int j) {
+    return KIND == kInt8RowsNorm ? v[KIND == kInt8RowsNorm ? i : 0][j] : in_pair<KIND>(xw[i][j]);
+  };
+  if (KIND == kInt8RowsHidden) {
+    // A hidden value and its factor: h = value * block, q = rn(value * block * r).
+    quantise([&](int i, int j) {
+      const float hr = hm[KIND == kInt8RowsHidden ? i : 0] * u.up * u.r * (1.0f / 32767.0f);
+      return u.r != 0.0f ? q_pair(t_of(i, j), f2(hr, hr), one) : uint64_t(0);
+    });
+  } else if (u.r != 0.0f && u.up == 1.0f) {
+    quantise([&](int i, int j) { return q_pair(t_of(i, j), rr, one); });
+  } else {
+    quantise([&](int i, int j) {
+      return u.r != 0.0f ? q_pair(f2_mul(t_of(i, j), f2(u.up, u.up)), rr, one) : uint64_t(0);
+    });
   }
 }
 

@@ -267,7 +267,7 @@ _DTYPES = {torch.bfloat16: L.TFB200_BF16, torch.float32: L.TFB200_F32, torch.int
 # that build no Python objects: ``_rows`` and ``_out`` return the operand's C descriptor beside its shape, devices are
 # compared by index (25 us of host time a product with torch.cuda's accessors, 11 us without).
 _Tensor = torch.Tensor
-_stream = torch._C._cuda_getCurrentRawStream
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # absent from builds of torch without CUDA
 _BF16, _F32, _I8 = torch.bfloat16, torch.float32, torch.int8
 
 
