@@ -225,7 +225,8 @@ int tfb200_fused_mlp_noalloc(const tfb200_mat* x, const void* gamma, const tfb20
  * A row that holds an infinity or a NaN gets scale NaN (and q = 0), so every
  * value computed from it is NaN; the other rows are not touched by it. A row of
  * zeros gets scale 0. RMSNorm's sum of squares is held in fp32: a row where it
- * overflows (values above about 1e18) counts as not finite. */
+ * overflows (values above about 1e18) counts as not finite, and with eps == 0 one
+ * whose mean square is 0 there has no norm and gets scale NaN. */
 
 /* q[m,k] = rn(x[m,k] * 127 / amax), scale[m] = amax / 127, amax = max_k |x[m,k]|,
  * rounding half to even. X [M,K] bf16, Q [M,K] int8, scale [M]. Also lays out

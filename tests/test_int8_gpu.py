@@ -195,6 +195,24 @@ def test_rows_special_values(ops, k):
     assert ops.rmsnorm_int8(x[:1], gamma, 0.0)[1].isnan().all()
 
 
+@pytest.mark.parametrize("k", [5, 520, 3001, 8192, 40000])
+def test_rows_without_a_norm(ops, k):
+    """eps = 0: rows whose mean square is 0 in fp32 have no norm; the rows beside them do."""
+    x = normal(gen(k), 4, k).bfloat16()
+    x[1] = 0
+    x[2] *= 1e-30  # its squares are below the smallest fp32
+    gamma = torch.ones(k, device="cuda", dtype=torch.bfloat16)
+    for residual in (None, torch.zeros_like(x)):
+        q, scale = ops.rmsnorm_int8(x, gamma, 0.0, residual=residual)[:2]
+        assert scale[1:3].isnan().all()
+        for i in (0, 3):
+            qi, si = ops.rmsnorm_int8(x[i:i + 1], gamma, 0.0)[:2]
+            ref = norm64(x[i:i + 1], gamma, eps=0.0)[2]
+            # one row alone may be summed over more threads: mean of squares, root and two divisions, and the sum
+            assert ((scale[i] - ref).abs() <= 60 * U32 * ref).all() and ((si - ref).abs() <= 60 * U32 * ref).all()
+            assert torch.equal(q[i:i + 1], qi)
+
+
 def test_rows_empty_and_long_offsets(ops):
     q, scale = ops.quantize_int8(torch.empty(0, 64, dtype=torch.bfloat16, device="cuda"))
     assert q.shape == (0, 64) and scale.shape == (0,)

@@ -656,7 +656,8 @@ PairPlan pair_plan(int64_t m, int64_t n, int64_t k) {
       // Equal pieces: kc = ceil(KB / (parts + 1)), the parts share the rest.
       const int kc = (kb + parts) / (parts + 1);
       if (kb - kc < parts) break;
-      const double split = static_cast<double>(best.s.tiles / kSmPairs) * kb + kc + kSplitCost + kReadCost * parts + fixed;
+      const double split =
+          static_cast<double>(best.s.tiles / kSmPairs) * kb + kc + kSplitCost + kReadCost * parts + fixed;
       if (split < best.cost) {
         best.cost = split;
         best.s.waves = best.s.tiles / kSmPairs;
@@ -733,7 +734,8 @@ int launch_pair(const Int8Gemm& g, cudaStream_t s, std::string* err) {
   p.a_early = g.a_stable;
   const PairPlan plan = pair_plan(g.M, g.N, g.K);
   CUtensorMap ta{}, tb{}, tc{};
-  if (!int8_map(&ta, g.A, g.M, g.K, g.lda, kBM, err) || !int8_map(&tb, g.B, g.N, g.K, g.ldb, static_cast<uint32_t>(plan.bn / 2), err))
+  if (!int8_map(&ta, g.A, g.M, g.K, g.lda, kBM, err) ||
+      !int8_map(&tb, g.B, g.N, g.K, g.ldb, static_cast<uint32_t>(plan.bn / 2), err))
     return -3;
   if (p.fast && !make_map_box(&tc, g.C, g.M, g.N, g.ldc, static_cast<uint32_t>(64 / esz), 32,
                                    CU_TENSOR_MAP_SWIZZLE_64B, err,
@@ -816,7 +818,8 @@ int run_int8_gemm(const Int8Gemm& g, cudaStream_t stream, std::string* err) {
       pair_tiles(g.M, g.N, kMaxBN) <= (1 << 30))
     return use_stream(g.M, g.N, g.K) ? run_int8_stream(g, stream, err) : launch_pair(g, stream, err);
   const int64_t by = (g.N + kAnyTile - 1) / kAnyTile;
-  const dim3 grid(static_cast<unsigned>((g.M + kAnyTile - 1) / kAnyTile), static_cast<unsigned>(by < 65535 ? by : 65535));
+  const dim3 grid(static_cast<unsigned>((g.M + kAnyTile - 1) / kAnyTile),
+                  static_cast<unsigned>(by < 65535 ? by : 65535));
   k_int8_gemm_any<<<grid, 256, 0, stream>>>(g.A, g.lda, g.B, g.ldb, int8_epi(g));
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) {

@@ -126,8 +126,9 @@ template <int KIND>
 __device__ __forceinline__ float row_scale(const RowsParams& p, RowStat s) {
   if (s.amax >= 0x7F800000u) return __uint_as_float(0x7FC00000u);
   const float amax = __uint_as_float(s.amax);
-  return KIND == kInt8RowsNorm ? amax * (1.0f / sqrtf(s.ss / static_cast<float>(p.K) + p.eps) / 127.0f)
-                               : amax / 127.0f;
+  if (KIND != kInt8RowsNorm) return amax / 127.0f;
+  const float mean = s.ss / static_cast<float>(p.K) + p.eps;
+  return mean > 0.0f ? amax * (1.0f / sqrtf(mean) / 127.0f) : __uint_as_float(0x7FC00000u);
 }
 // Marks a row whose sum of squares left fp32 as not finite.
 template <int KIND>
@@ -187,7 +188,8 @@ __device__ __forceinline__ void prefetch_row(const uint16_t* row, int K) {
 // WARP: a warp per row (T = 32), else a block per row (T = blockDim.x).
 // PER: values per thread.
 template <int KIND, bool RES, Mode MODE, bool WARP, int PER>
-__global__ void __launch_bounds__(WARP ? 128 : kMaxT, !WARP && PER == 32 && MODE == kVec && KIND != kInt8RowsNorm ? 3 : 1)
+__global__ void __launch_bounds__(WARP ? 128 : kMaxT,
+                                  !WARP && PER == 32 && MODE == kVec && KIND != kInt8RowsNorm ? 3 : 1)
     k_int8_rows(const RowsParams p) {
   // Launched with programmatic serialization: wait for the grid before (it may
   // write x or still read q), then let the next grid start its prologue.
@@ -402,8 +404,7 @@ __global__ void __launch_bounds__(WARP ? 128 : kMaxT, !WARP && PER == 32 && MODE
 }
 
 // Rows longer than the registers of a block (unaligned ones over 16384 values):
-// the row is read twice, the second
-// time mostly from L2.
+// the row is read twice, the second time mostly from L2.
 template <int KIND, bool RES>
 __global__ void __launch_bounds__(1024) k_int8_rows_long(const RowsParams p) {
   grid_dep_wait();

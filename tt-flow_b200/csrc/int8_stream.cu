@@ -9,15 +9,16 @@
 // each channel block that lies in its range in TMEM. A block that lies whole in
 // one range is finished by its CTA; otherwise each CTA writes its int32 sums to
 // its slot (block + CTA, unique because the ranges are contiguous), and the last
-// to arrive (a counter) adds the slots and finishes the block. int32 sums are exact in any order, so equal
-// calls give equal bits.
+// to arrive (a counter) adds the slots and finishes the block. int32 sums are
+// exact in any order, so equal calls give equal bits.
 //
 // Only the counters must be zero on entry; the launch before clears them. The
 // first ring of B is requested before that launch has completed (it does not
 // write B), with an evict-first policy so that the stream does not push slots
 // and activations out of L2; A follows after the wait.
 //
-// Warps: 0 TMA producer, 1 MMA issuer, 2 TMEM allocator, 4-11 epilogue. All waits are bounded (kDevTimeout in the status word).
+// Warps: 0 TMA producer, 1 MMA issuer, 2 TMEM allocator, 4-11 epilogue. All
+// waits are bounded (kDevTimeout in the status word).
 #include <atomic>
 #include <mutex>
 
