@@ -410,7 +410,7 @@ def test_matmul_strides_and_surroundings(ops, m, n, k):
         assert (buf == 77).all(), "wrote outside the rows"
 
 
-@pytest.mark.parametrize("m", [1, 40, 100, 300])  # 131071 deep: streamed up to 128 rows
+@pytest.mark.parametrize("m", [1, 16, 40, 100, 300])  # 131071 deep: streamed up to 128 rows
 def test_matmul_extremes(ops, m):
     # The longest inner dimension with the largest products: the sums reach 2147467264 of 2147483647.
     k, n = 131071, 20
@@ -440,6 +440,46 @@ def test_matmul_extremes(ops, m):
 
 @pytest.mark.parametrize("m", [20, 300])
 def test_matmul_long_offsets(ops, m):
+    ld, n, k = 1 << 28, 10, 528
+    a, sa, b, sb, _, _ = operands(m, m, n, k)
+    big = torch.empty(9 * ld + k, dtype=torch.int8, device="cuda")
+    bv = torch.as_strided(big, (n, k), (ld, 1))
+    bv.copy_(b)
+    check(ops.matmul_int8(a, sa, bv, sb), product64(a, sa, b, sb))
+
+
+# (M, N, K): up to 16 rows, read straight into registers: both row counts' kernels, every width of a block (8, 16, 32
+# channels), ragged channels, inner dimensions that end inside a lane's 16 or 32 bytes, inside a step and after many
+HANDFULS = [(1, 1, 31), (1, 7, 16), (2, 33, 48), (1, 1000, 1009), (2, 4736, 1024), (2, 4745, 1040), (1, 9480, 272),
+            (1, 300, 16400), (3, 5, 31), (5, 33, 32), (8, 100, 63), (7, 1000, 1009), (8, 4745, 1040), (9, 31, 48),
+            (16, 9480, 272), (13, 300, 16400), (16, 4096, 4096), (11, 2000, 8223)]
+
+
+@pytest.mark.parametrize("m,n,k", HANDFULS)
+@pytest.mark.parametrize("off", [0, 16])
+def test_matmul_handful(ops, m, n, k, off):
+    a, sa, b, sb, bias, res = operands(m + 5 * n + 11 * k, m, n, k, lo=-128)
+    ld = (k + 15) // 16 * 16 + off
+    a, b = rows_at(a, off, ld)[0], rows_at(b, off, ld)[0]
+    check(ops.matmul_int8(a, sa, b, sb, out_dtype=torch.float32), product64(a, sa, b, sb, dtype=torch.float32))
+    y = res.clone()
+    check(ops.matmul_int8(a, sa, b, sb, bias=bias, gelu="erf", residual=y, out=y),
+          product64(a, sa, b, sb, bias, "erf", res))
+
+
+@pytest.mark.parametrize("n,k", [(33, 48), (520, 1009), (4800, 2048), (300, 16400)])
+def test_matmul_row_count_keeps_the_bits(ops, n, k):
+    """A row's result does not depend on how many rows are computed with it, whichever kernel that takes."""
+    a, sa, b, sb, bias, res = operands(n + k, 300, n, k)
+    a, b = aligned(a), aligned(b)
+    want = ops.matmul_int8(a, sa, b, sb, bias=bias, gelu="tanh", residual=res)
+    for m in (1, 2, 3, 8, 9, 16, 17, 32, 33, 128, 129):
+        y = ops.matmul_int8(a[:m], sa[:m], b, sb, bias=bias, gelu="tanh", residual=res[:m])
+        assert torch.equal(y, want[:m]), m
+
+
+@pytest.mark.parametrize("m", [1, 2, 16])
+def test_matmul_handful_long_offsets(ops, m):
     ld, n, k = 1 << 28, 10, 528
     a, sa, b, sb, _, _ = operands(m, m, n, k)
     big = torch.empty(9 * ld + k, dtype=torch.int8, device="cuda")
@@ -562,6 +602,28 @@ def test_mlp_bad_rows_stay_apart(ops):
         assert torch.equal(y[rest], good[rest])
 
 
+@pytest.mark.parametrize("k,h,n", [(100, 333, 50), (1024, 4100, 1000), (2048, 16400, 520), (9008, 520, 256)])
+def test_mlp_row_count_keeps_the_bits(ops, k, h, n):
+    g = gen(k + h)
+    x, gamma = normal(g, 300, k).bfloat16(), (torch.rand(k, generator=g, device="cuda") + 0.5).bfloat16()
+    w1, s1 = weight(ops, g, h, k)
+    w2, s2 = weight(ops, g, n, h)
+    b1, res = (normal(g, h) * 0.1).bfloat16(), normal(g, 300, n).bfloat16()
+    x[2, 1], x[5] = float("inf"), 0
+    want = ops.fused_mlp_int8(x, gamma, w1, s1, b1, w2, s2, res, EPS)
+    assert want[2].isnan().all() and not want[3:].isnan().any()
+    q, scale = ops.rmsnorm_int8(x, gamma, EPS)
+    for m in (1, 2, 7, 8, 9, 16, 17, 64, 128, 129):
+        # The norm's sum of squares is in the order of its block's threads, which are fewer for many rows: the scale
+        # of a row may differ in its last bits (the sums of up to 64 and a few more terms a thread: 60 U32), q not.
+        qm, sm = ops.rmsnorm_int8(x[:m], gamma, EPS)
+        assert torch.equal(qm, q[:m]) and ((sm - scale[:m]).abs() <= 60 * U32 * sm)[sm == sm].all()
+        same = sm.view(torch.int32) == scale[:m].view(torch.int32)
+        assert m < 64 or same.any()
+        y = ops.fused_mlp_int8(x[:m], gamma, w1, s1, b1, w2, s2, res[:m], EPS)
+        assert torch.equal(y[same].view(torch.int16), want[:m][same].view(torch.int16)), m
+
+
 # ------------------------------------------------------- streams and graphs
 
 
@@ -636,6 +698,29 @@ def test_split_products_on_two_streams(ops):
     assert L.lib().tfb200_device_status() == L.TFB200_OK
 
 
+@pytest.mark.parametrize("m", [1, 8, 40, 300])
+def test_fused_calls_behind_their_weights(ops, m):
+    """The products of the fused calls ask for weights before the launch ahead of them has ended."""
+    g = gen(m)
+    k, n = 2048, 4096
+    x, res = normal(g, m, k).bfloat16(), normal(g, m, k).bfloat16()
+    gamma = torch.ones(k, dtype=torch.bfloat16, device="cuda")
+    ups, downs = ([(normal(g, *s) / 45).bfloat16() for _ in range(3)] for s in ((n, k), (k, n)))
+    want = []
+    for u, d in zip(ups, downs):
+        (w1, s1), (w2, s2) = ops.quantize_int8(u), ops.quantize_int8(d)
+        want.append((ops.fused_rmsnorm_matmul_int8(x, gamma, w1, s1, EPS),
+                     ops.fused_mlp_int8(x, gamma, w1, s1, None, w2, s2, res, EPS)))
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for u, d, (y, z) in zip(ups, downs, want):
+            ops.quantize_int8(u, out=(w1, s1))
+            assert torch.equal(ops.fused_rmsnorm_matmul_int8(x, gamma, w1, s1, EPS), y)
+            ops.quantize_int8(d, out=(w2, s2))
+            ops.quantize_int8(u, out=(w1, s1))
+            assert torch.equal(ops.fused_mlp_int8(x, gamma, w1, s1, None, w2, s2, res, EPS), z)
+
+
 @pytest.mark.parametrize("m", [16, 80, 384])
 def test_weights_written_just_before(ops, m):
     """A product right behind the launch that writes its weights and scales."""
@@ -659,7 +744,7 @@ def test_workspace_reuse_and_checks(ops):
         a, sa, b, sb, _, _ = operands(m, m, n, k)
         a, b = aligned(a), aligned(b)
         need = ops.matmul_int8_workspace_bytes(m, k, n)
-        assert (need > 0) == (m != 400)
+        assert (need > 0) == (m in (100, 200))
         ws = torch.full((need + 256,), 255, dtype=torch.uint8, device="cuda")  # whatever it held before
         y = ops.matmul_int8(a, sa, b, sb, workspace=ws)
         assert torch.equal(y, ops.matmul_int8(a, sa, b, sb))

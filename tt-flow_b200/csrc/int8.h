@@ -70,13 +70,17 @@ struct Int8Gemm {
 struct Int8GemmWs {
   size_t clear_bytes = 0, total = 0;
 };
-Int8GemmWs int8_gemm_ws(int64_t m, int64_t n, int64_t k);
+Int8GemmWs int8_gemm_ws(int64_t m, int64_t n, int64_t k, bool hidden = false);
 int run_int8_gemm(const Int8Gemm& g, cudaStream_t stream, std::string* err);
 
 // Few rows (int8_stream.cu); operands as run_int8_gemm checks them for TMA.
 constexpr int64_t kInt8StreamRows = 128;
 Int8GemmWs int8_stream_ws(int64_t m, int64_t n);
 int run_int8_stream(const Int8Gemm& g, cudaStream_t stream, std::string* err);
+// A handful of rows (int8_gemv.cu); operands as above, no workspace.
+constexpr int64_t kInt8GemvRows = 16;
+double int8_gemv_us(int64_t m, int64_t n, int64_t k, bool hidden);  // estimate
+int run_int8_gemv(const Int8Gemm& g, cudaStream_t stream, std::string* err);
 // Tensor map of an int8 matrix in boxes of 128 columns (int8_gemm.cu).
 bool int8_map(CUtensorMap* m, const int8_t* base, int64_t rows, int64_t cols, int64_t ld, uint32_t box_rows,
               std::string* err);

@@ -88,7 +88,7 @@ Layout layout(int64_t m, int64_t k, int64_t h, int64_t n) {
     l.hq = take(rows * ld16(h));
     l.hscale = take(rows * 4);
   }
-  const Int8GemmWs up = int8_gemm_ws(m, h > 0 ? h : n, k);
+  const Int8GemmWs up = int8_gemm_ws(m, h > 0 ? h : n, k, h > 0);
   l.up = take(up.total);
   l.up_clear = up.clear_bytes;
   if (h > 0) {

@@ -747,7 +747,8 @@ int launch_pair(const Int8Gemm& g, cudaStream_t s, std::string* err) {
   p.ps = plan.s;
   if (p.ps.rem > 0 && resident >= kSmPairs) {
     p.flags = static_cast<int*>(g.ws);
-    p.slots = reinterpret_cast<int32_t*>(static_cast<char*>(g.ws) + int8_gemm_ws(g.M, g.N, g.K).clear_bytes);
+    const size_t clear = int8_gemm_ws(g.M, g.N, g.K, g.out == kInt8OutHidden).clear_bytes;
+    p.slots = reinterpret_cast<int32_t*>(static_cast<char*>(g.ws) + clear);
   } else {
     p.ps = sched::plan(p.ps.tiles, p.ps.kblocks, p.ps.tiles < resident ? p.ps.tiles : resident, 0);
   }
@@ -781,24 +782,32 @@ bool int8_map(CUtensorMap* m, const int8_t* base, int64_t rows, int64_t cols, in
                       CU_TENSOR_MAP_SWIZZLE_128B, err, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1);
 }
 
-// Few rows go to the weight-streaming kernel, unless the whole product is so
-// small that its per-call costs outweigh the weights' stream: by estimates in us,
-//   stream  5.6 + 0.075 per row (slots, arrivals, finish) + weights at 6 TB/s
-//   pair    2.5 + 0.29 per k-block of its plan + weights at 12 TB/s.
-// Measured, us, stream / pair: 2 x 1024 x 1024 6.3 / 5.5, 2 x 4096 x 4096 9.7 /
-// 14.3, 32 x 2048 x 2048 8.8 / 7.8, 32 x 4096 x 4096 11.3 / 13.4, 128 x 1024 x 1024
-// 16.1 / 5.8, 128 x 4096 x 4096 15.7 / 13.6, 128 x 16384 x 4096 23.3 / 30.8,
-// 128 x 8192 x 28672 50.0 / 53.4.
-static bool use_stream(int64_t m, int64_t n, int64_t k) {
-  if (m > kInt8StreamRows) return false;
+// The kernel of a product whose operands are aligned, by estimates in us:
+//   stream  up to 128 rows: 5.6 + 0.075 per row (slots, arrivals, finish) + weights
+//           at 6 TB/s
+//   gemv    up to 16 rows: int8_gemv_us
+//   pair    2.5 + 0.29 per k-block of its plan + weights at 12 TB/s
+// Measured, us, gemv / stream / pair: 1 x 1024 x 1024 2.0 / 6.3 / 5.5, 1 x 4096 x 4096
+// 4.4 / 9.7 / 14.3, 8 x 4096 x 16384 13.0 / 16.7, 8 x 8192 x 28672 39.9 / 42.5, 16 x
+// 8192 x 28672 47.0 / 42.9, 32 x 2048 x 2048 - / 8.8 / 7.8, 32 x 4096 x 4096 - / 11.3 /
+// 13.4, 128 x 1024 x 1024 - / 16.1 / 5.8, 128 x 4096 x 4096 - / 15.7 / 13.6,
+// 128 x 16384 x 4096 - / 23.3 / 30.8, 128 x 8192 x 28672 - / 50.0 / 53.4.
+enum Kernel { kPair, kStream, kGemv };
+static Kernel kernel_of(int64_t m, int64_t n, int64_t k, bool hidden) {
+  if (m > kInt8StreamRows) return kPair;
   const double mb = static_cast<double>(n) * static_cast<double>(k) * 1e-6;
-  return 5.6 + 0.075 * static_cast<double>(m) + mb / 6.0 <= 2.5 + 0.29 * pair_plan(m, n, k).cost + mb / 12.0;
+  const double stream = 5.6 + 0.075 * static_cast<double>(m) + mb / 6.0;
+  const double pair = 2.5 + 0.29 * pair_plan(m, n, k).cost + mb / 12.0;
+  if (m <= kInt8GemvRows && int8_gemv_us(m, n, k, hidden) <= (stream < pair ? stream : pair)) return kGemv;
+  return stream <= pair ? kStream : kPair;
 }
 
-Int8GemmWs int8_gemm_ws(int64_t m, int64_t n, int64_t k) {
+Int8GemmWs int8_gemm_ws(int64_t m, int64_t n, int64_t k, bool hidden) {
   Int8GemmWs w;
   if (k <= 0 || pair_tiles(m, n, kMaxBN) > (1 << 30)) return w;
-  if (use_stream(m, n, k)) return int8_stream_ws(m, n);
+  const Kernel kernel = kernel_of(m, n, k, hidden);
+  if (kernel == kGemv) return w;
+  if (kernel == kStream) return int8_stream_ws(m, n);
   const sched::PairSched ps = pair_plan(m, n, k).s;
   if (ps.rem > 0) {
     w.clear_bytes = (static_cast<size_t>(ps.rem) * ps.parts * 2 * kEpiWarps * sizeof(int) + 255) / 256 * 256;
@@ -816,7 +825,11 @@ int run_int8_gemm(const Int8Gemm& g, cudaStream_t stream, std::string* err) {
   // that are multiples of 16 bytes (one row has no stride).
   if (g.K > 0 && al(g.A, 16) && al(g.B, 16) && (g.lda % 16 == 0 || g.M == 1) && (g.ldb % 16 == 0 || g.N == 1) &&
       pair_tiles(g.M, g.N, kMaxBN) <= (1 << 30))
-    return use_stream(g.M, g.N, g.K) ? run_int8_stream(g, stream, err) : launch_pair(g, stream, err);
+    switch (kernel_of(g.M, g.N, g.K, g.out == kInt8OutHidden)) {
+      case kGemv: return run_int8_gemv(g, stream, err);
+      case kStream: return run_int8_stream(g, stream, err);
+      case kPair: return launch_pair(g, stream, err);
+    }
   const int64_t by = (g.N + kAnyTile - 1) / kAnyTile;
   const dim3 grid(static_cast<unsigned>((g.M + kAnyTile - 1) / kAnyTile),
                   static_cast<unsigned>(by < 65535 ? by : 65535));
