@@ -19,6 +19,8 @@
 // warp (with three blocks of more registers 4096 channels no longer fit the GPU at
 // once: 8 x 16384 x 4096 19 us). Copies through shared memory (cp.async) were
 // slower at every size.
+#include <algorithm>
+
 #include "int8_math.cuh"
 
 namespace tfb200 {
@@ -94,6 +96,22 @@ __device__ __forceinline__ Col load_col(const Int8Epi& e, int n0) {
   return c;
 }
 
+// The rows of the next product's weights, the first bytes of which are brought
+// into L2 when the block's own are on their way (0: none).
+struct Next {
+  const int8_t* b;
+  int64_t ld;
+  int rows, rows_per_block;
+  uint32_t bytes;
+};
+__device__ __forceinline__ void prefetch_next(const Next& x) {
+  for (int i = threadIdx.x; i < x.rows_per_block; i += kWarps * 32) {
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * x.rows_per_block + i;
+    if (row < x.rows)
+      asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(x.b + row * x.ld), "r"(x.bytes) : "memory");
+  }
+}
+
 // A thread finishes eight neighbouring channels of a token.
 template <int MT, int CH, int KS>
 __device__ __forceinline__ void finish(const Int8Epi& e, Sums<MT, CH, KS>& s, int n0, const Col& col) {
@@ -132,7 +150,8 @@ __device__ __forceinline__ void finish(const Int8Epi& e, Sums<MT, CH, KS>& s, in
 // MT tokens (M rounded up), four channels a warp, KS warps to a channel's K.
 template <int MT, int CH>
 __global__ void __launch_bounds__(kWarps * 32, kBlocks)
-    k_int8_gemv_dot(const int8_t* A, int64_t lda, const int8_t* B, int64_t ldb, const Int8Epi e, int b_early) {
+    k_int8_gemv_dot(const int8_t* A, int64_t lda, const int8_t* B, int64_t ldb, const Int8Epi e, int b_early,
+                    const Next next) {
   constexpr int kR = 4, KS = kWarps * kR / CH, kU = 2, kStep = KS * 512;
   __shared__ Sums<MT, CH, KS> s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -180,6 +199,7 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocks)
     if (k - lane * 16 >= K) break;  // warp-uniform
     load_b();
   }
+  prefetch_next(next);
   // The row's last K % 16 values, a lane each.
   if (part == 0 && lane < (K & 15)) {
     const int at = (K & ~15) + lane;
@@ -201,7 +221,8 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocks)
 // MT 8 or 16, eight channels a warp.
 template <int MT, int CH, bool WIDE>
 __global__ void __launch_bounds__(kWarps * 32, kBlocks)
-    k_int8_gemv_mma(const int8_t* A, int64_t lda, const int8_t* B, int64_t ldb, const Int8Epi e, int b_early) {
+    k_int8_gemv_mma(const int8_t* A, int64_t lda, const int8_t* B, int64_t ldb, const Int8Epi e, int b_early,
+                    const Next next) {
   constexpr int KS = kWarps * 8 / CH, kU = 2, kSeg = kU * 128;
   __shared__ Sums<MT, CH, KS> s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -244,6 +265,7 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocks)
     if (k - t * 32 >= K) break;  // warp-uniform
     load_b();
   }
+  prefetch_next(next);
   if (part == 0 && (K & 31)) {  // the row's last K % 32 values, eight a lane
     const int n = (K & 31) - t * 8, at = (K & ~31) + t * 8;
     uint32_t x[2][2] = {};
@@ -258,7 +280,7 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocks)
   finish(e, s, n0, col);
 }
 
-using GemvKernel = void (*)(const int8_t*, int64_t, const int8_t*, int64_t, const Int8Epi, int);
+using GemvKernel = void (*)(const int8_t*, int64_t, const int8_t*, int64_t, const Int8Epi, int, const Next);
 template <int CH>
 GemvKernel gemv_kernel(int64_t m, bool wide) {
   if (m <= 2) return m == 1 ? k_int8_gemv_dot<1, CH> : k_int8_gemv_dot<2, CH>;
@@ -279,22 +301,41 @@ int channels(int64_t n, int64_t k, bool hidden) {
 
 }  // namespace
 
-// Start and end, then the weights at the rate the kernels reach (6.7, 5.9 and 5
-// TB/s for up to 2, 8 and 16 rows), or a warp's batches one after the other.
+// Start and end, then the weights at the rate the kernels reach, or a warp's batches
+// one after the other.
 double int8_gemv_us(int64_t m, int64_t n, int64_t k, bool hidden) {
   const int ch = channels(n, k, hidden);
   const int64_t blocks = (n + ch - 1) / ch;
   const int64_t batch = m <= 2 ? 1024 * (kWarps * 4 / ch) : 256 * (kWarps * 8 / ch);  // k values of a step
   const double steps = static_cast<double>((k + batch - 1) / batch * ((blocks + kAtOnce - 1) / kAtOnce));
-  const double stream = static_cast<double>(n) * static_cast<double>(k) * 1e-6 / (m <= 2 ? 6.7 : m <= 8 ? 5.9 : 5.0);
+  const double rate = m <= 2 ? 6.7 : m <= 8 ? 5.9 : 5.0;  // TB/s
+  const double stream = static_cast<double>(n) * static_cast<double>(k) * 1e-6 / rate;
   return 1.2 + (stream > 0.7 * steps ? stream : 0.7 * steps);
 }
+
+// Bytes of the next product's weights that are brought into L2, which fills HBM's
+// pause between the MLP's products. Whole MLP, us, with 0 / 12 / 40 MB:
+// 1 x 4096 x 16384 26.5 / 26.1 / 25.4, 2 x 4096 x 16384 28.9 / 28.1 / 27.0,
+// 1 x 8192 x 28672 74.4 / 74.0 / 74.2, 8 x 8192 x 28672 85.9 / 85.5 / 86.1,
+// 8 x 4096 x 16384 30.2 / 30.3 / 30.6, 8 x 2048 x 8192 15.5 / 15.0 / 14.7,
+// 16 x 4096 x 16384 35.2 / 34.9 / 35.8.
+int64_t next_bytes(int64_t m) { return static_cast<int64_t>(m <= 2 ? 40 : 12) << 20; }
 
 int run_int8_gemv(const Int8Gemm& g, cudaStream_t stream, std::string* err) {
   const bool wide = (reinterpret_cast<uintptr_t>(g.B) & 31u) == 0 && (g.ldb % 32 == 0 || g.N == 1);
   const int ch = channels(g.N, g.K, g.out == kInt8OutHidden);
   const GemvKernel kernel =
       ch == 8 ? gemv_kernel<8>(g.M, wide) : ch == 16 ? gemv_kernel<16>(g.M, wide) : gemv_kernel<32>(g.M, wide);
+  Next next{};
+  if (g.next_b && g.next_ld % 16 == 0 && (reinterpret_cast<uintptr_t>(g.next_b) & 15u) == 0) {
+    const int64_t blocks = (g.N + ch - 1) / ch;
+    next.b = g.next_b;
+    next.ld = g.next_ld;
+    next.rows = static_cast<int>(g.next_n);
+    next.rows_per_block = static_cast<int>((g.next_n + blocks - 1) / blocks);
+    next.bytes = static_cast<uint32_t>(std::min(g.next_k, next_bytes(g.M) / g.next_n) / 16 * 16);
+    if (next.bytes == 0) next.rows_per_block = 0;
+  }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>((g.N + ch - 1) / ch), 1, 1);
   cfg.blockDim = dim3(kWarps * 32, 1, 1);
@@ -304,7 +345,8 @@ int run_int8_gemv(const Int8Gemm& g, cudaStream_t stream, std::string* err) {
   a[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = a;
   cfg.numAttrs = 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, g.A, g.lda, g.B, g.ldb, int8_epi(g), static_cast<int>(g.b_stable));
+  cudaError_t e =
+      cudaLaunchKernelEx(&cfg, kernel, g.A, g.lda, g.B, g.ldb, int8_epi(g), static_cast<int>(g.b_stable), next);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) {
     *err = std::string("int8 gemv launch: ") + cudaGetErrorString(e);
