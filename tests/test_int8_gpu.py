@@ -448,11 +448,14 @@ def test_matmul_long_offsets(ops, m):
     check(ops.matmul_int8(a, sa, bv, sb), product64(a, sa, b, sb))
 
 
-# (M, N, K): up to 16 rows, read straight into registers: both row counts' kernels, every width of a block (8, 16, 32
+# (M, N, K): up to 32 rows, read straight into registers: every row count's kernel, every width of a block (8, 16, 32
 # channels), ragged channels, inner dimensions that end inside a lane's 16 or 32 bytes, inside a step and after many
 HANDFULS = [(1, 1, 31), (1, 7, 16), (2, 33, 48), (1, 1000, 1009), (2, 4736, 1024), (2, 4745, 1040), (1, 9480, 272),
             (1, 300, 16400), (3, 5, 31), (5, 33, 32), (8, 100, 63), (7, 1000, 1009), (8, 4745, 1040), (9, 31, 48),
-            (16, 9480, 272), (13, 300, 16400), (16, 4096, 4096), (11, 2000, 8223)]
+            (16, 9480, 272), (13, 300, 16400), (16, 4096, 4096), (11, 2000, 8223), (17, 33, 48), (24, 1000, 1009),
+            (32, 4745, 1040), (25, 9480, 272), (31, 300, 16400), (32, 7, 31),
+            # more rows before larger weights: the weight-streaming kernel again
+            (20, 6144, 4100), (16, 28672, 8192), (32, 28672, 1024)]
 
 
 @pytest.mark.parametrize("m,n,k", HANDFULS)
@@ -473,12 +476,12 @@ def test_matmul_row_count_keeps_the_bits(ops, n, k):
     a, sa, b, sb, bias, res = operands(n + k, 300, n, k)
     a, b = aligned(a), aligned(b)
     want = ops.matmul_int8(a, sa, b, sb, bias=bias, gelu="tanh", residual=res)
-    for m in (1, 2, 3, 8, 9, 16, 17, 32, 33, 128, 129):
+    for m in (1, 2, 3, 8, 9, 16, 17, 24, 25, 32, 33, 128, 129):
         y = ops.matmul_int8(a[:m], sa[:m], b, sb, bias=bias, gelu="tanh", residual=res[:m])
         assert torch.equal(y, want[:m]), m
 
 
-@pytest.mark.parametrize("m", [1, 2, 16])
+@pytest.mark.parametrize("m", [1, 2, 16, 32])
 def test_matmul_handful_long_offsets(ops, m):
     ld, n, k = 1 << 28, 10, 528
     a, sa, b, sb, _, _ = operands(m, m, n, k)
@@ -613,7 +616,7 @@ def test_mlp_row_count_keeps_the_bits(ops, k, h, n):
     want = ops.fused_mlp_int8(x, gamma, w1, s1, b1, w2, s2, res, EPS)
     assert want[2].isnan().all() and not want[3:].isnan().any()
     q, scale = ops.rmsnorm_int8(x, gamma, EPS)
-    for m in (1, 2, 7, 8, 9, 16, 17, 64, 128, 129):
+    for m in (1, 2, 7, 8, 9, 16, 17, 25, 32, 64, 128, 129):
         # The norm's sum of squares is in the order of its block's threads, which are fewer for many rows: the scale
         # of a row may differ in its last bits (the sums of up to 64 and a few more terms a thread: 60 U32), q not.
         qm, sm = ops.rmsnorm_int8(x[:m], gamma, EPS)

@@ -78,7 +78,7 @@ constexpr int64_t kInt8StreamRows = 128;
 Int8GemmWs int8_stream_ws(int64_t m, int64_t n);
 int run_int8_stream(const Int8Gemm& g, cudaStream_t stream, std::string* err);
 // A handful of rows (int8_gemv.cu); operands as above, no workspace.
-constexpr int64_t kInt8GemvRows = 16;
+constexpr int64_t kInt8GemvRows = 32;
 double int8_gemv_us(int64_t m, int64_t n, int64_t k, bool hidden);  // estimate
 int run_int8_gemv(const Int8Gemm& g, cudaStream_t stream, std::string* err);
 // Tensor map of an int8 matrix in boxes of 128 columns (int8_gemm.cu).

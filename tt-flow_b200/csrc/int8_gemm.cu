@@ -785,13 +785,15 @@ bool int8_map(CUtensorMap* m, const int8_t* base, int64_t rows, int64_t cols, in
 // The kernel of a product whose operands are aligned, by estimates in us:
 //   stream  up to 128 rows: 5.6 + 0.075 per row (slots, arrivals, finish) + weights
 //           at 6 TB/s
-//   gemv    up to 16 rows: int8_gemv_us
+//   gemv    up to 32 rows: int8_gemv_us
 //   pair    2.5 + 0.29 per k-block of its plan + weights at 12 TB/s
 // Measured, us, gemv / stream / pair: 1 x 1024 x 1024 2.0 / 6.3 / 5.5, 1 x 4096 x 4096
-// 4.4 / 9.7 / 14.3, 8 x 4096 x 16384 13.0 / 16.7, 8 x 8192 x 28672 39.9 / 42.5, 16 x
-// 8192 x 28672 47.0 / 42.9, 32 x 2048 x 2048 - / 8.8 / 7.8, 32 x 4096 x 4096 - / 11.3 /
-// 13.4, 128 x 1024 x 1024 - / 16.1 / 5.8, 128 x 4096 x 4096 - / 15.7 / 13.6,
-// 128 x 16384 x 4096 - / 23.3 / 30.8, 128 x 8192 x 28672 - / 50.0 / 53.4.
+// 4.4 / 9.7 / 14.3, 8 x 4096 x 16384 13.0 / 16.7, 8 x 8192 x 28672 39.9 / 42.5,
+// 16 x 4096 x 4096 5.9 / 10.2, 16 x 8192 x 28672 47.0 / 42.9, 32 x 2048 x 2048 4.8 / 8.8 /
+// 7.8, 32 x 4096 x 4096 8.6 / 11.3 / 13.4, 32 x 4096 x 6144 13.6 / 13.1, 64 x 2048 x 2048
+// (four tiles of tokens) 11.3 / - / 7.9, 128 x 1024 x 1024 - / 16.1 / 5.8,
+// 128 x 4096 x 4096 - / 15.7 / 13.6, 128 x 16384 x 4096 - / 23.3 / 30.8,
+// 128 x 8192 x 28672 - / 50.0 / 53.4.
 enum Kernel { kPair, kStream, kGemv };
 static Kernel kernel_of(int64_t m, int64_t n, int64_t k, bool hidden) {
   if (m > kInt8StreamRows) return kPair;

@@ -9,7 +9,7 @@
 //   k_int8_gemv_dot: one or two tokens. A warp reads 512 bytes of each of four
 //     channels at a time and multiplies by dp4a; a lane's sums are added up at the
 //     end. More tokens run into dp4a's latency (8 x 16384 x 4096: 24 us, 13 below).
-//   k_int8_gemv_mma: up to 16 tokens, mma m16n8k32 with tokens as the 16 rows and
+//   k_int8_gemv_mma: up to 32 tokens, mma m16n8k32 with tokens as the 16 rows and
 //     channels as the 8 columns. A lane holds 4 + 4 k values of one token and one
 //     channel per instruction; which k they are is free as long as both operands
 //     agree, so a lane takes 32 neighbouring bytes of each for four of them, and a
@@ -218,12 +218,13 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocks)
   finish(e, s, n0, col);
 }
 
-// MT 8 or 16, eight channels a warp.
+// MT 8, 16 or 32, eight channels a warp.
 template <int MT, int CH, bool WIDE>
 __global__ void __launch_bounds__(kWarps * 32, kBlocks)
     k_int8_gemv_mma(const int8_t* A, int64_t lda, const int8_t* B, int64_t ldb, const Int8Epi e, int b_early,
                     const Next next) {
   constexpr int KS = kWarps * 8 / CH, kU = 2, kSeg = kU * 128;
+  constexpr int kTiles = (MT + 15) / 16, kHalves = MT >= 16 ? 2 : 1;  // tiles of 16 tokens, one or both halves
   __shared__ Sums<MT, CH, KS> s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int grp = warp / KS, part = warp % KS;
@@ -232,9 +233,7 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocks)
   grid_dep_launch();
   if (!b_early) grid_dep_wait();
   const int8_t* b = B + static_cast<int64_t>(min(n0 + grp * 8 + g, e.N - 1)) * ldb;
-  const int8_t* a[MT / 8];
-#pragma unroll
-  for (int i = 0; i < MT / 8; ++i) a[i] = A + min(g + 8 * i, e.M - 1) * lda;
+  auto token = [&](int m) { return A + min(g + m, e.M - 1) * lda; };
   const int K = e.K;
   const uint64_t policy = l2_policy_evict_first();
   Bytes32 bv[kU];
@@ -247,19 +246,23 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocks)
   load_b();
   if (b_early) grid_dep_wait();
   const Col col = load_col<CH>(e, n0);
-  int32_t acc[4] = {};
+  int32_t acc[kTiles][4] = {};
   while (true) {
 #pragma unroll
     for (int u = 0; u < kU; ++u)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int at = k + u * 128 + h * 16;
-        uint4 x[2] = {};
 #pragma unroll
-        for (int i = 0; i < MT / 8; ++i)
-          if (k + u * 128 + 32 <= K && g + 8 * i < e.M) x[i] = *reinterpret_cast<const uint4*>(a[i] + at);
-        mma_16x8x32(acc, x[0].x, x[1].x, x[0].y, x[1].y, bv[u].w[4 * h], bv[u].w[4 * h + 1]);
-        mma_16x8x32(acc, x[0].z, x[1].z, x[0].w, x[1].w, bv[u].w[4 * h + 2], bv[u].w[4 * h + 3]);
+        for (int j = 0; j < kTiles; ++j) {
+          uint4 x[2] = {};
+#pragma unroll
+          for (int i = 0; i < kHalves; ++i)
+            if (k + u * 128 + 32 <= K && g + 16 * j + 8 * i < e.M)
+              x[i] = *reinterpret_cast<const uint4*>(token(16 * j + 8 * i) + at);
+          mma_16x8x32(acc[j], x[0].x, x[1].x, x[0].y, x[1].y, bv[u].w[4 * h], bv[u].w[4 * h + 1]);
+          mma_16x8x32(acc[j], x[0].z, x[1].z, x[0].w, x[1].w, bv[u].w[4 * h + 2], bv[u].w[4 * h + 3]);
+        }
       }
     k += KS * kSeg;
     if (k - t * 32 >= K) break;  // warp-uniform
@@ -268,15 +271,24 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocks)
   prefetch_next(next);
   if (part == 0 && (K & 31)) {  // the row's last K % 32 values, eight a lane
     const int n = (K & 31) - t * 8, at = (K & ~31) + t * 8;
-    uint32_t x[2][2] = {};
+    const uint32_t w[2] = {load_part(b + at, n), load_part(b + at + 4, n - 4)};
 #pragma unroll
-    for (int i = 0; i < MT / 8; ++i)
-      if (g + 8 * i < e.M) x[i][0] = load_part(a[i] + at, n), x[i][1] = load_part(a[i] + at + 4, n - 4);
-    mma_16x8x32(acc, x[0][0], x[1][0], x[0][1], x[1][1], load_part(b + at, n), load_part(b + at + 4, n - 4));
+    for (int j = 0; j < kTiles; ++j) {
+      uint32_t x[2][2] = {};
+#pragma unroll
+      for (int i = 0; i < kHalves; ++i) {
+        const int8_t* a = token(16 * j + 8 * i) + at;
+        if (g + 16 * j + 8 * i < e.M) x[i][0] = load_part(a, n), x[i][1] = load_part(a + 4, n - 4);
+      }
+      mma_16x8x32(acc[j], x[0][0], x[1][0], x[0][1], x[1][1], w[0], w[1]);
+    }
   }
 #pragma unroll
-  for (int i = 0; i < MT / 8; ++i)
-    *reinterpret_cast<int2*>(&s.v[part][g + 8 * i][grp * 8 + 2 * t]) = make_int2(acc[2 * i], acc[2 * i + 1]);
+  for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+    for (int i = 0; i < kHalves; ++i)
+      *reinterpret_cast<int2*>(&s.v[part][g + 16 * j + 8 * i][grp * 8 + 2 * t]) =
+          make_int2(acc[j][2 * i], acc[j][2 * i + 1]);
   finish(e, s, n0, col);
 }
 
@@ -285,7 +297,8 @@ template <int CH>
 GemvKernel gemv_kernel(int64_t m, bool wide) {
   if (m <= 2) return m == 1 ? k_int8_gemv_dot<1, CH> : k_int8_gemv_dot<2, CH>;
   if (m <= 8) return wide ? k_int8_gemv_mma<8, CH, true> : k_int8_gemv_mma<8, CH, false>;
-  return wide ? k_int8_gemv_mma<16, CH, true> : k_int8_gemv_mma<16, CH, false>;
+  if (m <= 16) return wide ? k_int8_gemv_mma<16, CH, true> : k_int8_gemv_mma<16, CH, false>;
+  return wide ? k_int8_gemv_mma<32, CH, true> : k_int8_gemv_mma<32, CH, false>;
 }
 
 // Channels a block: eight, the warps sharing K as widely as they can, unless that
@@ -301,16 +314,16 @@ int channels(int64_t n, int64_t k, bool hidden) {
 
 }  // namespace
 
-// Start and end, then the weights at the rate the kernels reach, or a warp's batches
-// one after the other.
+// Start and end, then the weights at the rate the kernels reach (for more tokens what
+// L1 delivers of them), or a warp's batches one after the other.
 double int8_gemv_us(int64_t m, int64_t n, int64_t k, bool hidden) {
   const int ch = channels(n, k, hidden);
   const int64_t blocks = (n + ch - 1) / ch;
   const int64_t batch = m <= 2 ? 1024 * (kWarps * 4 / ch) : 256 * (kWarps * 8 / ch);  // k values of a step
   const double steps = static_cast<double>((k + batch - 1) / batch * ((blocks + kAtOnce - 1) / kAtOnce));
-  const double rate = m <= 2 ? 6.7 : m <= 8 ? 5.9 : 5.0;  // TB/s
+  const double rate = m <= 2 ? 6.7 : m <= 8 ? 5.9 : m <= 16 ? 5.0 : 2.4;  // TB/s
   const double stream = static_cast<double>(n) * static_cast<double>(k) * 1e-6 / rate;
-  return 1.2 + (stream > 0.7 * steps ? stream : 0.7 * steps);
+  return (m <= 16 ? 1.2 : 2.2) + (stream > 0.7 * steps ? stream : 0.7 * steps);
 }
 
 // Bytes of the next product's weights that are brought into L2, which fills HBM's
