@@ -220,7 +220,9 @@ int tfb200_fused_mlp_noalloc(const tfb200_mat* x, const void* gamma, const tfb20
  * (golden.py:97-122).
  *
  * A workspace belongs to one call at a time: calls on one stream may share it,
- * calls that may overlap on the GPU each need their own.
+ * calls that may overlap on the GPU each need their own. Its size depends on the
+ * kernel that the sizes take, and so may be larger for fewer rows (and 0 for a
+ * handful): one that serves several row counts has the largest of their sizes.
  *
  * A row that holds an infinity or a NaN gets scale NaN (and q = 0), so every
  * value computed from it is NaN; the other rows are not touched by it. A row of

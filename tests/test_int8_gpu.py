@@ -758,6 +758,33 @@ def test_workspace_reuse_and_checks(ops):
                 ops.matmul_int8(a, sa, b, sb, workspace=ws[:need - 1])
 
 
+def test_one_workspace_behind_one_another(ops):
+    """Calls of every row count's kernels share a workspace on one stream, each launched while the last still runs."""
+    g = gen(12)
+    k, h = 1024, 4096
+    gamma = torch.ones(k, dtype=torch.bfloat16, device="cuda")
+    w1, s1 = weight(ops, g, h, k)
+    w2, s2 = weight(ops, g, k, h)
+    xs = [normal(g, m, k).bfloat16() for m in (1, 8, 24, 60, 100, 150, 300)]
+    hs = [ops.quantize_int8(normal(g, m, h).bfloat16()) for m in (1, 8, 24, 60, 100, 150, 300)]
+    need = max(max(ops.mlp_int8_workspace_bytes(x.shape[0], k, h, k), ops.matmul_int8_workspace_bytes(x.shape[0], h, k),
+                   ops.rmsnorm_matmul_int8_workspace_bytes(x.shape[0], k, h)) for x in xs)
+    ws = torch.full((need,), 255, dtype=torch.uint8, device="cuda")
+
+    def calls(**kw):
+        for x, (q, s) in zip(xs, hs):
+            yield ops.fused_mlp_int8(x, gamma, w1, s1, None, w2, s2, x, EPS, **kw)
+            yield ops.matmul_int8(q, s, w2, s2, residual=x, **kw)
+            yield ops.fused_rmsnorm_matmul_int8(x, gamma, w1, s1, EPS, **kw)
+
+    want = list(calls())
+    torch.cuda.synchronize()
+    got = [list(calls(workspace=ws)) for _ in range(5)]
+    torch.cuda.synchronize()
+    for ys in got:
+        assert all(torch.equal(y, w) for y, w in zip(ys, want))
+
+
 def test_refusals(ops):
     g = gen(1)
     x = normal(g, 4, 64).bfloat16()
