@@ -350,6 +350,11 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
     const int c0 = (ew >> 2) * kChunks;
     const int r = q * 32 + lane;
     const uint32_t bufs = smem_u32(sC) + static_cast<uint32_t>(ew * 2) * kStageOut;
+    // Of 16-bit results, a store's block is staged while the one before it may
+    // still be read, so the warp's stores take its two buffers in turn. They are
+    // counted over all its tiles: a tile may end after any number of them (one in
+    // a 64-column tile, or where the matrix ends).
+    uint32_t odd_store = 0;
     for (int i = 0; i < nwork; ++i) {
       const Work w = item_at(ps, pair, i);
       int tm, tn;
@@ -445,7 +450,7 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
             }
           }
         }
-        const uint32_t buf = bufs + (p.e.out == kInt8OutF32 ? 0u : static_cast<uint32_t>(c & 1) * kStageOut);
+        const uint32_t buf = bufs + (p.e.out == kInt8OutF32 ? 0u : odd_store * kStageOut);
         uint64_t v2[16];  // fp32 pairs
         {
           const ulonglong2* sb = reinterpret_cast<const ulonglong2*>(ctl->sb + c * 32);
@@ -526,7 +531,8 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
                 f[j] = __fadd_rn(f[j], __bfloat162float(p.e.residual[row * p.e.ldr + col0 + j]));
           }
         }
-        // The stores that used this buffer (fp32: both buffers) have read it.
+        // The store that used this buffer has read it: 16-bit results, all but the
+        // last (which used the other); fp32 results fill both, so all of them.
         if (lane == 0) {
           if (p.e.out == kInt8OutF32)
             bulk_wait_read<0>();
@@ -572,6 +578,7 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
             tma_store_2d(&tmC, buf + kStageOut, col0 + 16, static_cast<int32_t>(row0));
           bulk_commit();
         }
+        odd_store ^= 1u;
       }
       if (part) {
         // One release for the warp's rows (one per chunk cost 1.3 us each).
