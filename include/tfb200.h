@@ -263,7 +263,7 @@ int tfb200_fused_rmsnorm_matmul_int8(const tfb200_mat* x, const void* gamma, con
                                      size_t workspace_bytes);
 
 /* Y = quantize(gelu(rmsnorm_int8(X) @ W1^T + b1)) @ W2^T + R, the hidden block
- * quantised per token. W1 [H,K], w1_scale [H], b1 [H] bf16 or NULL, W2 [N,H],
+ * held in fp32 (in the workspace) and quantised per token. W1 [H,K], w1_scale [H], b1 [H] bf16 or NULL, W2 [N,H],
  * w2_scale [N], R [M,N] (may be X when N == K), Y [M,N] bf16; K and H at most
  * 131071. workspace: tfb200_fused_mlp_int8_workspace_size bytes, 256-byte
  * aligned. */

@@ -6,33 +6,11 @@
 
 namespace tfb200 {
 
-// What a product's epilogue writes: bf16 or fp32 for the caller, or the fused
-// MLP's hidden block (Int8Hidden).
-enum Int8Out : int { kInt8OutBf16 = 0, kInt8OutF32 = 1, kInt8OutHidden = 2 };
+// What a product's epilogue writes. The fused MLP's hidden block is fp32.
+enum Int8Out : int { kInt8OutBf16 = 0, kInt8OutF32 = 1 };
 
 // Longest inner dimension: |sum_k a b| <= 128 * 128 * K must stay in int32.
 constexpr int64_t kInt8MaxK = 131071;
-
-// The hidden block between an MLP's products, which is quantised again per row
-// once the whole row is known: 16-bit integers with the largest magnitude of
-// each 32 columns of a row beside them, h = value * max / 32767. That is as many
-// bytes as bf16 and keeps h to 2^-16 of its neighbourhood: with fp16 (bf16) the
-// second quantisation moved about 0.5 % (2 %) of the values by an int8 step, here
-// under 0.1 %. It holds the whole range of fp32; a block of 32 with an infinity
-// or a NaN has maximum NaN.
-constexpr int kHiddenBlock = 32;
-struct Int8Hidden {
-  int64_t ld = 0, ldm = 0;  // row strides of the values and of the maxima
-  size_t max_at = 0, bytes = 0;
-};
-inline Int8Hidden int8_hidden(int64_t m, int64_t h) {
-  Int8Hidden l;
-  l.ld = (h + 15) / 16 * 16;
-  l.ldm = (h + 127) / 128 * 4;  // four maxima at a time
-  l.max_at = (static_cast<size_t>(m) * l.ld * 2 + 255) / 256 * 256;
-  l.bytes = l.max_at + static_cast<size_t>(m) * l.ldm * 4;
-  return l;
-}
 
 // v = a_scale[m] * b_scale[n] * sum_k A[m,k] B[n,k], then + bias[n], GELU and
 // + residual[m,n] (each optional). A [M,K] and B [N,K] are int8, row-major.
@@ -51,8 +29,6 @@ struct Int8Gemm {
   void* C = nullptr;
   int64_t ldc = 0;
   int out = kInt8OutBf16;
-  float* hidden_max = nullptr;  // kInt8OutHidden: maxima, ldm apart
-  int64_t ldm = 0;
   void* ws = nullptr;            // int8_gemm_ws(M, N, K).total bytes, 256-byte aligned, its counters cleared
   // The kernel that precedes this product in the stream writes neither B nor
   // b_scale (it is this library's own staging launch), so their first tiles may
@@ -70,7 +46,7 @@ struct Int8Gemm {
 struct Int8GemmWs {
   size_t clear_bytes = 0, total = 0;
 };
-Int8GemmWs int8_gemm_ws(int64_t m, int64_t n, int64_t k, bool hidden = false);
+Int8GemmWs int8_gemm_ws(int64_t m, int64_t n, int64_t k);
 int run_int8_gemm(const Int8Gemm& g, cudaStream_t stream, std::string* err);
 
 // Few rows (int8_stream.cu); operands as run_int8_gemm checks them for TMA.
@@ -79,7 +55,7 @@ Int8GemmWs int8_stream_ws(int64_t m, int64_t n);
 int run_int8_stream(const Int8Gemm& g, cudaStream_t stream, std::string* err);
 // A handful of rows (int8_gemv.cu); operands as above, no workspace.
 constexpr int64_t kInt8GemvRows = 32;
-double int8_gemv_us(int64_t m, int64_t n, int64_t k, bool hidden);  // estimate
+double int8_gemv_us(int64_t m, int64_t n, int64_t k);  // estimate
 int run_int8_gemv(const Int8Gemm& g, cudaStream_t stream, std::string* err);
 // Tensor map of an int8 matrix in boxes of 128 columns (int8_gemm.cu).
 bool int8_map(CUtensorMap* m, const int8_t* base, int64_t rows, int64_t cols, int64_t ld, uint32_t box_rows,
@@ -87,7 +63,8 @@ bool int8_map(CUtensorMap* m, const int8_t* base, int64_t rows, int64_t cols, in
 
 // One row at a time: q = rn(t * 127 / amax_k |t|) with t = x (kInt8RowsQuant),
 // t = (x + residual) * gamma with scale = amax / (127 rms) (kInt8RowsNorm), or
-// t = the fused MLP's hidden block (kInt8RowsHidden).
+// t = the fp32 rows of the fused MLP's hidden block (kInt8RowsHidden; they start
+// on 32-byte boundaries).
 enum Int8RowsKind : int { kInt8RowsQuant = 0, kInt8RowsNorm = 1, kInt8RowsHidden = 2 };
 struct Int8Rows {
   int kind = kInt8RowsQuant;
@@ -103,8 +80,6 @@ struct Int8Rows {
   int8_t* q = nullptr;
   int64_t ldq = 0;
   float* scale = nullptr;
-  const float* hidden_max = nullptr;  // kInt8RowsHidden
-  int64_t ldm = 0;
   // Optional: counters of the products that follow, cleared by the same launch
   // (16-byte aligned, a multiple of 16 bytes).
   void* zero = nullptr;

@@ -14,6 +14,7 @@ constexpr size_t kTooBig = ~size_t(0);
 
 size_t al256(size_t b) { return (b + 255) & ~static_cast<size_t>(255); }
 int64_t ld16(int64_t k) { return (k + 15) / 16 * 16; }
+int64_t ld_hidden(int64_t h) { return (h + 7) / 8 * 8; }  // fp32 rows on 32-byte boundaries
 
 int fail(int code, const char* fn, const std::string& msg) {
   set_last_error(std::string(fn) + ": " + msg);
@@ -65,7 +66,7 @@ bool same_shape(const tfb200_mat* a, const tfb200_mat* b) { return a->rows == b-
 const bf16* as_bf16(const void* p) { return static_cast<const bf16*>(p); }
 
 // Workspace of the fused calls: int8 rows and their scales, (MLP: the hidden
-// block, its int8 form and scales), then each product's region, whose
+// block in fp32, its int8 form and scales), then each product's region, whose
 // counters the rows launch ahead of it clears.
 struct Layout {
   size_t q = 0, scale = 0, hidden = 0, hq = 0, hscale = 0, up = 0, down = 0, up_clear = 0, down_clear = 0,
@@ -84,11 +85,11 @@ Layout layout(int64_t m, int64_t k, int64_t h, int64_t n) {
   l.q = take(rows * ld16(k));
   l.scale = take(rows * 4);
   if (h > 0) {
-    l.hidden = take(int8_hidden(m, h).bytes);
+    l.hidden = take(rows * ld_hidden(h) * sizeof(float));
     l.hq = take(rows * ld16(h));
     l.hscale = take(rows * 4);
   }
-  const Int8GemmWs up = int8_gemm_ws(m, h > 0 ? h : n, k, h > 0);
+  const Int8GemmWs up = int8_gemm_ws(m, h > 0 ? h : n, k);
   l.up = take(up.total);
   l.up_clear = up.clear_bytes;
   if (h > 0) {
@@ -337,8 +338,6 @@ int tfb200_fused_mlp_int8(const tfb200_mat* x, const void* gamma, const tfb200_m
     if (const int rc = ws_check(fn, workspace, workspace_bytes, l.total)) return rc;
     char* ws = static_cast<char*>(workspace);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const Int8Hidden hl = int8_hidden(M, H);
-    float* hmax = reinterpret_cast<float*>(ws + l.hidden + hl.max_at);
     // Norm and quantisation of the tokens; the same launch clears the up
     // projection's counters.
     Int8Rows r;
@@ -369,10 +368,8 @@ int tfb200_fused_mlp_int8(const tfb200_mat* x, const void* gamma, const tfb200_m
     up.bias = as_bf16(b1);
     up.gelu = gelu_of(gelu_mode);
     up.C = ws + l.hidden;
-    up.ldc = hl.ld;
-    up.out = kInt8OutHidden;
-    up.hidden_max = hmax;
-    up.ldm = hl.ldm;
+    up.ldc = ld_hidden(H);
+    up.out = kInt8OutF32;
     up.ws = ws + l.up;
     up.b_stable = true;
     up.next_b = static_cast<const int8_t*>(w2->data);
@@ -388,8 +385,6 @@ int tfb200_fused_mlp_int8(const tfb200_mat* x, const void* gamma, const tfb200_m
     hr.K = H;
     hr.x = up.C;
     hr.ldx = up.ldc;
-    hr.hidden_max = hmax;
-    hr.ldm = hl.ldm;
     hr.q = reinterpret_cast<int8_t*>(ws + l.hq);
     hr.ldq = ld16(H);
     hr.scale = reinterpret_cast<float*>(ws + l.hscale);

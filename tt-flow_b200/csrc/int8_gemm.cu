@@ -78,18 +78,14 @@ __global__ void __launch_bounds__(256) k_int8_gemm_any(const int8_t* A, int64_t 
       const int64_t m = m0 + it / (kAnyTile / 8);
       const int c = it % (kAnyTile / 8) * 8;
       const int n = static_cast<int>(n0) + c;
-      const bool in = m < e.M && n < e.N;
+      if (m >= e.M || n >= e.N) continue;
       uint32_t v[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = sums[it / (kAnyTile / 8) * kAnyTile + c + j];
-      float f[8] = {};
-      if (in) int8_values(e, v, e.a_scale[m], int8_cols(e, n, e.vec_cols), f);
-      if (e.out == kInt8OutHidden) {
-        int8_store_hidden(e, m, n, in, f);
-      } else if (in) {
-        if (e.residual) int8_residual(e, m, n, e.vec_res, f);
-        int8_store(e, m, n, e.vec_out, f);
-      }
+      float f[8];
+      int8_values(e, v, e.a_scale[m], int8_cols(e, n, e.vec_cols), f);
+      if (e.residual) int8_residual(e, m, n, e.vec_res, f);
+      int8_store(e, m, n, e.vec_out, f);
     }
     __syncthreads();
   }
@@ -190,8 +186,9 @@ __device__ __forceinline__ void stage16(uint32_t buf, int lane, int u, uint32_t 
 // Barrier of the four epilogue warps that share a half of the tile's columns.
 __device__ __forceinline__ void half_bar(int half) { asm volatile("bar.sync %0, 128;" ::"r"(half + 1) : "memory"); }
 
-// HIDDEN: C is the hidden block of an MLP (Int8Hidden), else bf16 or fp32.
-template <bool HIDDEN, int BN>
+// PLAIN: an fp32 result whose rows lie in 16-byte steps, without a residual, as an
+// MLP's hidden block is (the code of the other forms costs registers).
+template <bool PLAIN, int BN>
 __global__ void __launch_bounds__(cfg::kPairThreads, 1)
     k_int8_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                 const __grid_constant__ CUtensorMap tmC, const PairParams p) {
@@ -375,7 +372,7 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
         const uint16_t bias = p.e.bias && col_in ? reinterpret_cast<const uint16_t*>(p.e.bias)[n] : uint16_t(0);
         if (row_in) {
           sa = p.e.a_scale[row];
-          if (!HIDDEN && p.e.residual)
+          if (!PLAIN && p.e.residual)
             for (int c = c0; c < c0 + kChunks && tn * BN + c * 32 < p.e.N; c += 2)
               prefetch_l2(p.e.residual + row * p.e.ldr + tn * BN + c * 32);
         }
@@ -411,7 +408,6 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
           continue;
         }
       }
-      float hmax[kChunks] = {};
       for (int c = c0; c < c0 + kChunks; ++c) {
         const int col0 = tn * BN + c * 32;
         if (col0 >= p.e.N || row0 >= p.e.M) break;  // warp-uniform: nothing of this block is in the matrix
@@ -421,7 +417,7 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
                      c * 8 * kBM + r;
         uint4 res[4];
         const bool whole = col0 + 32 <= p.e.N;
-        if (!HIDDEN && p.fast && p.e.residual && whole && row_in && !part) {
+        if (!PLAIN && p.fast && p.e.residual && whole && row_in && !part) {
 #pragma unroll
           for (int u = 0; u < 4; ++u)
             res[u] = *reinterpret_cast<const uint4*>(p.e.residual + row * p.e.ldr + col0 + u * 8);
@@ -450,7 +446,8 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
             }
           }
         }
-        const uint32_t buf = bufs + (p.e.out == kInt8OutF32 ? 0u : odd_store * kStageOut);
+        const bool f32 = PLAIN || p.e.out == kInt8OutF32;
+        const uint32_t buf = bufs + (f32 ? 0u : odd_store * kStageOut);
         uint64_t v2[16];  // fp32 pairs
         {
           const ulonglong2* sb = reinterpret_cast<const ulonglong2*>(ctl->sb + c * 32);
@@ -478,7 +475,7 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
         float f[32];
 #pragma unroll
         for (int j = 0; j < 16; ++j) f2_split(v2[j], f[2 * j], f[2 * j + 1]);
-        if (!HIDDEN && !p.fast) {
+        if (!PLAIN && !p.fast) {
           // The residual or C is not laid out in 16-byte steps: the block goes
           // through shared memory (as fp32 in both buffers, unit j ^ row of a row)
           // and is finished row by row, a lane per column.
@@ -506,7 +503,7 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
               if (k0 + k >= rows) break;
               const int64_t at = (row0 + k0 + k) * p.e.ldc + n;
               const float z = __fadd_rn(x[k], y[k]);
-              if (p.e.out == kInt8OutF32)
+              if (f32)
                 static_cast<float*>(p.e.C)[at] = z;
               else
                 static_cast<bf16*>(p.e.C)[at] = __float2bfloat16_rn(z);
@@ -515,7 +512,7 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
           __syncwarp();
           continue;
         }
-        if (!HIDDEN && p.e.residual && row_in) {
+        if (!PLAIN && p.e.residual && row_in) {
           if (whole) {
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
@@ -534,30 +531,13 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
         // The store that used this buffer has read it: 16-bit results, all but the
         // last (which used the other); fp32 results fill both, so all of them.
         if (lane == 0) {
-          if (p.e.out == kInt8OutF32)
+          if (f32)
             bulk_wait_read<0>();
           else
             bulk_wait_read<1>();
         }
         __syncwarp();
-        if (HIDDEN) {
-          float amax = 0.0f;
-#pragma unroll
-          for (int j = 0; j < 32; ++j) amax = max_abs(amax, f[j]);
-          const UpScale us = up_scale(mag(amax), 32767.0f);
-#pragma unroll
-          for (int k = 0; k < kChunks; ++k)
-            if (k == c - c0) hmax[k] = hidden_max(mag(amax));
-          if (us.up != 1.0f) {  // blocks of the smallest fp32 values
-#pragma unroll
-            for (int j = 0; j < 16; ++j) v2[j] = f2_mul(v2[j], f2(us.up, us.up));
-          }
-          const uint64_t r2 = f2(us.r, us.r);
-#pragma unroll
-          for (int u = 0; u < 4; ++u)
-            stage16(buf, lane, u, hidden_pair(v2[u * 4], r2), hidden_pair(v2[u * 4 + 1], r2),
-                    hidden_pair(v2[u * 4 + 2], r2), hidden_pair(v2[u * 4 + 3], r2));
-        } else if (p.e.out == kInt8OutF32) {
+        if (f32) {
           // Two blocks of 32 x 16 fp32 values.
 #pragma unroll
           for (int u = 0; u < 8; ++u)
@@ -574,7 +554,7 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
         __syncwarp();
         if (lane == 0) {
           tma_store_2d(&tmC, buf, col0, static_cast<int32_t>(row0));
-          if (p.e.out == kInt8OutF32 && col0 + 16 < p.e.N)
+          if (f32 && col0 + 16 < p.e.N)
             tma_store_2d(&tmC, buf + kStageOut, col0 + 16, static_cast<int32_t>(row0));
           bulk_commit();
         }
@@ -584,16 +564,6 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
         // One release for the warp's rows (one per chunk cost 1.3 us each).
         __syncwarp();
         if (lane == 0) st_release_gpu(flag, 1);
-      }
-      // The maxima of this warp's columns (a row of them is padded to 128 columns).
-      if (HIDDEN && !part && row_in && tn * BN + c0 * 32 < p.e.N) {
-        float* at = p.e.hidden_max + row * p.e.ldm + tn * (BN / kHiddenBlock) + c0;
-        if constexpr (kChunks == 4)
-          *reinterpret_cast<float4*>(at) = make_float4(hmax[0], hmax[1], hmax[2], hmax[3]);
-        else if constexpr (kChunks == 2)
-          *reinterpret_cast<float2*>(at) = make_float2(hmax[0], hmax[1]);
-        else
-          *at = hmax[0];
       }
       tc_fence_before();
       __syncwarp();
@@ -605,7 +575,7 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
           mbar_arrive_cluster(mapa_shared(te, 0));
       }
     }
-    if (lane == 0 && p.fast) bulk_wait_all();  // staged stores have left shared memory
+    if (lane == 0 && (PLAIN || p.fast)) bulk_wait_all();  // staged stores have left shared memory
   }
   tc_fence_before();
   __syncthreads();
@@ -679,11 +649,11 @@ PairPlan pair_plan(int64_t m, int64_t n, int64_t k) {
 
 using PairKernel = void (*)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const PairParams);
 template <int BN>
-PairKernel pair_kernel(bool hidden) {
-  return hidden ? k_int8_pair<true, BN> : k_int8_pair<false, BN>;
+PairKernel pair_kernel(bool plain) {
+  return plain ? k_int8_pair<true, BN> : k_int8_pair<false, BN>;
 }
-PairKernel pair_kernel(bool hidden, int bn) {
-  return bn == 256 ? pair_kernel<256>(hidden) : bn == 128 ? pair_kernel<128>(hidden) : pair_kernel<64>(hidden);
+PairKernel pair_kernel(bool plain, int bn) {
+  return bn == 256 ? pair_kernel<256>(plain) : bn == 128 ? pair_kernel<128>(plain) : pair_kernel<64>(plain);
 }
 size_t pair_smem(int bn) { return bn == 256 ? pair_smem<256>() : bn == 128 ? pair_smem<128>() : pair_smem<64>(); }
 
@@ -700,8 +670,8 @@ cudaError_t pair_ready(int* pairs) {
   if (*pairs > 0) return cudaSuccess;
   std::lock_guard<std::mutex> lock(mu);
   for (const int bn : {64, 128, 256})
-    for (const bool hidden : {false, true}) {
-      e = cudaFuncSetAttribute(pair_kernel(hidden, bn), cudaFuncAttributeMaxDynamicSharedMemorySize,
+    for (const bool plain : {false, true}) {
+      e = cudaFuncSetAttribute(pair_kernel(plain, bn), cudaFuncAttributeMaxDynamicSharedMemorySize,
                                static_cast<int>(pair_smem(bn)));
       if (e != cudaSuccess) return e;
     }
@@ -746,15 +716,14 @@ int launch_pair(const Int8Gemm& g, cudaStream_t s, std::string* err) {
     return -3;
   if (p.fast && !make_map_box(&tc, g.C, g.M, g.N, g.ldc, static_cast<uint32_t>(64 / esz), 32,
                                    CU_TENSOR_MAP_SWIZZLE_64B, err,
-                                   g.out == kInt8OutF32      ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
-                                   : g.out == kInt8OutHidden ? CU_TENSOR_MAP_DATA_TYPE_UINT16
-                                                             : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                                   g.out == kInt8OutF32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                                        : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
                                    esz))
     return -3;
   p.ps = plan.s;
   if (p.ps.rem > 0 && resident >= kSmPairs) {
     p.flags = static_cast<int*>(g.ws);
-    const size_t clear = int8_gemm_ws(g.M, g.N, g.K, g.out == kInt8OutHidden).clear_bytes;
+    const size_t clear = int8_gemm_ws(g.M, g.N, g.K).clear_bytes;
     p.slots = reinterpret_cast<int32_t*>(static_cast<char*>(g.ws) + clear);
   } else {
     p.ps = sched::plan(p.ps.tiles, p.ps.kblocks, p.ps.tiles < resident ? p.ps.tiles : resident, 0);
@@ -771,7 +740,7 @@ int launch_pair(const Int8Gemm& g, cudaStream_t s, std::string* err) {
   a[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = a;
   cfg.numAttrs = 2;
-  e = cudaLaunchKernelEx(&cfg, pair_kernel(g.out == kInt8OutHidden, plan.bn), ta, tb, tc, p);
+  e = cudaLaunchKernelEx(&cfg, pair_kernel(g.out == kInt8OutF32 && p.fast && !g.residual, plan.bn), ta, tb, tc, p);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) {
     *err = std::string("int8 pair gemm launch: ") + cudaGetErrorString(e);
@@ -802,19 +771,19 @@ bool int8_map(CUtensorMap* m, const int8_t* base, int64_t rows, int64_t cols, in
 // 128 x 4096 x 4096 - / 15.7 / 13.6, 128 x 16384 x 4096 - / 23.3 / 30.8,
 // 128 x 8192 x 28672 - / 50.0 / 53.4.
 enum Kernel { kPair, kStream, kGemv };
-static Kernel kernel_of(int64_t m, int64_t n, int64_t k, bool hidden) {
+static Kernel kernel_of(int64_t m, int64_t n, int64_t k) {
   if (m > kInt8StreamRows) return kPair;
   const double mb = static_cast<double>(n) * static_cast<double>(k) * 1e-6;
   const double stream = 5.6 + 0.075 * static_cast<double>(m) + mb / 6.0;
   const double pair = 2.5 + 0.29 * pair_plan(m, n, k).cost + mb / 12.0;
-  if (m <= kInt8GemvRows && int8_gemv_us(m, n, k, hidden) <= (stream < pair ? stream : pair)) return kGemv;
+  if (m <= kInt8GemvRows && int8_gemv_us(m, n, k) <= (stream < pair ? stream : pair)) return kGemv;
   return stream <= pair ? kStream : kPair;
 }
 
-Int8GemmWs int8_gemm_ws(int64_t m, int64_t n, int64_t k, bool hidden) {
+Int8GemmWs int8_gemm_ws(int64_t m, int64_t n, int64_t k) {
   Int8GemmWs w;
   if (k <= 0 || pair_tiles(m, n, kMaxBN) > (1 << 30)) return w;
-  const Kernel kernel = kernel_of(m, n, k, hidden);
+  const Kernel kernel = kernel_of(m, n, k);
   if (kernel == kGemv) return w;
   if (kernel == kStream) return int8_stream_ws(m, n);
   const sched::PairSched ps = pair_plan(m, n, k).s;
@@ -834,7 +803,7 @@ int run_int8_gemm(const Int8Gemm& g, cudaStream_t stream, std::string* err) {
   // that are multiples of 16 bytes (one row has no stride).
   if (g.K > 0 && al(g.A, 16) && al(g.B, 16) && (g.lda % 16 == 0 || g.M == 1) && (g.ldb % 16 == 0 || g.N == 1) &&
       pair_tiles(g.M, g.N, kMaxBN) <= (1 << 30))
-    switch (kernel_of(g.M, g.N, g.K, g.out == kInt8OutHidden)) {
+    switch (kernel_of(g.M, g.N, g.K)) {
       case kGemv: return run_int8_gemv(g, stream, err);
       case kStream: return run_int8_stream(g, stream, err);
       case kPair: return launch_pair(g, stream, err);

@@ -120,31 +120,23 @@ __device__ __forceinline__ void finish(const Int8Epi& e, Sums<MT, CH, KS>& s, in
     s.bias[threadIdx.x] = col.bias;
   }
   __syncthreads();
-  constexpr int kThreads = (MT * CH / 8 + 31) / 32 * 32;  // whole warps (int8_store_hidden)
-  if (threadIdx.x >= kThreads) return;
   const int m = threadIdx.x / (CH / 8), c = threadIdx.x % (CH / 8) * 8, n = n0 + c;
-  const bool in = m < e.M && n < e.N;
-  float f[8] = {};
-  if (in) {
-    uint32_t v[8] = {};
+  if (m >= e.M || n >= e.N) return;
+  uint32_t v[8] = {};
 #pragma unroll
-    for (int p = 0; p < KS; ++p)
+  for (int p = 0; p < KS; ++p)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] += static_cast<uint32_t>(s.v[p][m][c + j]);
-    Cols8 cols;
+    for (int j = 0; j < 8; ++j) v[j] += static_cast<uint32_t>(s.v[p][m][c + j]);
+  Cols8 cols;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      cols.sb[j] = f2(s.sb[c + 2 * j], s.sb[c + 2 * j + 1]);
-      cols.bias[j] = f2(s.bias[c + 2 * j], s.bias[c + 2 * j + 1]);
-    }
-    int8_values(e, v, e.a_scale[m], cols, f);
+  for (int j = 0; j < 4; ++j) {
+    cols.sb[j] = f2(s.sb[c + 2 * j], s.sb[c + 2 * j + 1]);
+    cols.bias[j] = f2(s.bias[c + 2 * j], s.bias[c + 2 * j + 1]);
   }
-  if (CH == 32 && e.out == kInt8OutHidden) {
-    int8_store_hidden(e, m, n, in, f);
-  } else if (in) {
-    if (e.residual) int8_residual(e, m, n, e.vec_res, f);
-    int8_store(e, m, n, e.vec_out, f);
-  }
+  float f[8];
+  int8_values(e, v, e.a_scale[m], cols, f);
+  if (e.residual) int8_residual(e, m, n, e.vec_res, f);
+  int8_store(e, m, n, e.vec_out, f);
 }
 
 // MT tokens (M rounded up), four channels a warp, KS warps to a channel's K.
@@ -305,9 +297,8 @@ GemvKernel gemv_kernel(int64_t m, bool wide) {
 // leaves too little of a row to each of more blocks than fit at once. us with 8 / 16
 // / 32: 1 x 16384 x 4096 11.9 / 13.5 / 17.3, 8 x 8192 x 28672 39.9 / 41.6 / 41.7,
 // 16 x 4096 x 6144 9.4 / 8.5 / 13.2, 16 x 4096 x 16384 16.4 / 16.0 / 15.1,
-// 1 x 1024 x 16384 7.2 / 5.2 / 4.6. The hidden block needs 32 (its maxima).
-int channels(int64_t n, int64_t k, bool hidden) {
-  if (hidden) return 32;
+// 1 x 1024 x 16384 7.2 / 5.2 / 4.6.
+int channels(int64_t n, int64_t k) {
   if (k > 4096 || n <= 8 * kAtOnce) return 8;
   return n <= 16 * kAtOnce ? 16 : 32;
 }
@@ -316,8 +307,8 @@ int channels(int64_t n, int64_t k, bool hidden) {
 
 // Start and end, then the weights at the rate the kernels reach (for more tokens what
 // L1 delivers of them), or a warp's batches one after the other.
-double int8_gemv_us(int64_t m, int64_t n, int64_t k, bool hidden) {
-  const int ch = channels(n, k, hidden);
+double int8_gemv_us(int64_t m, int64_t n, int64_t k) {
+  const int ch = channels(n, k);
   const int64_t blocks = (n + ch - 1) / ch;
   const int64_t batch = m <= 2 ? 1024 * (kWarps * 4 / ch) : 256 * (kWarps * 8 / ch);  // k values of a step
   const double steps = static_cast<double>((k + batch - 1) / batch * ((blocks + kAtOnce - 1) / kAtOnce));
@@ -327,16 +318,17 @@ double int8_gemv_us(int64_t m, int64_t n, int64_t k, bool hidden) {
 }
 
 // Bytes of the next product's weights that are brought into L2, which fills HBM's
-// pause between the MLP's products. Whole MLP, us, with 0 / 12 / 40 MB:
-// 1 x 4096 x 16384 26.5 / 26.1 / 25.4, 2 x 4096 x 16384 28.9 / 28.1 / 27.0,
-// 1 x 8192 x 28672 74.4 / 74.0 / 74.2, 8 x 8192 x 28672 85.9 / 85.5 / 86.1,
-// 8 x 4096 x 16384 30.2 / 30.3 / 30.6, 8 x 2048 x 8192 15.5 / 15.0 / 14.7,
-// 16 x 4096 x 16384 35.2 / 34.9 / 35.8.
+// pause between the MLP's products. Whole MLP (rows x width x hidden), us, with 0 /
+// 12 / 40 MB, weights rotated: 1 x 4096 x 16384 26.3 / 25.4 / 24.9, 2 x 4096 x 16384
+// 28.9 / 26.6 / 26.6, 1 x 8192 x 28672 71.7 / 71.6 / 72.3, 3 x 4096 x 16384 30.0 / 29.8 /
+// 30.0, 8 x 8192 x 28672 84.0 / 84.0 / 84.0, 8 x 4096 x 16384 30.3 / 30.2 / 30.3, 8 x 2048
+// x 8192 14.2 / 13.8 / 13.5, 16 x 4096 x 16384 34.9 / 34.8 / 36.2, 24 x 4096 x 16384 37.1 /
+// 36.9 / 36.9, 32 x 2048 x 8192 23.7 / 23.4 / 23.2.
 int64_t next_bytes(int64_t m) { return static_cast<int64_t>(m <= 2 ? 40 : 12) << 20; }
 
 int run_int8_gemv(const Int8Gemm& g, cudaStream_t stream, std::string* err) {
   const bool wide = (reinterpret_cast<uintptr_t>(g.B) & 31u) == 0 && (g.ldb % 32 == 0 || g.N == 1);
-  const int ch = channels(g.N, g.K, g.out == kInt8OutHidden);
+  const int ch = channels(g.N, g.K);
   const GemvKernel kernel =
       ch == 8 ? gemv_kernel<8>(g.M, wide) : ch == 16 ? gemv_kernel<16>(g.M, wide) : gemv_kernel<32>(g.M, wide);
   Next next{};

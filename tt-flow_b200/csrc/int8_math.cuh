@@ -18,8 +18,6 @@ struct Int8Epi {
   void* C;
   int64_t ldc;
   int out;
-  float* hidden_max;
-  int64_t ldm;
   // 16-byte accesses: scales and bias; the residual's rows; C's rows.
   bool vec_cols, vec_res, vec_out;
 };
@@ -38,8 +36,6 @@ inline Int8Epi int8_epi(const Int8Gemm& g) {
   e.C = g.C;
   e.ldc = g.ldc;
   e.out = g.out;
-  e.hidden_max = g.hidden_max;
-  e.ldm = g.ldm;
   auto al16 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
   e.vec_cols = al16(g.b_scale) && (!g.bias || al16(g.bias));
   e.vec_res = al16(g.residual) && (g.ldr % 8 == 0 || g.M == 1);
@@ -47,8 +43,8 @@ inline Int8Epi int8_epi(const Int8Gemm& g) {
   return e;
 }
 
-// GELU in fp32, on packed pairs. The int8 hidden block is quantised again right
-// after it, so its error has to stay well under an int8 step of the row's largest
+// GELU in fp32, on packed pairs. The MLP's hidden block is quantised right after
+// it, so its error has to stay well under an int8 step of the row's largest
 // value: the hardware tanh (error 2^-11 of the tanh) moved about 1 % of the
 // hidden values by a step. The tanh form is written with a sigmoid instead,
 //   0.5 x (1 + tanh z) = x / (1 + exp(-2z)),  -2z log2(e) = x (k1 + k2 x^2),
@@ -88,36 +84,18 @@ __device__ __forceinline__ uint32_t mag(float v) { return __float_as_uint(v) & 0
 // of the add's rate).
 __device__ __forceinline__ uint32_t round_bits(float v) { return __float_as_uint(__fadd_rn(v, 12582912.0f)); }
 
-// limit / amax as two factors: the reciprocal leaves fp32 for the smallest amax,
-// which are taken up by a power of two first (exact). {0, 0} for a maximum of
-// zero and for one that is not finite.
+// 127 / amax as two factors: the reciprocal leaves fp32 for the smallest amax,
+// which are taken up by a power of two first (exact). r = 0 for a maximum of zero
+// and for one that is not finite.
 struct UpScale {
   float up, r;
 };
-__device__ __forceinline__ UpScale up_scale(uint32_t amax_bits, float limit) {
+__device__ __forceinline__ UpScale up_scale(uint32_t amax_bits) {
   const float amax = __uint_as_float(amax_bits);
   UpScale s;
   s.up = amax < 1e-30f ? 7.9228163e28f : 1.0f;
-  s.r = amax_bits == 0u || amax_bits >= 0x7F800000u ? 0.0f : __fmul_rn(__frcp_rn(amax * s.up), limit);
+  s.r = amax_bits == 0u || amax_bits >= 0x7F800000u ? 0.0f : __fmul_rn(__frcp_rn(amax * s.up), 127.0f);
   return s;
-}
-
-// The maximum kept for a block of the hidden values (Int8Hidden).
-__device__ __forceinline__ float hidden_max(uint32_t amax_bits) {
-  return __uint_as_float(amax_bits >= 0x7F800000u ? 0x7FC00000u : amax_bits);
-}
-// Two hidden values in a word; r = up_scale(their block's maximum, 32767).r, and
-// h has been taken up by its `up`. (What a block with a NaN maximum holds is not
-// read as values.)
-__device__ __forceinline__ uint32_t hidden_pair(uint64_t h, uint64_t r) {
-  const uint64_t b = f2_add(f2_mul(h, r), f2(12582912.0f, 12582912.0f));
-  return __byte_perm(static_cast<uint32_t>(b), static_cast<uint32_t>(b >> 32), 0x5410);
-}
-// max(a, |b|), NaN if one is.
-__device__ __forceinline__ float max_abs(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
-  return r;
 }
 
 // acc * sa * sb + bias of two columns: the same roundings in every kernel and
@@ -195,30 +173,6 @@ __device__ __forceinline__ void int8_residual(const Int8Epi& e, int64_t m, int n
     for (int j = 0; j < 8; ++j)
       if (n + j < e.N) f[j] = __fadd_rn(f[j], __bfloat162float(r[j]));
   }
-}
-
-// Eight hidden values of row m, columns n .. n + 7 (zeros past the matrix), whose
-// block of 32 lies in four neighbouring lanes; `in`: row and first column are in
-// the matrix. The warp calls it together.
-__device__ __forceinline__ void int8_store_hidden(const Int8Epi& e, int64_t m, int n, bool in, float (&f)[8]) {
-  uint32_t amax = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    if (n + j >= e.N) f[j] = 0.0f;
-    amax = max(amax, mag(f[j]));
-  }
-  amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-  amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-  if (!in) return;
-  const UpScale us = up_scale(amax, 32767.0f);
-  uint32_t w[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    w[j] = hidden_pair(f2_mul(f2(f[2 * j], f[2 * j + 1]), f2(us.up, us.up)), f2(us.r, us.r));
-  // The block's row stride is a multiple of 16 values, so eight at a multiple of
-  // eight stay in the row.
-  *reinterpret_cast<uint4*>(static_cast<int16_t*>(e.C) + m * e.ldc + n) = make_uint4(w[0], w[1], w[2], w[3]);
-  if ((n & (kHiddenBlock - 1)) == 0) e.hidden_max[m * e.ldm + n / kHiddenBlock] = hidden_max(amax);
 }
 
 __device__ __forceinline__ uint4 pack8_bf16(const float (&f)[8]) {

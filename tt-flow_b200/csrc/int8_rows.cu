@@ -12,13 +12,13 @@
 // infinity or a NaN (or whose sum of squares leaves fp32) gives q = 0 and scale
 // NaN, so everything computed from it is NaN.
 //
-// HBM-bound: 2K bytes read and K written per row (4K and 3K with a residual). A
-// row's T threads hold it in registers, so that it is read once and all its
-// loads are in flight together. The arithmetic has to be kept short beside that:
-// values are held as packed fp32 pairs (one f32x2 instruction for two), plain
-// quantisation takes its maximum on the 16-bit words, and the hidden block's
-// comes with it (the first form, which widened every value twice, took 105 us
-// for an 8192 x 16384 hidden block and 86 us for as many bf16 values).
+// HBM-bound: 2K bytes read and K written per row (4K and 3K with a residual; the
+// hidden block is fp32, 4K and K). A row's T threads hold it in registers, so that
+// it is read once and all its loads are in flight together. The arithmetic has to
+// be kept short beside that: values are held as packed fp32 pairs (one f32x2
+// instruction for two), and plain quantisation takes its maximum on the 16-bit
+// words (the first form, which widened every value twice, took 86 us for 8192 x
+// 16384 bf16 values, 58 now).
 #include <algorithm>
 
 #include "int8_math.cuh"
@@ -43,8 +43,6 @@ struct RowsParams {
   int8_t* q;
   int64_t ldq;
   float* scale;
-  const float* hidden_max;
-  int64_t ldm;
   float one;  // 1 (q_pair)
   int ahead;  // prefetch_row
   int64_t span_x, span_r;  // values from the first row's start to the last row's end
@@ -65,16 +63,24 @@ __global__ void __launch_bounds__(256) k_int8_clear(uint4* zero, int64_t n) {
   clear_words(zero, n);
 }
 
+// What a row is read as: bf16, or fp32 (the hidden block).
 template <int KIND>
-__device__ __forceinline__ float in_value(uint32_t bits) {
-  if (KIND == kInt8RowsHidden) return static_cast<float>(static_cast<int16_t>(bits));
-  return __uint_as_float(bits << 16);
-}
-// The two values of a 32-bit word.
-template <int KIND>
-__device__ __forceinline__ uint64_t in_pair(uint32_t w) {
-  if (KIND == kInt8RowsHidden) return f2(in_value<KIND>(w & 0xFFFFu), in_value<KIND>(w >> 16));
-  return f2_from_bf16x2(w);
+struct RowIn {
+  using type = uint16_t;
+};
+template <>
+struct RowIn<kInt8RowsHidden> {
+  using type = float;
+};
+__device__ __forceinline__ float in_value(uint16_t bits) { return __uint_as_float(static_cast<uint32_t>(bits) << 16); }
+__device__ __forceinline__ float in_value(float v) { return v; }
+
+// 32 bytes at a 32-byte boundary, read once.
+__device__ __forceinline__ void load8_f32(const float* p, uint64_t (&v)[4]) {
+  asm volatile("ld.global.L1::no_allocate.v4.b64 {%0, %1, %2, %3}, [%4];"
+               : "=l"(v[0]), "=l"(v[1]), "=l"(v[2]), "=l"(v[3])
+               : "l"(p)
+               : "memory");
 }
 
 // max(a, |b|, |c|), NaN if one is (a is not negative).
@@ -177,7 +183,8 @@ enum Mode : int { kScalar, kVec, kShift };
 // busy while blocks reduce and store.
 constexpr int64_t kAheadBytes = 12 << 20;
 
-__device__ __forceinline__ void prefetch_row(const uint16_t* row, int K) {
+template <typename T>
+__device__ __forceinline__ void prefetch_row(const T* row, int K) {
   const uint64_t lo = (reinterpret_cast<uint64_t>(row) + 15) & ~uint64_t(15);
   const uint64_t hi = reinterpret_cast<uint64_t>(row + K) & ~uint64_t(15);
   if (hi > lo)
@@ -189,7 +196,9 @@ __device__ __forceinline__ void prefetch_row(const uint16_t* row, int K) {
 // PER: values per thread.
 template <int KIND, bool RES, Mode MODE, bool WARP, int PER>
 __global__ void __launch_bounds__(WARP ? 128 : kMaxT,
-                                  !WARP && PER == 32 && MODE == kVec && KIND != kInt8RowsNorm ? 3 : 1)
+                                  !WARP && PER == 32 && MODE == kVec && KIND != kInt8RowsNorm
+                                      ? KIND == kInt8RowsHidden ? 2 : 3
+                                      : 1)
     k_int8_rows(const RowsParams p) {
   // Launched with programmatic serialization: wait for the grid before (it may
   // write x or still read q), then let the next grid start its prologue.
@@ -204,9 +213,10 @@ __global__ void __launch_bounds__(WARP ? 128 : kMaxT,
   const int64_t at = WARP ? static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5) : blockIdx.x;
   const int64_t row = KIND == kInt8RowsHidden ? p.M - 1 - at : at;
   if (WARP && at >= p.M) return;
-  const uint16_t* const x0 = static_cast<const uint16_t*>(p.x);
+  using In = typename RowIn<KIND>::type;
+  const In* const x0 = static_cast<const In*>(p.x);
   const uint16_t* const r0 = reinterpret_cast<const uint16_t*>(p.residual);
-  const uint16_t* x = x0 + row * p.ldx;
+  const In* x = x0 + row * p.ldx;
   const uint16_t* r = RES ? r0 + row * p.ldr : nullptr;
   const uint16_t* g = reinterpret_cast<const uint16_t*>(p.gamma);
   const int K = p.K;
@@ -270,13 +280,22 @@ __global__ void __launch_bounds__(WARP ? 128 : kMaxT,
         w[j] &= (k + 2 * j < K ? 0xFFFFu : 0u) | (k + 2 * j + 1 < K ? 0xFFFF0000u : 0u);
     }
   };
-  uint32_t xw[G][4], rw[RES ? G : 1][4], gw[KIND == kInt8RowsNorm && MODE == kVec ? G : 1][4];
+  uint32_t xw[KIND == kInt8RowsHidden ? 1 : G][4], rw[RES ? G : 1][4];
+  uint32_t gw[KIND == kInt8RowsNorm && MODE == kVec ? G : 1][4];
   uint32_t sums[RES ? G : 1][4];  // bf16(x + residual); kShift: of the granule
-  float hm[KIND == kInt8RowsHidden ? G : 1];
+  uint64_t v[KIND == kInt8RowsQuant ? 1 : G][4];  // t
 #pragma unroll
   for (int i = 0; i < G; ++i) {
     const int k = first(i);
-    if (MODE == kShift) {
+    if constexpr (KIND == kInt8RowsHidden) {
+      if (k + 8 <= K) {
+        load8_f32(x + k, v[i]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          v[i][j] = f2(k + 2 * j < K ? x[k + 2 * j] : 0.0f, k + 2 * j + 1 < K ? x[k + 2 * j + 1] : 0.0f);
+      }
+    } else if constexpr (MODE == kShift) {
       uint32_t xg[4], rg[4];
       load_shifted(x, k, x0, p.span_x, xw[i], xg);
       if (RES) {
@@ -284,7 +303,7 @@ __global__ void __launch_bounds__(WARP ? 128 : kMaxT,
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           float lo, hi;
-          f2_split(f2_add(in_pair<KIND>(xg[j]), in_pair<KIND>(rg[j])), lo, hi);
+          f2_split(f2_add(f2_from_bf16x2(xg[j]), f2_from_bf16x2(rg[j])), lo, hi);
           sums[i][j] = pack_bf16(lo, hi);
         }
       }
@@ -293,14 +312,15 @@ __global__ void __launch_bounds__(WARP ? 128 : kMaxT,
       if (RES) load8(r, k, rw[i]);
     }
     if (KIND == kInt8RowsNorm && MODE == kVec) load8(g, k, gw[MODE == kVec ? i : 0]);
-    // Eight hidden values lie in one block of 32.
-    if (KIND == kInt8RowsHidden) hm[i] = k < K ? p.hidden_max[row * p.ldm + k / kHiddenBlock] : 0.0f;
   }
   RowStat st{0.0f, 0u};
-  uint64_t v[KIND == kInt8RowsNorm ? G : 1][4];  // kInt8RowsNorm: t
-  if (KIND == kInt8RowsHidden) {
+  if constexpr (KIND == kInt8RowsHidden) {
+    float amax = 0.0f;
 #pragma unroll
-    for (int i = 0; i < G; ++i) st.amax = max(st.amax, mag(hm[i]));
+    for (int i = 0; i < G; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) amax = max_abs(amax, v[i][j]);
+    st.amax = mag(amax);
   } else if (KIND == kInt8RowsQuant) {
     uint32_t m = 0;
 #pragma unroll
@@ -319,10 +339,10 @@ __global__ void __launch_bounds__(WARP ? 128 : kMaxT,
         if (MODE != kVec) load8(g, k, gw[0]);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          uint64_t s = in_pair<KIND>(xw[i][j]);
-          if (RES) s = f2_add(s, in_pair<KIND>(rw[RES ? i : 0][j]));
+          uint64_t s = f2_from_bf16x2(xw[i][j]);
+          if (RES) s = f2_add(s, f2_from_bf16x2(rw[RES ? i : 0][j]));
           ss = f2_fma(s, s, ss);
-          v[i][j] = f2_mul(s, in_pair<KIND>(gw[MODE == kVec ? i : 0][j]));
+          v[i][j] = f2_mul(s, f2_from_bf16x2(gw[MODE == kVec ? i : 0][j]));
           amax = max_abs(amax, v[i][j]);
           if (RES && MODE != kShift) {
             float lo, hi;
@@ -358,7 +378,7 @@ __global__ void __launch_bounds__(WARP ? 128 : kMaxT,
     }
   }
   st = checked<KIND>(st);
-  const UpScale u = up_scale(st.amax, 127.0f);  // q = rn(t * u.up * u.r)
+  const UpScale u = up_scale(st.amax);  // q = rn(t * u.up * u.r)
   if (t == 0) p.scale[row] = row_scale<KIND>(p, st);
   int8_t* q = p.q + row * p.ldq;
   const uint64_t rr = f2(u.r, u.r), one = f2(p.one, p.one);
@@ -386,15 +406,9 @@ __global__ void __launch_bounds__(WARP ? 128 : kMaxT,
   // the smallest fp32 values go apart, so that the usual row costs nothing for
   // them.
   auto t_of = [&](int i, int j) {
-    return KIND == kInt8RowsNorm ? v[KIND == kInt8RowsNorm ? i : 0][j] : in_pair<KIND>(xw[i][j]);
+    return KIND == kInt8RowsQuant ? f2_from_bf16x2(xw[i][j]) : v[KIND == kInt8RowsQuant ? 0 : i][j];
   };
-  if (KIND == kInt8RowsHidden) {
-    // A hidden value and its factor: h = value * block, q = rn(value * block * r).
-    quantise([&](int i, int j) {
-      const float hr = hm[KIND == kInt8RowsHidden ? i : 0] * u.up * u.r * (1.0f / 32767.0f);
-      return u.r != 0.0f ? q_pair(t_of(i, j), f2(hr, hr), one) : uint64_t(0);
-    });
-  } else if (u.r != 0.0f && u.up == 1.0f) {
+  if (u.r != 0.0f && u.up == 1.0f) {
     quantise([&](int i, int j) { return q_pair(t_of(i, j), rr, one); });
   } else {
     quantise([&](int i, int j) {
@@ -411,44 +425,35 @@ __global__ void __launch_bounds__(1024) k_int8_rows_long(const RowsParams p) {
   grid_dep_launch();
   clear_words(p.zero, p.zero_vecs);
   const int64_t row = blockIdx.x;
-  const uint16_t* x = static_cast<const uint16_t*>(p.x) + row * p.ldx;
+  const typename RowIn<KIND>::type* x = static_cast<const typename RowIn<KIND>::type*>(p.x) + row * p.ldx;
   const uint16_t* r = RES ? reinterpret_cast<const uint16_t*>(p.residual) + row * p.ldr : nullptr;
   const uint16_t* g = reinterpret_cast<const uint16_t*>(p.gamma);
   auto value = [&](int k) {
-    float s = in_value<KIND>(x[k]);
-    if (RES) s = __fadd_rn(s, in_value<KIND>(r[k]));
+    float s = in_value(x[k]);
+    if (RES) s = __fadd_rn(s, in_value(r[k]));
     return s;
   };
   RowStat st{0.0f, 0u};
-  if (KIND == kInt8RowsHidden) {
-    for (int k = threadIdx.x * kHiddenBlock; k < p.K; k += blockDim.x * kHiddenBlock)
-      st.amax = max(st.amax, mag(p.hidden_max[row * p.ldm + k / kHiddenBlock]));
-  } else {
 #pragma unroll 4
-    for (int k = threadIdx.x; k < p.K; k += blockDim.x) {
-      float s = value(k);
-      if (KIND == kInt8RowsNorm) {
-        st.ss = fmaf(s, s, st.ss);
-        s = __fmul_rn(s, in_value<KIND>(g[k]));
-      }
-      st.amax = max(st.amax, mag(s));
+  for (int k = threadIdx.x; k < p.K; k += blockDim.x) {
+    float s = value(k);
+    if (KIND == kInt8RowsNorm) {
+      st.ss = fmaf(s, s, st.ss);
+      s = __fmul_rn(s, in_value(g[k]));
     }
+    st.amax = max(st.amax, mag(s));
   }
   st = block_stat(st, KIND == kInt8RowsNorm);
   st = checked<KIND>(st);
-  const UpScale u = up_scale(st.amax, 127.0f);  // q = rn(t * u.up * u.r)
+  const UpScale u = up_scale(st.amax);  // q = rn(t * u.up * u.r)
   if (threadIdx.x == 0) p.scale[row] = row_scale<KIND>(p, st);
   // A thread reads a value of x again before it writes the sum, which may be x.
 #pragma unroll 4
   for (int k = threadIdx.x; k < p.K; k += blockDim.x) {
     float s = value(k);
     if (RES) p.sum[row * p.lds + k] = __float2bfloat16_rn(s);
-    if (KIND == kInt8RowsNorm) s = __fmul_rn(s, in_value<KIND>(g[k]));
-    uint32_t b;
-    if (KIND == kInt8RowsHidden)
-      b = round_bits(s * (p.hidden_max[row * p.ldm + k / kHiddenBlock] * u.up * u.r * (1.0f / 32767.0f)));
-    else
-      b = round_bits(__fmul_rn(__fmul_rn(s, u.up), u.r));
+    if (KIND == kInt8RowsNorm) s = __fmul_rn(s, in_value(g[k]));
+    const uint32_t b = round_bits(__fmul_rn(__fmul_rn(s, u.up), u.r));
     p.q[row * p.ldq + k] = u.r == 0.0f ? 0 : static_cast<int8_t>(b & 0xFFu);
   }
 }
@@ -466,7 +471,8 @@ cudaError_t launch_rows(RowsParams p, Mode mode, cudaStream_t s) {
   int T = std::min(kMaxT, std::max(128, (K + 32 * per - 1) / (32 * per) * 32));
   if (warp) T = 128;
   if (longer) T = 1024;
-  p.ahead = static_cast<int>(std::max<int64_t>(148, kAheadBytes / (static_cast<int64_t>(p.K) * (RES ? 4 : 2) + 1)));
+  const int64_t row_bytes = static_cast<int64_t>(p.K) * (RES || hidden ? 4 : 2);
+  p.ahead = static_cast<int>(std::max<int64_t>(148, kAheadBytes / (row_bytes + 1)));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(warp && !longer ? (p.M + 3) / 4 : p.M), 1, 1);
   cfg.blockDim = dim3(static_cast<unsigned>(T), 1, 1);
@@ -538,9 +544,7 @@ int run_int8_rows(const Int8Rows& r, cudaStream_t stream, std::string* err) {
   p.q = r.q;
   p.ldq = r.ldq;
   p.scale = r.scale;
-  p.hidden_max = r.hidden_max;
   p.one = 1.0f;
-  p.ldm = r.ldm;
   p.zero = static_cast<uint4*>(r.zero);
   p.zero_vecs = static_cast<int64_t>(r.zero_bytes / 16);
   const bool norm = r.kind == kInt8RowsNorm, res = norm && r.residual;

@@ -145,27 +145,19 @@ __device__ __forceinline__ void epilogue(const StreamParams& p, Ctl* ctl, const 
     }
     const int32_t* s0 = p.slots + (static_cast<int64_t>(nb) + c_first) * slot_elems + c8;
 #pragma unroll 1
-    for (int it = et; it < p.mpad * (kN / 8); it += kEpiThreads) {
-      const int m = it / (kN / 8);
-      const bool in = m < e.M && n < e.N;
+    for (int m = et / (kN / 8); n < e.N && m < e.M; m += kEpiThreads / (kN / 8)) {
       uint32_t v[8] = {};
-      if (in) {
 #pragma unroll 4
-        for (int c = 0; c <= c_last - c_first; ++c) {
-          const int4* s = reinterpret_cast<const int4*>(s0 + c * slot_elems + m * kN);
-          const int4 a = __ldcg(s), b = __ldcg(s + 1);
-          v[0] += a.x, v[1] += a.y, v[2] += a.z, v[3] += a.w;
-          v[4] += b.x, v[5] += b.y, v[6] += b.z, v[7] += b.w;
-        }
+      for (int c = 0; c <= c_last - c_first; ++c) {
+        const int4* s = reinterpret_cast<const int4*>(s0 + c * slot_elems + m * kN);
+        const int4 a = __ldcg(s), b = __ldcg(s + 1);
+        v[0] += a.x, v[1] += a.y, v[2] += a.z, v[3] += a.w;
+        v[4] += b.x, v[5] += b.y, v[6] += b.z, v[7] += b.w;
       }
-      float f[8] = {};
-      if (in) int8_values(e, v, s_scale[m], cols, f);
-      if (e.out == kInt8OutHidden) {
-        int8_store_hidden(e, m, n, in, f);
-      } else if (in) {
-        if (e.residual) int8_residual(e, m, n, e.vec_res, f);
-        int8_store(e, m, n, e.vec_out, f);
-      }
+      float f[8];
+      int8_values(e, v, s_scale[m], cols, f);
+      if (e.residual) int8_residual(e, m, n, e.vec_res, f);
+      int8_store(e, m, n, e.vec_out, f);
     }
   }
 }

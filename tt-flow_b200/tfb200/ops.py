@@ -535,7 +535,7 @@ def fused_mlp_int8(x: torch.Tensor, gamma: torch.Tensor, w1: torch.Tensor, w1_sc
                    eps: float = 1e-6, gelu: str = "erf", out: torch.Tensor | None = None,
                    workspace: torch.Tensor | None = None) -> torch.Tensor:
     """``fused_mlp`` on int8 ``w1 [H, K]`` and ``w2 [N, H]`` with a scale per row: the normalised rows and the hidden
-    block are quantised per token. ``b1`` is a bf16 ``[H]`` bias or None."""
+    block (fp32 until then) are quantised per token. ``b1`` is a bf16 ``[H]`` bias or None."""
     dev = _first(x, "x")
     xr = _rows(x, "x", _BF16, dev)
     M, K = xr[:2]
