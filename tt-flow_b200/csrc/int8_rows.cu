@@ -22,6 +22,7 @@
 #include <algorithm>
 
 #include "int8_math.cuh"
+#include "int8_rows_span.h"
 
 namespace tfb200 {
 
@@ -45,7 +46,6 @@ struct RowsParams {
   float* scale;
   float one;  // 1 (q_pair)
   int ahead;  // prefetch_row
-  int64_t span_x, span_r;  // values from the first row's start to the last row's end
   uint4* zero;
   int64_t zero_vecs;
 };
@@ -145,7 +145,8 @@ __device__ __forceinline__ RowStat checked(RowStat s) {
 
 // rn of two values in the low bytes of a pair's halves. The product is rounded to
 // fp32 before the integer: bf16 rows hold many values halfway between two steps,
-// and 127 / amax rounded down would take them off the tie. ptxas contracts a
+// and 127 / amax rounded down would take them off the tie (it still takes amax / 2
+// off for 20 of the 128 significands of amax). ptxas contracts a
 // packed product and sum into one rounding, so the sum is a multiply-add by a 1
 // that only the launch knows.
 __device__ __forceinline__ uint64_t q_pair(uint64_t v, uint64_t r, uint64_t one) {
@@ -175,7 +176,7 @@ __device__ __forceinline__ void from_half(const uint32_t (&w)[8], int half, uint
 //   kShift:  8 neighbours at a time; the rows of x, residual and sum start
 //            anywhere, but all three at the same place of their 16-byte granules
 //            (odd widths). A thread reads two neighbouring granules and takes
-//            its 8 values from them; the sum is formed on granules. Single loads
+//            its 8 values from them (at the ends of a padded row value by value); the sum is formed on granules. Single loads
 //            took 7 times as long (8192 x 4099: 117 us against 16).
 enum Mode : int { kScalar, kVec, kShift };
 
@@ -232,6 +233,8 @@ __global__ void __launch_bounds__(WARP ? 128 : kMaxT,
   // kShift: granule i holds values 8i - phase ..
   const int phase = MODE == kShift ? static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15u) / 2) : 0;
 
+  const RowSpan span_x = row_span(row, p.M, K, p.ldx), span_r = row_span(row, p.M, K, p.ldr);
+
   // Plain loads: the sum may be written over x or the residual.
   auto load8 = [&](const uint16_t* src, int k, uint32_t (&w)[4]) {
     if (MODE != kScalar && k + 8 <= K) {
@@ -246,13 +249,13 @@ __global__ void __launch_bounds__(WARP ? 128 : kMaxT,
       }
     }
   };
-  // A granule from value k (k may be negative) of a row of [base, base + span);
-  // one that reaches past the matrix is read value by value.
-  auto granule = [&](const uint16_t* src, int k, const uint16_t* base, int64_t span, uint32_t* w) {
+  // A granule from value k (k may be negative) of a row; one that reaches past
+  // what the row's span allows is read value by value.
+  auto granule = [&](const uint16_t* src, int k, const RowSpan& span, uint32_t* w) {
     const uint16_t* s = src + k;
     if (k >= K) {
       w[0] = w[1] = w[2] = w[3] = 0u;
-    } else if (s >= base && s + 8 <= base + span) {
+    } else if (whole_granule(span, k)) {
       const uint4 v = *reinterpret_cast<const uint4*>(s);
       w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
     } else {
@@ -266,11 +269,10 @@ __global__ void __launch_bounds__(WARP ? 128 : kMaxT,
   };
   // The row's values k .. k + 7 (0 past its end) from its granules; raw gets the
   // first of these.
-  auto load_shifted = [&](const uint16_t* src, int k, const uint16_t* base, int64_t span, uint32_t (&w)[4],
-                          uint32_t (&raw)[4]) {
+  auto load_shifted = [&](const uint16_t* src, int k, const RowSpan& span, uint32_t (&w)[4], uint32_t (&raw)[4]) {
     uint32_t b[8];
-    granule(src, k - phase, base, span, b);
-    granule(src, k - phase + 8, base, span, b + 4);
+    granule(src, k - phase, span, b);
+    granule(src, k - phase + 8, span, b + 4);
 #pragma unroll
     for (int j = 0; j < 4; ++j) raw[j] = b[j];
     from_half(b, phase, w);
@@ -297,9 +299,9 @@ __global__ void __launch_bounds__(WARP ? 128 : kMaxT,
       }
     } else if constexpr (MODE == kShift) {
       uint32_t xg[4], rg[4];
-      load_shifted(x, k, x0, p.span_x, xw[i], xg);
+      load_shifted(x, k, span_x, xw[i], xg);
       if (RES) {
-        load_shifted(r, k, r0, p.span_r, rw[i], rg);
+        load_shifted(r, k, span_r, rw[i], rg);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           float lo, hi;
@@ -561,8 +563,6 @@ int run_int8_rows(const Int8Rows& r, cudaStream_t stream, std::string* err) {
     else if (!res || (same_place(r.residual, r.ldr) && same_place(r.sum, r.lds)))
       mode = kShift;
   }
-  p.span_x = (r.M - 1) * r.ldx + r.K;
-  p.span_r = (r.M - 1) * r.ldr + r.K;
   const cudaError_t e = r.kind == kInt8RowsHidden ? launch_rows<kInt8RowsHidden, false>(p, mode, stream)
                         : !norm                   ? launch_rows<kInt8RowsQuant, false>(p, mode, stream)
                         : res                     ? launch_rows<kInt8RowsNorm, true>(p, mode, stream)
