@@ -227,11 +227,16 @@ int tfb200_fused_mlp_noalloc(const tfb200_mat* x, const void* gamma, const tfb20
  * A row that holds an infinity or a NaN gets scale NaN (and q = 0), so every
  * value computed from it is NaN; the other rows are not touched by it. A row of
  * zeros gets scale 0. RMSNorm's sum of squares is held in fp32: a row where it
- * overflows (values above about 1e18) counts as not finite, and with eps == 0 one
- * whose mean square is 0 there has no norm and gets scale NaN. */
+ * overflows (a root mean square above sqrt(3.4e38 / K), 2.9e17 for K = 4096), or
+ * whose product with gamma does, counts as not finite, and with eps == 0 one whose
+ * mean square is 0 there has no norm and gets scale NaN. */
 
-/* q[m,k] = rn(x[m,k] * 127 / amax), scale[m] = amax / 127, amax = max_k |x[m,k]|,
- * rounding half to even. X [M,K] bf16, Q [M,K] int8, scale [M]. Also lays out
+/* q[m,k] = rn(x[m,k] * r), r = 127 / amax, scale[m] = amax / 127, amax = max_k
+ * |x[m,k]|. In fp32: r = fl(fl(1 / amax) * 127), and q is fl(x * r) rounded to an
+ * integer, halves to even. So q is the integer next to the exact quotient, but a
+ * quotient of exactly 63.5 (|x| = amax / 2) gives 63 or 64 as fl(x * r) falls: 63
+ * for 20 of the 128 significands amax can have (more above amax = 8.5e37, where 1 /
+ * amax is subnormal). X [M,K] bf16, Q [M,K] int8, scale [M]. Also lays out
  * weights: the rows of W^T are its output channels. */
 int tfb200_quantize_int8(const tfb200_mat* x, tfb200_mat* q, float* scale, void* stream);
 

@@ -396,7 +396,8 @@ def _new_int8(shape, rows: int, dev):
 
 def quantize_int8(x: torch.Tensor, out: tuple | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """``(q, scale)``: int8 ``q = round(x * 127 / amax)`` of ``x``'s shape and fp32 ``scale = amax / 127`` of its
-    leading dimensions, ``amax`` the largest magnitude of each row (last dimension), halves to even.
+    leading dimensions, ``amax`` the largest magnitude of each row (last dimension). ``q`` is the fp32 product
+    ``x * ((1 / amax) * 127)`` rounded to an integer, halves of that product to even.
 
     A weight ``w [in, out]`` is laid out for the products once: ``w_q, w_scale = quantize_int8(w.t())``. The rows of
     a returned ``q`` start 16 bytes apart or a multiple of it (its row stride may exceed its width); the products copy
