@@ -24,3 +24,9 @@ def run(tmp_path, name):
 def test_rows_read_only_their_columns(tmp_path):
     """Rows that start anywhere are read in 16-byte granules; padding between rows is not read."""
     assert "OK 34560 layouts" in run(tmp_path, "int8_span_check")
+
+
+def test_pair_schedule(tmp_path):
+    """Tiles, splits and slots of the CTA-pair kernel: every k-block once, waits only on pairs dispatched before."""
+    out = run(tmp_path, "int8_sched_check")
+    assert out.startswith("OK ") and "schedules" in out

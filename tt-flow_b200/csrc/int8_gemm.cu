@@ -15,8 +15,8 @@
 #include <mutex>
 
 #include "int8_math.cuh"
+#include "int8_sched.h"
 #include "kernel_config.h"
-#include "pair_sched.h"
 
 namespace tfb200 {
 
@@ -93,14 +93,13 @@ __global__ void __launch_bounds__(256) k_int8_gemm_any(const int8_t* A, int64_t 
 
 // ------------------------------------------------------------ CTA-pair kernel
 
-constexpr int kBM = 128;                   // rows of A, and rows of B, per CTA
-constexpr int kBK = 128;                   // k values per stage (128 bytes)
+constexpr int kBM = kPairBM;               // rows of A, and rows of B, per CTA
+constexpr int kBK = kPairBK;               // k values per stage (128 bytes)
 constexpr uint32_t kABytes = kBM * kBK;    // A's share of a stage: 16 KiB
 constexpr int kEpiWarps = cfg::kPairEpiWarps;
 constexpr uint32_t kStageOut = 32 * 64;    // one staged block: 32 rows of 64 bytes
 constexpr int kGroup = cfg::kGroupM;       // row tiles per raster group
-constexpr int kSmPairs = 74;               // CTA pairs of a B200
-constexpr int kMaxBN = 256, kMaxStages = 9;
+constexpr int kMaxStages = 9;
 
 template <int BN>
 struct Geo {
@@ -150,24 +149,6 @@ __device__ __forceinline__ void tile_of(int t, int num_m, int num_n, int& tm, in
   const int local = t - g * per_group;
   tm = g * kGroup + local % rows;
   tn = local / rows;
-}
-
-// Work item i of a pair: the full waves' tiles, then one piece of the split last
-// wave. The last `rem` pairs keep k-blocks [0, kc) of its tiles and finish them;
-// of the pairs before them, pair g takes part g (tile g / parts).
-struct Work {
-  int tile, k0, k1, role, slot;
-};
-__device__ __forceinline__ int item_count(const sched::PairSched& s, int p) {
-  if (s.rem == 0) return p < s.tiles ? (s.tiles - 1 - p) / s.pairs + 1 : 0;
-  return s.waves + (p >= s.pairs - s.rem || p < s.rem * s.parts ? 1 : 0);
-}
-__device__ __forceinline__ Work item_at(const sched::PairSched& s, int p, int i) {
-  if (s.rem == 0 || i < s.waves) return {p + i * s.pairs, 0, s.kblocks, sched::kFull, 0};
-  const int base = s.waves * s.pairs, r = p - (s.pairs - s.rem);
-  if (r >= 0) return {base + r, 0, s.kc, sched::kMain, r * s.parts};
-  const int j = p % s.parts, tail = s.kblocks - s.kc;
-  return {base + p / s.parts, s.kc + tail * j / s.parts, s.kc + tail * (j + 1) / s.parts, sched::kPart, p};
 }
 
 __device__ __forceinline__ void give_up(PairCtl* ctl, int* status) {
@@ -250,7 +231,7 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
       // that kernel does not write it either.
       int npre = 0;
       if (p.b_prefetch && nwork > 0) {
-        const Work w = item_at(ps, pair, 0);
+        const PairWork w = item_at(ps, pair, 0);
         int tm, tn;
         tile_of(w.tile, num_m, num_n, tm, tn);
         npre = min(kStages, w.k1 - w.k0);
@@ -263,7 +244,7 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
       }
       if (!p.a_early) grid_dep_wait();
       for (int i = 0; i < nwork && ok; ++i) {
-        const Work w = item_at(ps, pair, i);
+        const PairWork w = item_at(ps, pair, i);
         int tm, tn;
         tile_of(w.tile, num_m, num_n, tm, tn);
         for (int kb = w.k0; kb < w.k1; ++kb) {
@@ -302,7 +283,7 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
       uint32_t phase = 0;
       bool ok = true;
       for (int i = 0; i < nwork && ok; ++i) {
-        const Work w = item_at(ps, pair, i);
+        const PairWork w = item_at(ps, pair, i);
         const int acc = i & 1;
         const uint32_t use = static_cast<uint32_t>(i >> 1);
         if (!mbar_wait(smem_u32(&ctl->tempty[acc]), (use & 1u) ^ 1u, &ctl->abort, p.timeout_ns)) {
@@ -353,7 +334,7 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
     // a 64-column tile, or where the matrix ends).
     uint32_t odd_store = 0;
     for (int i = 0; i < nwork; ++i) {
-      const Work w = item_at(ps, pair, i);
+      const PairWork w = item_at(ps, pair, i);
       int tm, tn;
       tile_of(w.tile, num_m, num_n, tm, tn);
       const int acc = i & 1;
@@ -587,65 +568,6 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
 }
 
 bool al(const void* p, unsigned b) { return (reinterpret_cast<uintptr_t>(p) & (b - 1)) == 0; }
-
-int64_t pair_tiles(int64_t m, int64_t n, int bn) { return (m + 2 * kBM - 1) / (2 * kBM) * ((n + bn - 1) / bn); }
-
-struct PairPlan {
-  int bn = kMaxBN;
-  sched::PairSched s;
-  double cost = 0.0;  // k-blocks
-};
-
-// The tile width and schedule over all the pairs of a B200, by an estimate in
-// k-blocks of a 256-wide tile (0.3 us). A narrower tile's k-block is hardly
-// shorter (A's share of a stage stays, and comes out of L2 for every pair), but
-// its epilogue is, so narrow tiles pay where the wide ones leave pairs idle in a
-// single short wave; measured, us with 256 / 128 / 64 columns: 256 x 4096 x 4096
-// 16.2 / 14.6 / 13.9, 512 x 4096 x 4096 16.5 / 15.5 / 22.5, 200 x 512 x 2048 7.3 /
-// 5.7 / 4.8, 1024 x 4096 x 4096 17.7 / 24.8 / 40.0.
-// A last wave of R < 74 wide tiles is split when that shortens it: each of its
-// tiles keeps k-blocks [0, kc) on one pair, and S parts of the rest go to idle
-// pairs, one each. A split costs kSplitCost (writing and handing over the sums,
-// clearing the flags) and kReadCost per part, which the finishing pair reads.
-// Measured, us without a split / with 1 / 2 / 3 parts: 256 x 16384 x 4096 42.6 /
-// 34.5 / 31.8 / 32.3, 1200 x 16384 x 4096 79.8 / 72.0 / 67.8 / 66.8, and where it
-// does not pay, 256 x 4096 x 4096 16.1 / 20.2 / 20.9 / 22.6.
-constexpr int kSplitCost = 30, kReadCost = 8;
-PairPlan pair_plan(int64_t m, int64_t n, int64_t k) {
-  const int kb = static_cast<int>((k + kBK - 1) / kBK);
-  PairPlan best;
-  for (const int bn : {256, 128, 64}) {
-    const int64_t tiles = pair_tiles(m, n, bn);
-    if (bn < kMaxBN && tiles > 4 * kSmPairs) break;
-    const double block = bn == 256 ? 1.0 : bn == 128 ? 0.96 : 0.92, fixed = bn == 256 ? 10.0 : bn == 128 ? 6.0 : 4.0;
-    const double cost = static_cast<double>((tiles + kSmPairs - 1) / kSmPairs) * kb * block + fixed;
-    if (bn == kMaxBN || cost < best.cost) {
-      best.cost = cost;
-      best.bn = bn;
-      best.s = sched::PairSched();
-      best.s.tiles = static_cast<int>(tiles);
-      best.s.kblocks = kb;
-      best.s.pairs = kSmPairs;
-    }
-    if (bn < kMaxBN) continue;
-    const int rem = best.s.tiles % kSmPairs, idle = kSmPairs - rem;
-    for (int parts = 1; rem > 0 && parts <= sched::kMaxParts && rem * parts <= idle; ++parts) {
-      // Equal pieces: kc = ceil(KB / (parts + 1)), the parts share the rest.
-      const int kc = (kb + parts) / (parts + 1);
-      if (kb - kc < parts) break;
-      const double split =
-          static_cast<double>(best.s.tiles / kSmPairs) * kb + kc + kSplitCost + kReadCost * parts + fixed;
-      if (split < best.cost) {
-        best.cost = split;
-        best.s.waves = best.s.tiles / kSmPairs;
-        best.s.rem = rem;
-        best.s.parts = parts;
-        best.s.kc = kc;
-      }
-    }
-  }
-  return best;
-}
 
 using PairKernel = void (*)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const PairParams);
 template <int BN>
