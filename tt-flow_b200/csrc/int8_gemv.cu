@@ -293,14 +293,31 @@ GemvKernel gemv_kernel(int64_t m, bool wide) {
   return wide ? k_int8_gemv_mma<32, CH, true> : k_int8_gemv_mma<32, CH, false>;
 }
 
-// Channels a block: eight, the warps sharing K as widely as they can, unless that
-// leaves too little of a row to each of more blocks than fit at once. us with 8 / 16
-// / 32: 1 x 16384 x 4096 11.9 / 13.5 / 17.3, 8 x 8192 x 28672 39.9 / 41.6 / 41.7,
-// 16 x 4096 x 6144 9.4 / 8.5 / 13.2, 16 x 4096 x 16384 16.4 / 16.0 / 15.1,
-// 1 x 1024 x 16384 7.2 / 5.2 / 4.6.
-int channels(int64_t n, int64_t k) {
-  if (k > 4096 || n <= 8 * kAtOnce) return 8;
-  return n <= 16 * kAtOnce ? 16 : 32;
+// Batches of weights that a warp reads one after the other, times the rounds in which
+// the blocks fit the GPU. A warp holds 4 (8) channels for up to two (more) tokens, so
+// 32 / CH (64 / CH) warps of a block share a channel's K, 1024 (256) values a batch.
+int64_t steps(int64_t m, int64_t n, int64_t k, int ch) {
+  const int64_t blocks = (n + ch - 1) / ch;
+  const int64_t batch = m <= 2 ? 1024 * (kWarps * 4 / ch) : 256 * (kWarps * 8 / ch);
+  return (k + batch - 1) / batch * ((blocks + kAtOnce - 1) / kAtOnce);
+}
+
+// Channels a block. Long rows (K >= 8192) and few channels: eight, the warps sharing K
+// as widely as they can. Otherwise the fewest that fit the GPU at once, so that a
+// block's warps share less of K, or fewer yet where that takes fewer steps. us with 8 /
+// 16 / 32, weights rotated: 1 x 16384 x 8192 20.8 / 21.5 / 21.9, 8 x 8192 x 28672 39.9 /
+// 41.6 / 41.7; 1 x 6144 x 5120 8.0 / 7.3 / 7.6, 16 x 6144 x 4096 9.6 / 8.5 / 12.9,
+// 16 x 6144 x 5120 11.8 / 10.0 / 15.4; 1 x 16384 x 1024 7.2 / 5.2 / 4.6, 16 x 16384 x
+// 4096 17.4 / 16.3 / 15.3, 1 x 16384 x 5120 16.1 / 14.8 / 14.0; with more channels than
+// fit at once, 16 x 20480 x 4096 20.9 / - / 26.3, 16 x 24576 x 5120 29.3 / 26.7 / -, and
+// where the steps mislead, 8 x 28672 x 2048 13.4 / - / 12.9, 2 x 28672 x 6144 30.4 / - /
+// 31.6.
+int channels(int64_t m, int64_t n, int64_t k) {
+  if (k >= 8192 || n <= 8 * kAtOnce) return 8;
+  int best = n <= 16 * kAtOnce ? 16 : 32;
+  for (int ch = best / 2; ch >= 8; ch /= 2)
+    if (steps(m, n, k, ch) < steps(m, n, k, best)) best = ch;
+  return best;
 }
 
 }  // namespace
@@ -308,13 +325,10 @@ int channels(int64_t n, int64_t k) {
 // Start and end, then the weights at the rate the kernels reach (for more tokens what
 // L1 delivers of them), or a warp's batches one after the other.
 double int8_gemv_us(int64_t m, int64_t n, int64_t k) {
-  const int ch = channels(n, k);
-  const int64_t blocks = (n + ch - 1) / ch;
-  const int64_t batch = m <= 2 ? 1024 * (kWarps * 4 / ch) : 256 * (kWarps * 8 / ch);  // k values of a step
-  const double steps = static_cast<double>((k + batch - 1) / batch * ((blocks + kAtOnce - 1) / kAtOnce));
+  const double few = static_cast<double>(steps(m, n, k, channels(m, n, k)));
   const double rate = m <= 2 ? 6.7 : m <= 8 ? 5.9 : m <= 16 ? 5.0 : 2.4;  // TB/s
   const double stream = static_cast<double>(n) * static_cast<double>(k) * 1e-6 / rate;
-  return (m <= 16 ? 1.2 : 2.2) + (stream > 0.7 * steps ? stream : 0.7 * steps);
+  return (m <= 16 ? 1.2 : 2.2) + (stream > 0.7 * few ? stream : 0.7 * few);
 }
 
 // Bytes of the next product's weights that are brought into L2, which fills HBM's
@@ -328,7 +342,7 @@ int64_t next_bytes(int64_t m) { return static_cast<int64_t>(m <= 2 ? 40 : 12) <<
 
 int run_int8_gemv(const Int8Gemm& g, cudaStream_t stream, std::string* err) {
   const bool wide = (reinterpret_cast<uintptr_t>(g.B) & 31u) == 0 && (g.ldb % 32 == 0 || g.N == 1);
-  const int ch = channels(g.N, g.K);
+  const int ch = channels(g.M, g.N, g.K);
   const GemvKernel kernel =
       ch == 8 ? gemv_kernel<8>(g.M, wide) : ch == 16 ? gemv_kernel<16>(g.M, wide) : gemv_kernel<32>(g.M, wide);
   Next next{};
