@@ -22,7 +22,8 @@ namespace tfb200 {
 
 namespace {
 
-// Any alignment: 64 x 64 tiles, 64 k values a step in shared memory, dp4a.
+// Any alignment: 64 x 64 tiles, 64 k values a step in shared memory, dp4a (1024 x 4096 x
+// 4096 706 us, 17 in the layout TMA reads).
 constexpr int kAnyTile = 64, kAnyK = 64;
 
 __device__ __forceinline__ uint32_t load4(const int8_t* p, int k, int K) {
