@@ -251,8 +251,9 @@ int tfb200_rmsnorm_int8(const tfb200_mat* x, const tfb200_mat* residual, const v
  * A [M,K] and B [N,K] int8, a_scale [M], b_scale [N], bias [N] bf16 or NULL,
  * gelu_mode any of enum tfb200_gelu, residual [M,N] bf16 or NULL, C [M,N] bf16 or
  * fp32. The sums are exact in int32, which bounds K to 131071
- * (TFB200_EUNSUPPORTED above); scales, bias, GELU and residual are applied in
- * fp32 and rounded once. K == 0 gives gelu(bias) + R. C may be R. Equal calls
+ * (TFB200_EUNSUPPORTED above); a sum is then rounded to fp32 (above 2^24 it may
+ * not be exact there), scales, bias, GELU and residual are applied in fp32, and the
+ * result is rounded to C's type. K == 0 gives gelu(bias) + R. C may be R. Equal calls
  * give equal bits. workspace: tfb200_matmul_int8_workspace_size bytes, 256-byte aligned. */
 size_t tfb200_matmul_int8_workspace_size(int64_t m, int64_t k, int64_t n);
 int tfb200_matmul_int8(const tfb200_mat* a, const float* a_scale, const tfb200_mat* b, const float* b_scale,

@@ -471,8 +471,8 @@ def matmul_int8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale
                 out_dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None,
                 workspace: torch.Tensor | None = None) -> torch.Tensor:
     """``gelu((a * a_scale) @ (b * b_scale).T + bias) + residual`` of int8 ``a [..., K]`` and ``b [N, K]``, one scale
-    per row of each; exact integer sums, the rest in fp32, rounded once to ``out_dtype`` (bf16 or fp32). ``bias`` is
-    bf16 ``[N]``, ``gelu`` "erf", "tanh" or None, ``residual`` bf16 ``[..., N]``. K is at most 131071.
+    per row of each; exact integer sums, the rest in fp32 steps, the result rounded to ``out_dtype`` (bf16 or fp32).
+    ``bias`` is bf16 ``[N]``, ``gelu`` "erf", "tanh" or None, ``residual`` bf16 ``[..., N]``. K is at most 131071.
     """
     dev = _first(a, "a")
     ar = _rows_int8(a, "a", dev)
