@@ -694,9 +694,6 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
     const int ew = warp - 4;                 // epilogue warp 0 .. PEPI-1
     const int c0 = (ew >> 2) * PCHUNKS;      // first of this warp's 32-column chunks
     const int r = q * 32 + lane;
-    // The warp's stores take its two staging buffers in turn, counted over all its
-    // tiles: a last column tile may end after an odd number of chunks.
-    uint32_t odd_store = 0;
     for (int i = 0; i < nwork; ++i) {
       const sched::Work w = sched::work_item(ps, pair, i);
       int tm, tn;
@@ -807,9 +804,16 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
 #pragma unroll
           for (int j = 0; j < 32; ++j) f[j] = 0.0f;
         }
-        if (lane == 0) bulk_wait_read<1>();  // the store that used this buffer has read it
+        // The store that used this buffer has read it. Within a tile that is the last
+        // but one; the tile before may have ended on either buffer.
+        if (lane == 0) {
+          if (c == c0)
+            bulk_wait_read<0>();
+          else
+            bulk_wait_read<1>();
+        }
         __syncwarp();
-        const uint32_t buf = smem_u32(sC) + (static_cast<uint32_t>(ew * 2) + odd_store) * C_STAGE_BYTES;
+        const uint32_t buf = smem_u32(sC) + static_cast<uint32_t>((ew * 2 + (c & 1)) * C_STAGE_BYTES);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           const uint32_t a = buf + static_cast<uint32_t>(lane * 64 + ((u ^ ((lane >> 1) & 3)) << 4));
@@ -824,7 +828,6 @@ __global__ void __launch_bounds__(cfg::kPairThreads, 1)
           tma_store_2d(&tmC, buf, col0, static_cast<int32_t>(row0));
           bulk_commit();
         }
-        odd_store ^= 1u;
       }
       if (!fix_ok) break;
       if (fix) {

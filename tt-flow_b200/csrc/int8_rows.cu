@@ -177,8 +177,9 @@ __device__ __forceinline__ void from_half(const uint32_t (&w)[8], int half, uint
 //            anywhere, but all three at the same place of their 16-byte granules
 //            (odd widths). A thread reads two neighbouring granules and takes
 //            its 8 values from them (at the ends of a padded row value by value,
-//            int8_rows_span.h); the sum is formed on granules. Single loads took
-//            7 times as long (8192 x 4099: 117 us against 16).
+//            int8_rows_span.h: 32735 x 1001 30 us padded, 26.5 read across the
+//            padding; 7994 x 4099 30, 28); the sum is formed on granules. Single
+//            loads took 7 times as long (8192 x 4099: 117 us against 16).
 enum Mode : int { kScalar, kVec, kShift };
 
 // Rows ahead that are brought into L2: about 12 MB of them, so that HBM is kept
